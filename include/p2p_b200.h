@@ -325,6 +325,82 @@ int p2p_peer_push(const void* y, void* const* peers, int n_peers, int64_t tokens
 int p2p_peer_status(int reset, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------
+ * (2d) 4-bit weights with group scales: W[r, c] = (code[r, c] - zero[r, g]) * scale[r, g], g = c / group, the groups
+ * 32, 64 or 128 columns, code in 0..15, scales in the weights' dtype (bf16 or f16), zero 8 where no zero points are
+ * given. No counterpart in the reference, which keeps 16 bits a kept weight.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* Codes [rows, ceil(cols / 2)] (the even column in the low half of a byte), scales [rows, ceil(cols / group)] and, if
+ * zeros is not null, zero points of the same shape, of w [rows, cols] (row stride ldw). Without zero points a group's
+ * scale is dtype(max |w| / 7); with them dtype((max(w, 0) - min(w, 0)) / 15) and the zero point round(-min(w, 0) /
+ * scale). code = clamp(round(w / scale) + zero, 0, 15), halves to even; a group whose scale is 0 holds zeros, one with
+ * a NaN becomes NaN. */
+int p2p_int4_quantize(const void* w, int dtype, int64_t rows, int64_t cols, int64_t ldw, int group, uint8_t* codes,
+                      void* scales, uint8_t* zeros, void* stream);
+
+/* dense [rows, cols] = dtype((code - zero) * scale), contiguous. */
+int p2p_int4_expand(const uint8_t* codes, const void* scales, const uint8_t* zeros, int dtype, int64_t rows,
+                    int64_t cols, int group, void* dense, void* stream);
+
+/* Row blocks (16 rows) of one expert in the layout: ceil(rows / 16), of a gated module 2 ceil(rows / 2 / 16); -1 for
+ * rows below zero or an odd gated count. */
+int64_t p2p_int4_row_blocks(int64_t rows, int gated);
+
+/* Codes, scales and zero points (contiguous, [experts, rows, ..]) into the layout that the products read: words of
+ * experts x row blocks x ceil(cols / 64) x 512 bytes (16-byte aligned), out_scales and out_zeros of experts x row
+ * blocks x ceil(cols / group) x 16. gated: the first half of an expert's rows is the gate, the second the up
+ * projection. Load time; synchronise before the layout is used. */
+int p2p_int4_layout(const uint8_t* codes, const void* scales, const uint8_t* zeros, int64_t experts, int64_t rows,
+                    int64_t cols, int group, int gated, void* words, void* out_scales, uint8_t* out_zeros,
+                    void* stream);
+
+/* y [tokens, rows] = x [tokens, cols] W^T of a module in the layout; gated: y [tokens, rows / 2] =
+ * dtype(silu(gate) * up), from the fp32 sums. Each group's sum of exact code differences is multiplied by its scale in
+ * fp32; no weight is rounded. Any tokens, rows and cols. As the other GEMMs, a programmatic dependent of the stream's
+ * previous kernel that reads its weights before that kernel completes. */
+int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* words,
+                const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated, void* y, int64_t ldy,
+                void* stream);
+
+/* The same for routed experts: y [pairs, rows] (gated: rows / 2), row p being x's row times the weights of the expert
+ * whose item holds place p. items, n_items: p2p_moe_sort's, of at most max_tokens <= 32 places each; order and topk:
+ * x's row of place p is order[p] / topk (order null: p itself). routed: null, or the number of routed pairs on the
+ * device: rows from there to `pairs` become zero (null: they stay as they were). */
+int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* words, const void* scales,
+                     const uint8_t* zeros, int64_t rows, int group, int gated, const int32_t* items,
+                     const int32_t* n_items, int64_t max_items, int64_t max_tokens, const int32_t* order, int topk,
+                     const int32_t* routed, int64_t pairs, void* y, int64_t ldy, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * (2e) Tokens sorted by expert and back, all on the device (p2p_moe_route's counts go to the host)
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* ids [n_pairs] (32- or 64-bit: ids_bytes) of (token, slot) pairs; an id outside 0..experts - 1 is routed nowhere.
+ * order [n_pairs]: the routed pairs sorted by expert, those of one expert in their own order, then -1; where
+ * [n_pairs]: each pair's place in it, or -1; offsets [experts + 1]: each expert's first place, the last one the number
+ * of routed pairs; items [max_items, 4]: {expert, first place, places, 0}, runs of at most item_tokens places of one
+ * expert, and n_items [1] their number. max_items >= min(n_pairs, ceil(n_pairs / item_tokens) + experts); at most 1024
+ * experts. One launch, deterministic. */
+int p2p_moe_sort(const void* ids, int ids_bytes, int64_t n_pairs, int experts, int32_t* order, int32_t* where,
+                 int32_t* offsets, int32_t* items, int64_t max_items, int item_tokens, int32_t* n_items, void* stream);
+
+/* out [tokens * k, hidden]: row where[t * k + j] = x[t] for every routed pair; rows from *routed (offsets[experts]) on
+ * are zero. dtype bf16, f16 or f32. */
+int p2p_moe_spread(const void* x, int dtype, int64_t tokens, int k, int64_t hidden, int64_t ldx, const int32_t* where,
+                   const int32_t* routed, void* out, int64_t ldo, void* stream);
+
+/* out[t] = dtype(sum over slots j in order of w[t, j] * float(y[where[t * k + j]])), fp32 sums; pairs routed nowhere
+ * add nothing. weights of weights_dtype, or null: 1 (the gradient of the spread). */
+int p2p_moe_sum(const void* y, int dtype, int64_t tokens, int k, int64_t hidden, int64_t ldy, const int32_t* where,
+                const void* weights, int weights_dtype, void* out, int64_t ldo, void* stream);
+
+/* The gradients of p2p_moe_sum: dy[where[t * k + j]] = dtype(w[t, j] * dout[t]), rows from *routed on zero, and
+ * dweights[t, j] = <dout[t], y[where[t * k + j]]> (fp32, 0 for a pair routed nowhere) in weights_dtype. */
+int p2p_moe_sum_back(const void* dout, const void* y, int dtype, int64_t tokens, int k, int64_t hidden, int64_t ldd,
+                     int64_t ldy, const int32_t* where, const int32_t* routed, const void* weights, int weights_dtype,
+                     void* dy, int64_t lddy, void* dweights, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
  * (3) Group combine epilogue
  * ------------------------------------------------------------------------------------------------------------------ */
 

@@ -36,14 +36,14 @@ def stale() -> bool:
     return any(os.path.getmtime(p) > built for p in DEPS)
 
 
-OPS_SRC = os.path.join(HERE, "torch_ops", "ops.cpp")
+OPS_SRCS = sorted(glob.glob(os.path.join(HERE, "torch_ops", "*.cpp")))
 OPS_LIB = os.path.join(HERE, "libp2p_torch_ops.so")
 
 
 def build_ops(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the torch custom operators (torch_ops/ops.cpp, TORCH_LIBRARY p2p_b200) over the C ABI into
+    """Compiles the torch custom operators (torch_ops/*.cpp, TORCH_LIBRARY p2p_b200) over the C ABI into
     libp2p_torch_ops.so. It leaves the p2p_* symbols undefined: _lib loads libp2p_b200.so into the global scope first."""
-    deps = [OPS_SRC, os.path.join(ROOT, "include", "p2p_b200.h")]
+    deps = [*OPS_SRCS, *glob.glob(os.path.join(HERE, "torch_ops", "*.h")), os.path.join(ROOT, "include", "p2p_b200.h")]
     if not force and os.path.exists(OPS_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(OPS_LIB) for d in deps):
         return OPS_LIB
     import torch
@@ -52,11 +52,11 @@ def build_ops(force: bool = False, verbose: bool = False) -> str:
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in cpp_extension.include_paths()], f"-I{os.path.join(cuda_home, 'include')}",
-           f"-I{os.path.join(ROOT, 'include')}", OPS_SRC, f"-L{torch_lib}", "-lc10", "-ltorch_cpu", "-ltorch",
+           f"-I{os.path.join(ROOT, 'include')}", *OPS_SRCS, f"-L{torch_lib}", "-lc10", "-ltorch_cpu", "-ltorch",
            "-lc10_cuda", f"-Wl,-rpath,{torch_lib}", "-o", OPS_LIB + ".tmp"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
-        raise RuntimeError(f"g++ failed on torch_ops/ops.cpp:\n{r.stderr[-6000:]}")
+        raise RuntimeError(f"g++ failed on torch_ops/*.cpp:\n{r.stderr[-6000:]}")
     if verbose:
         sys.stderr.write(r.stderr)
     os.replace(OPS_LIB + ".tmp", OPS_LIB)

@@ -10,6 +10,7 @@ Block list (p2p/compact.py:88-97, prepare.py:201-203), in row order:
     ("dense", W [rows, cols])                                  kept whole
     ("sparse", values [rows, k], words [rows, ceil(cols/32)], cols)   the reference's packed form
     ("compact", values [rows, k], idx [rows, k], cols)          this package's form (values + column indices)
+    ("int4", codes, scales, zeros, cols, group)                 whole rows in 4 bits with group scales (int4.py)
 each with an optional leading expert dimension for routed experts.
 """
 from __future__ import annotations
@@ -18,7 +19,7 @@ import os
 
 import torch
 
-from . import kernels
+from . import int4, kernels
 from ._lib import P2PError, idx_dtype
 
 __all__ = ["pack", "unpack", "expand", "to_compact", "Tiles", "GatedTiles", "Compact", "CompactMoE"]
@@ -41,6 +42,8 @@ def unpack(values: torch.Tensor, words: torch.Tensor, cols: int) -> torch.Tensor
 
 
 def _cols(block: tuple) -> int:
+    if block[0] == "int4":
+        return block[4]
     return block[3] if block[0] in ("sparse", "compact") else block[1].shape[-1]
 
 
@@ -49,6 +52,8 @@ def expand(block: tuple, experts=None) -> torch.Tensor:
     `experts` (ids), if given. p2p/compact.py:88-97."""
     if block[0] == "dense":
         return block[1] if experts is None else block[1][experts]
+    if block[0] == "int4":
+        return int4.expand(block, experts)
     kind, values, meta, cols = block
     if experts is not None:
         values, meta = values[experts], meta[experts]
@@ -64,6 +69,8 @@ def to_compact(block: tuple) -> tuple:
     checking that every row keeps k); column indices are range-checked once here, so the GEMMs need not."""
     if block[0] == "dense":
         return block
+    if block[0] == "int4":
+        raise P2PError("4-bit blocks make up a whole module, in the layout \"int4\"")
     kind, values, meta, cols = block
     if kind == "sparse":
         k = values.shape[-1]
@@ -83,18 +90,24 @@ class Tiles:
     """A module's row blocks on the GPU, as the compact GEMM reads them; calling it multiplies tokens by them.
     The B200 counterpart of p2p/compact.py:113-202 (Tiles). bf16 / f16 modules whose columns are a multiple of 8 are
     re-laid once into (128-row x 64-column) segments of packed (value, row, column) words and multiplied on tcgen05
-    tensor cores; fp32 modules (and others) keep rows of values + column indices for the CUDA-core kernel."""
+    tensor cores; fp32 modules (and others) keep rows of values + column indices for the CUDA-core kernel. A module
+    whose blocks are all 4-bit ones takes the layout "int4"."""
 
     @staticmethod
     def usable(blocks: list) -> bool:
         """CUDA tensors of bf16, f16 or f32, 2-D blocks (p2p/compact.py:117-122 asks for the same, less fp32, plus
         columns in multiples of 8, which only the tensor-core layout needs)."""
+        if blocks[0][0] == "int4":
+            return blocks[0][1].is_cuda and blocks[0][1].dim() == 2
         t = blocks[0][1]
         return t.is_cuda and t.dtype in (torch.bfloat16, torch.float16, torch.float32) and t.dim() == 2
 
     def __init__(self, blocks: list, layout: str | None = None):
         if not blocks:
             raise P2PError("a module needs at least one row block")
+        if any(b[0] == "int4" for b in blocks):
+            self._init_int4(blocks, layout)
+            return
         blocks = [to_compact(b) for b in blocks]
         self.cols = _cols(blocks[0])
         self.dtype = blocks[0][1].dtype
@@ -131,8 +144,20 @@ class Tiles:
         else:
             raise P2PError(f"unknown layout {self.layout!r}")
 
+    def _init_int4(self, blocks: list, layout: str | None) -> None:
+        if layout not in (None, "int4") or any(b[0] != "int4" for b in blocks):
+            raise P2PError("4-bit blocks make up a whole module, in the layout \"int4\"")
+        if any(b[1].dim() != 2 for b in blocks):
+            raise P2PError("blocks share one dtype and are 2-D")
+        self.int4 = int4.Layout(blocks)
+        self.layout, self.blocks = "int4", None
+        self.rows, self.cols, self.dtype, self.device = (self.int4.rows, self.int4.cols, self.int4.dtype,
+                                                         self.int4.device)
+
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [T, cols] @ W.T: [T, rows]. Any T (the reference launches at most 64 tokens at a time)."""
+        if self.layout == "int4":
+            return self.int4.mm(x, out=out)
         if x.dtype != self.dtype:
             raise P2PError(f"x is {x.dtype}, the weights {self.dtype}")
         if self.layout == "mask":
@@ -142,6 +167,8 @@ class Tiles:
         return kernels.spmm_rows(x, self.blocks, self.cols, self.rows, out=out)
 
     def nbytes(self) -> int:
+        if self.layout == "int4":
+            return self.int4.nbytes()
         if self.layout == "mask":
             return self.data.numel() + self.seg.numel() * 8
         if self.layout == "tc":

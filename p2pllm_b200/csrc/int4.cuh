@@ -1,0 +1,79 @@
+// The 4-bit weight layout (p2p_int4_layout), shared by the kernels that read it.
+//
+// A module's rows are cut into blocks of 16, its columns into blocks of 64. A (row block, column block) is 512 bytes:
+// lane t = 4 n + j of a warp owns the 16 bytes at 16 t, word r of them (r = 0..3) holding the codes of rows n and n + 8
+// at columns 16 r + 4 j .. + 3, as four pairs of neighbouring columns whose low column is nibble i and high column
+// nibble i + 4:
+//   i = 0: row n, columns 0 and 1    i = 1: row n, columns 2 and 3    i = 2, 3: the same of row n + 8
+// so that one mask leaves a pair in the low bits of both halves of the word, ready to become two 16-bit floats. That is
+// a lane's A fragment of four m16n8k16 products whose k runs 4 j .. 4 j + 3 instead of {2 j, 2 j + 1, 2 j + 8, 2 j + 9}
+// (the sum over k does not mind, B's fragment takes the same columns: one 8-byte load of x), and also a lane's part of
+// a tcgen05.st.16x256b.x4 of 16 rows by 64 columns into tensor memory.
+//   blocks   [experts][row blocks][column blocks][512]
+//   scales   [experts][row blocks][groups][8][2]: rows n and n + 8, 16-bit; zeros the same in bytes (absent: 8)
+// Of a gated module the even row blocks are gate rows, the odd ones the same units' up rows.
+#pragma once
+#include "common.cuh"
+
+namespace p2p {
+namespace q4 {
+
+constexpr int kRows = 16;
+constexpr int kCols = 64;
+constexpr int kBlockBytes = 512;
+
+__host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Row blocks of one expert; a gated module's halves are padded to whole blocks each.
+__host__ __device__ inline int64_t row_blocks(int64_t rows, int gated) {
+    return gated ? 2 * div_up(rows / 2, kRows) : div_up(rows, kRows);
+}
+
+template <typename T> struct Codes;
+
+// bf16 holds 128 + q exactly (8 significant bits): q lands in the last mantissa bits of 0x4300 = 128.
+template <> struct Codes<__nv_bfloat16> {
+    uint32_t sub[2];                                   // 128 + zero of rows n and n + 8, twice
+    __device__ __forceinline__ void zeros(uint32_t z0, uint32_t z1) {
+        sub[0] = (0x4300u | z0) * 0x10001u;
+        sub[1] = (0x4300u | z1) * 0x10001u;
+    }
+    // The four A registers of one word: (row n, k 0 1), (row n + 8, k 0 1), (row n, k 2 3), (row n + 8, k 2 3), each
+    // the exact difference code - zero.
+    __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t q = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+            const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&sub[i >> 1]));
+            a[(i >> 1) + 2 * (i & 1)] = *reinterpret_cast<const uint32_t*>(&d);
+        }
+    }
+};
+
+// f16 holds 1024 + 16 q exactly (11 significant bits): two of the four pairs need no shift, (1024 + 16 q) / 16 - (64 +
+// zero) being exact too.
+template <> struct Codes<__half> {
+    uint32_t sub[2], sub16[2];
+    __device__ __forceinline__ void zeros(uint32_t z0, uint32_t z1) {
+        sub[0] = (0x6400u | z0) * 0x10001u;
+        sub[1] = (0x6400u | z1) * 0x10001u;
+        sub16[0] = (0xd400u | (z0 << 4)) * 0x10001u;   // -(64 + zero): 64's mantissa steps are 1 / 16
+        sub16[1] = (0xd400u | (z1 << 4)) * 0x10001u;
+    }
+    __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) const {
+        const __half2 sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2c00));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t v = h ? w >> 8 : w;
+            const uint32_t q0 = (v & 0x000f000fu) | 0x64006400u, q1 = (v & 0x00f000f0u) | 0x64006400u;
+            const __half2 d0 = __hsub2(*reinterpret_cast<const __half2*>(&q0), *reinterpret_cast<const __half2*>(&sub[h]));
+            const __half2 d1 = __hfma2(*reinterpret_cast<const __half2*>(&q1), sixteenth,
+                                       *reinterpret_cast<const __half2*>(&sub16[h]));
+            a[h] = *reinterpret_cast<const uint32_t*>(&d0);
+            a[h + 2] = *reinterpret_cast<const uint32_t*>(&d1);
+        }
+    }
+};
+
+}  // namespace q4
+}  // namespace p2p

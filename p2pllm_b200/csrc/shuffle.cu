@@ -1,0 +1,410 @@
+// Routed experts, the tokens' way there and back, without a word to the host (p2p_moe_route reads its counts back):
+//
+//   p2p_moe_sort     the (token, slot) pairs with an expert sorted by expert, pairs of one expert in their own order
+//   p2p_moe_spread   out[where[t K + j]] = x[t]: the tokens' rows in that order (and the gradient's way back from sums)
+//   p2p_moe_sum      out[t] = sum_j w[t, j] y[where[t K + j]], fp32 in slot order (w = 1: the gradient of the spread)
+//   p2p_moe_sum_back dy[where[t K + j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], y[where[t K + j]]>
+//
+// Rows of an order are `pairs` long whatever the routing: behind the last routed pair order is -1 and rows are zero.
+// p2p/compact.py:241-256 leaves all of this to SGLang's fused MoE.
+#include "sm100.cuh"
+
+namespace p2p {
+namespace {
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortExperts = 1024;
+constexpr int kClusterCtas = 8;
+constexpr int64_t kOneCtaPairs = 8192;
+
+struct SortParams {
+    const void* ids;
+    int n, experts;
+    int32_t *order, *where, *offsets;
+    int32_t *items, *n_items;
+    int max_items, item_tokens;
+};
+
+// A stable counting sort by one CTA, or by a cluster of 8 above 8192 pairs (each then counts and places an eighth).
+// Every warp owns a run of consecutive pairs: it counts them into a histogram of its own, 32 at a step (lanes with the
+// same expert find each other by match.any, so no atomics and no order to lose), the histograms turn into first places
+// by sums over warps, CTAs (through distributed shared memory) and experts, and the warp walks its run again and places
+// the pairs.
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
+    extern __shared__ int sm[];
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.experts;
+    int* hist = sm;                                  // [warps][E]
+    int* mine = hist + warps * E;                    // [E]: this CTA's pairs of each expert, which the others read
+    __shared__ int s_sum[2][32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int cta = blockIdx.x, ctas = gridDim.x;    // the grid is one cluster
+    for (int i = threadIdx.x; i < warps * E; i += blockDim.x) hist[i] = 0;
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int runs = warps * ctas, per = ((p.n + runs - 1) / runs + 31) / 32 * 32;
+    const int begin = min(p.n, (cta * warps + warp) * per), end = min(p.n, begin + per);
+    const I* ids = reinterpret_cast<const I*>(p.ids);
+    const unsigned below = (1u << lane) - 1u;
+    int* h = hist + warp * E;
+    auto expert_at = [&](int i) -> int {             // -1: routed nowhere
+        const int64_t e = i < end ? (int64_t)ids[i] : -1;
+        return e >= 0 && e < E ? (int)e : -1;
+    };
+    for (int i0 = begin; i0 < end; i0 += 32) {
+        const int e = expert_at(i0 + lane);
+        const unsigned peers = __match_any_sync(0xffffffffu, e);
+        if (e >= 0 && (peers & below) == 0) h[e] += __popc(peers);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {              // first places within this CTA
+        int run = 0;
+        for (int w = 0; w < warps; ++w) {
+            const int c = hist[w * E + e];
+            hist[w * E + e] = run;
+            run += c;
+        }
+        mine[e] = run;
+    }
+    if (ctas > 1) sm100::cluster_sync_all(); else __syncthreads();
+    // totals over the CTAs, and exclusive sums over the experts: of the pairs and of the items. E <= blockDim.
+    int all = 0, before = 0;
+    if (threadIdx.x < E) {
+        if (ctas > 1) {
+            const uint32_t at = sm100::smem_u32(mine + threadIdx.x);
+            for (int c = 0; c < ctas; ++c) {
+                int v;
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(sm100::cluster_addr(at, c)) : "memory");
+                if (c < cta) before += v;
+                all += v;
+            }
+        } else {
+            all = mine[threadIdx.x];
+        }
+    }
+    const int n_it = (all + p.item_tokens - 1) / p.item_tokens;
+    int pairs = all, items = n_it;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, pairs, o), b = __shfl_up_sync(0xffffffffu, items, o);
+        if (lane >= o) { pairs += a; items += b; }
+    }
+    if (lane == 31) { s_sum[0][warp] = pairs; s_sum[1][warp] = items; }
+    __syncthreads();
+    int pair_base = 0, item_base = 0, pair_total = 0, item_total = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) { pair_base += s_sum[0][w]; item_base += s_sum[1][w]; }
+        pair_total += s_sum[0][w];
+        item_total += s_sum[1][w];
+    }
+    const int start = pair_base + pairs - all, first_item = item_base + items - n_it;
+    if (threadIdx.x < E) {
+        for (int w = 0; w < warps; ++w) hist[w * E + threadIdx.x] += start + before;
+        if (cta == 0) {
+            p.offsets[threadIdx.x] = start;
+            for (int k = 0; k < n_it && first_item + k < p.max_items; ++k)
+                reinterpret_cast<int4*>(p.items)[first_item + k] =
+                    make_int4(threadIdx.x, start + k * p.item_tokens, min(p.item_tokens, all - k * p.item_tokens), 0);
+        }
+    }
+    if (cta == 0 && threadIdx.x == 0) {
+        p.offsets[E] = pair_total;
+        *p.n_items = min(item_total, p.max_items);
+    }
+    __syncthreads();
+    for (int i0 = begin; i0 < end; i0 += 32) {
+        const int i = i0 + lane, e = expert_at(i);
+        const unsigned peers = __match_any_sync(0xffffffffu, e);
+        const int at = e >= 0 ? h[e] : 0;
+        __syncwarp();
+        if (e >= 0 && (peers & below) == 0) h[e] = at + __popc(peers);
+        __syncwarp();
+        if (i < end) {
+            const int place = at + __popc(peers & below);
+            p.where[i] = e >= 0 ? place : -1;
+            if (e >= 0) p.order[place] = i;
+        }
+    }
+    for (int i = pair_total + cta * blockDim.x + threadIdx.x; i < p.n; i += ctas * blockDim.x) p.order[i] = -1;
+    if (ctas > 1) sm100::cluster_sync_all();         // nobody leaves while its counts may still be read
+}
+
+// --- rows there and back: vectors of N elements of T, 16 bytes where every row allows it, else one element -------------
+
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+
+struct RowParams {
+    const void *x, *y;                               // [tokens, hidden] (x, or dout) and [pairs, hidden]
+    void* out;
+    int64_t ldx, ldy, ldo;
+    const int32_t *where, *last;                     // last: the number of routed pairs
+    const void* w;                                   // null: 1
+    void* dw;
+    int w_dtype, tokens, k, vecs;                    // vectors a row
+};
+
+__device__ __forceinline__ float load_weight(const void* w, int dtype, int64_t i) {
+    if (dtype == P2P_F32) return reinterpret_cast<const float*>(w)[i];
+    if (dtype == P2P_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(w)[i]);
+    return __half2float(reinterpret_cast<const __half*>(w)[i]);
+}
+__device__ __forceinline__ void store_weight(void* w, int dtype, int64_t i, float v) {
+    if (dtype == P2P_F32) reinterpret_cast<float*>(w)[i] = v;
+    else if (dtype == P2P_BF16) reinterpret_cast<__nv_bfloat16*>(w)[i] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(w)[i] = __float2half_rn(v);
+}
+
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_vec(const void* p, int64_t at) {
+    return *reinterpret_cast<const Vec<T, N>*>(reinterpret_cast<const T*>(p) + at);
+}
+template <typename T, int N> __device__ __forceinline__ void store_vec(void* p, int64_t at, const Vec<T, N>& v) {
+    *reinterpret_cast<Vec<T, N>*>(reinterpret_cast<T*>(p) + at) = v;
+}
+
+// Zeroes the rows of p.out behind the last routed pair; the whole grid takes part.
+template <typename T, int N> __device__ __forceinline__ void zero_behind(const RowParams& p) {
+    const int threads = blockDim.x * blockDim.y, last = *p.last;
+    const int64_t pairs = (int64_t)p.tokens * p.k, n = (pairs - last) * p.vecs;
+    Vec<T, N> zero;
+#pragma unroll
+    for (int i = 0; i < N; ++i) zero.v[i] = from_f32<T>(0.f);
+    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * threads + threadIdx.y * blockDim.x + threadIdx.x;
+         i < n; i += (int64_t)gridDim.x * gridDim.y * threads)
+        store_vec<T, N>(p.out, (last + i / p.vecs) * p.ldo + i % p.vecs * N, zero);
+}
+
+constexpr int kBatch = 8;                            // slots whose rows a thread holds at a time
+constexpr int kRowThreads = 256;
+
+template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) spread_kernel(const RowParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (t < p.tokens) {
+        for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < p.vecs; v += gridDim.y * blockDim.x) {
+            const Vec<T, N> val = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
+#pragma unroll 4
+            for (int j = 0; j < p.k; ++j) {
+                const int at = __ldg(p.where + t * p.k + j);
+                if (at >= 0) store_vec<T, N>(p.out, at * p.ldo + (int64_t)v * N, val);
+            }
+        }
+    }
+    zero_behind<T, N>(p);
+}
+
+template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_kernel(const RowParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= p.tokens) return;
+    for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < p.vecs; v += gridDim.y * blockDim.x) {
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        for (int j0 = 0; j0 < p.k; j0 += kBatch) {
+            Vec<T, N> rows[kBatch];
+            int at[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                at[b] = j0 + b < p.k ? __ldg(p.where + t * p.k + j0 + b) : -1;
+                if (at[b] >= 0) rows[b] = load_vec<T, N>(p.y, at[b] * p.ldy + (int64_t)v * N);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                if (at[b] < 0) continue;
+                const float w = p.w ? load_weight(p.w, p.w_dtype, t * p.k + j0 + b) : 1.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] = fmaf(w, to_f32(rows[b].v[i]), acc[i]);
+            }
+        }
+        Vec<T, N> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[i]);
+        store_vec<T, N>(p.out, t * p.ldo + (int64_t)v * N, o);
+    }
+}
+
+// blockDim.x is whole warps: a token's dots are summed by shuffles, then over its warps in warp order.
+template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_back_kernel(const RowParams p) {
+    __shared__ float s_dot[kRowThreads / 32][kBatch];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int lane = threadIdx.x & 31, row_warps = blockDim.x >> 5, row_warp = threadIdx.x >> 5;
+    const bool live = t < p.tokens;
+    for (int j0 = 0; j0 < p.k; j0 += kBatch) {
+        float dot[kBatch], w[kBatch];
+        int at[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const bool in = live && j0 + b < p.k;
+            dot[b] = 0.f;
+            at[b] = in ? __ldg(p.where + t * p.k + j0 + b) : -1;
+            w[b] = at[b] >= 0 ? load_weight(p.w, p.w_dtype, t * p.k + j0 + b) : 0.f;
+        }
+        for (int v = threadIdx.x; live && v < p.vecs; v += blockDim.x) {
+            const Vec<T, N> g = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
+            Vec<T, N> rows[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (at[b] >= 0) rows[b] = load_vec<T, N>(p.y, at[b] * p.ldy + (int64_t)v * N);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                if (at[b] < 0) continue;
+                Vec<T, N> o;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float gi = to_f32(g.v[i]);
+                    dot[b] = fmaf(gi, to_f32(rows[b].v[i]), dot[b]);
+                    o.v[i] = from_f32<T>(w[b] * gi);
+                }
+                store_vec<T, N>(p.out, at[b] * p.ldo + (int64_t)v * N, o);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], o);
+            if (lane == 0) s_dot[threadIdx.y * row_warps + row_warp][b] = dot[b];
+        }
+        __syncthreads();
+        const int b = threadIdx.x;
+        if (live && b < kBatch && j0 + b < p.k) {
+            float sum = 0.f;
+            for (int r = 0; r < row_warps; ++r) sum += s_dot[threadIdx.y * row_warps + r][b];
+            store_weight(p.dw, p.w_dtype, t * p.k + j0 + b, sum);
+        }
+        __syncthreads();
+    }
+    zero_behind<T, N>(p);
+}
+
+enum RowOp { kSpread, kSum, kSumBack };
+
+template <typename T, int N> int launch_rows(RowOp op, RowParams& p, int64_t hidden, cudaStream_t st, const char* what) {
+    p.vecs = (int)(hidden / N);
+    int bx = 32;
+    while (bx < kRowThreads && bx < p.vecs) bx *= 2;
+    const int by = kRowThreads / bx;
+    const int64_t gx = ((int64_t)p.tokens + by - 1) / by;
+    // few tokens: a row's vectors are dealt over blocks too (the backward sum reduces over a row in one block)
+    int64_t gy = 1;
+    if (op != kSumBack && gx < sm_count()) gy = (p.vecs + bx - 1) / bx;
+    if (gy > 65535) gy = 65535;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)gx, (unsigned)gy);
+    cfg.blockDim = dim3((unsigned)bx, (unsigned)by);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, op == kSpread ? spread_kernel<T, N> : op == kSum ? sum_kernel<T, N> : sum_back_kernel<T, N>,
+                       (const RowParams)p);
+    return launch_status(what);
+}
+
+int run_rows(RowOp op, RowParams& p, int dtype, int64_t hidden, cudaStream_t st, const char* what) {
+    const int size = dtype_size(dtype), n = 16 / size;
+    // strides that no access uses (of null pointers) are 0
+    const bool vec = hidden % n == 0 && p.ldx % n == 0 && p.ldy % n == 0 && p.ldo % n == 0 && aligned16(p.x) &&
+                     aligned16(p.y) && aligned16(p.out);
+    switch (dtype) {
+        case P2P_BF16: return vec ? launch_rows<__nv_bfloat16, 8>(op, p, hidden, st, what)
+                                  : launch_rows<__nv_bfloat16, 1>(op, p, hidden, st, what);
+        case P2P_F16: return vec ? launch_rows<__half, 8>(op, p, hidden, st, what)
+                                 : launch_rows<__half, 1>(op, p, hidden, st, what);
+        default: return vec ? launch_rows<float, 4>(op, p, hidden, st, what)
+                            : launch_rows<float, 1>(op, p, hidden, st, what);
+    }
+}
+
+int check_rows(const char* what, int dtype, int64_t tokens, int k, int64_t hidden) {
+    if (!dtype_ok(dtype)) return fail(P2P_EUNSUPPORTED, "%s: bf16, f16 or f32", what);
+    P2P_REQUIRE(tokens >= 0 && k >= 1 && hidden >= 1 && hidden <= 0x7fffffff && tokens <= 0x7fffffff / k,
+                "%s: bad shape (%lld tokens, %d slots, %lld columns)", what, (long long)tokens, k, (long long)hidden);
+    return P2P_OK;
+}
+
+}  // namespace
+}  // namespace p2p
+
+using namespace p2p;
+
+extern "C" int p2p_moe_sort(const void* ids, int ids_bytes, int64_t n_pairs, int experts, int32_t* order,
+                            int32_t* where, int32_t* offsets, int32_t* items, int64_t max_items, int item_tokens,
+                            int32_t* n_items, void* stream) {
+    P2P_REQUIRE(n_pairs >= 0 && n_pairs <= 0x7fffffff - 65536 && experts >= 1 && item_tokens >= 1,
+                "p2p_moe_sort: %lld pairs, %d experts, items of %d", (long long)n_pairs, experts, item_tokens);
+    if (experts > kSortExperts)
+        return fail(P2P_EUNSUPPORTED, "p2p_moe_sort: %d experts, at most %d", experts, kSortExperts);
+    P2P_REQUIRE(ids_bytes == 4 || ids_bytes == 8, "p2p_moe_sort: ids of %d bytes, not 4 or 8", ids_bytes);
+    P2P_REQUIRE(offsets && n_items && items && (n_pairs == 0 || (ids && order && where)), "p2p_moe_sort: null pointer");
+    P2P_REQUIRE(aligned16(items), "p2p_moe_sort: items must start on a 16-byte boundary");
+    const int64_t full = (n_pairs + item_tokens - 1) / item_tokens;
+    const int64_t need = n_pairs < full + experts ? n_pairs : full + experts;
+    P2P_REQUIRE(max_items >= need && max_items <= 0x7fffffff, "p2p_moe_sort: room for %lld items, up to %lld needed",
+                (long long)max_items, (long long)need);
+    SortParams p = {ids, (int)n_pairs, experts, order, where, offsets, items, n_items, (int)max_items, item_tokens};
+    const int ctas = n_pairs > kOneCtaPairs ? kClusterCtas : 1;
+    // threads: one an expert at least, 8 pairs a thread at most until the block is full
+    int threads = (experts + 31) / 32 * 32;
+    const int64_t want = (n_pairs / ctas / 8 + 31) / 32 * 32;
+    if (threads < want) threads = want < kSortThreads ? (int)want : kSortThreads;
+    // one histogram a warp: fewer warps where the experts are many
+    const size_t smem = ((size_t)(threads / 32) + 1) * experts * sizeof(int);
+    const void* fn = ids_bytes == 4 ? (const void*)sort_kernel<int32_t> : (const void*)sort_kernel<int64_t>;
+    if (int e = allow_smem(fn, (int)smem, "p2p_moe_sort")) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = as_stream(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = ctas > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, ids_bytes == 4 ? sort_kernel<int32_t> : sort_kernel<int64_t>, (const SortParams)p);
+    return launch_status("p2p_moe_sort");
+}
+
+extern "C" int p2p_moe_spread(const void* x, int dtype, int64_t tokens, int k, int64_t hidden, int64_t ldx,
+                              const int32_t* where, const int32_t* routed, void* out, int64_t ldo, void* stream) {
+    if (int e = check_rows("p2p_moe_spread", dtype, tokens, k, hidden)) return e;
+    if (tokens == 0) return P2P_OK;
+    P2P_REQUIRE(x && where && routed && out && ldx >= hidden && ldo >= hidden, "p2p_moe_spread: null pointer or stride");
+    RowParams p = {x, nullptr, out, ldx, 0, ldo, where, routed, nullptr, nullptr, P2P_F32, (int)tokens, k, 0};
+    return run_rows(kSpread, p, dtype, hidden, as_stream(stream), "p2p_moe_spread");
+}
+
+extern "C" int p2p_moe_sum(const void* y, int dtype, int64_t tokens, int k, int64_t hidden, int64_t ldy,
+                           const int32_t* where, const void* weights, int weights_dtype, void* out, int64_t ldo,
+                           void* stream) {
+    if (int e = check_rows("p2p_moe_sum", dtype, tokens, k, hidden)) return e;
+    if (tokens == 0) return P2P_OK;
+    P2P_REQUIRE(y && where && out && ldy >= hidden && ldo >= hidden && (!weights || dtype_ok(weights_dtype)),
+                "p2p_moe_sum: null pointer, stride or weights' type");
+    RowParams p = {nullptr, y, out, 0, ldy, ldo, where, nullptr, weights, nullptr, weights_dtype, (int)tokens, k, 0};
+    return run_rows(kSum, p, dtype, hidden, as_stream(stream), "p2p_moe_sum");
+}
+
+extern "C" int p2p_moe_sum_back(const void* dout, const void* y, int dtype, int64_t tokens, int k, int64_t hidden,
+                                int64_t ldd, int64_t ldy, const int32_t* where, const int32_t* routed,
+                                const void* weights, int weights_dtype, void* dy, int64_t lddy, void* dweights,
+                                void* stream) {
+    if (int e = check_rows("p2p_moe_sum_back", dtype, tokens, k, hidden)) return e;
+    if (tokens == 0) return P2P_OK;
+    P2P_REQUIRE(dout && y && where && routed && weights && dy && dweights && dtype_ok(weights_dtype),
+                "p2p_moe_sum_back: null pointer or weights' type");
+    P2P_REQUIRE(ldd >= hidden && ldy >= hidden && lddy >= hidden, "p2p_moe_sum_back: a row stride below the row");
+    RowParams p = {dout, y, dy, ldd, ldy, lddy, where, routed, weights, dweights, weights_dtype, (int)tokens, k, 0};
+    return run_rows(kSumBack, p, dtype, hidden, as_stream(stream), "p2p_moe_sum_back");
+}

@@ -3,7 +3,15 @@ instead of expanding every used expert to dense on every pass (p2p/compact.py:22
 
     ExpertTiles   one routed-expert tensor (row blocks with a leading expert dimension) in one tensor-core layout,
                   each expert starting on a 128-row tile
+    Int4Experts   the same for 4-bit blocks (int4.py)
     GroupedMoE    quant_method.apply(layer, dispatch_output): gated-SiLU experts (w13 = gate then up, w2 = down)
+
+and the tokens' way to the experts and back without a word to the host, so that a pass can be captured into a CUDA
+graph, and with gradients, so that experts of any kind can be trained between the two:
+
+    sort_tokens   ids [T, K] -> TokenOrder: the (token, slot) pairs sorted by expert
+    to_experts    x [T, H] -> [T K, H]: the tokens' rows in that order
+    from_experts  y [T K, H] -> [T, H]: each token's rows, weighted and added in slot order
 
 A pass: one kernel (p2p_moe_route) sorts the routed (token, slot) pairs by expert (stable) and writes the grouped
 GEMM's items; x's rows are gathered in that order; one grouped launch of the compact GEMM (p2p_spmm_tc_grouped_gated:
@@ -15,9 +23,11 @@ back once a pass to size the launches (the reference's CompactMoE also syncs, on
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
-from . import kernels
+from . import _lib, int4, kernels
 from ._lib import P2PError, call, dtype_code, ptr, require_cuda, stream_of
 from .compact import _cols, gate_up_rows, to_compact
 
@@ -104,21 +114,130 @@ def route(ids: torch.Tensor, experts: int) -> dict:
     return {"order": order[:pairs], "where": where[:n], "counts": counts, "items": items[:n_items], "most": most}
 
 
+@dataclass(frozen=True)
+class TokenOrder:
+    """A pass's routed (token, slot) pairs sorted by expert, those of one expert in their own order; all on the GPU.
+    Of the T K places the first offsets[-1] hold a pair."""
+    order: torch.Tensor           # int32 [T K]: the pair token * K + slot at each place, -1 behind the last
+    where: torch.Tensor           # int32 [T K]: each pair's place, -1 if it is routed nowhere
+    offsets: torch.Tensor         # int32 [experts + 1]: each expert's first place, then the number of routed pairs
+    items: torch.Tensor           # int32 [.., 4]: {expert, first place, places, 0}, runs of at most 32 places
+    n_items: torch.Tensor         # int32 [1]
+    tokens: int
+    topk: int
+
+    @property
+    def experts(self) -> int:
+        return self.offsets.numel() - 1
+
+    @property
+    def device(self) -> torch.device:
+        return self.order.device
+
+
+def sort_tokens(ids: torch.Tensor, experts: int) -> TokenOrder:
+    """The order of ids [T, K] (int32 or int64 expert ids; any id outside 0..experts - 1 is routed nowhere). One launch,
+    nothing read back; at most 1024 experts. The same expert may come up twice in a row: two pairs."""
+    require_cuda(ids)
+    if ids.dim() != 2 or ids.shape[1] < 1 or ids.dtype not in (torch.int32, torch.int64):
+        raise P2PError(f"ids of {tuple(ids.shape)} {ids.dtype}: int32 or int64 [tokens, slots]")
+    if not 1 <= experts <= 1024:
+        raise P2PError(f"{experts} experts: 1 to 1024")
+    return TokenOrder(*_lib.ops().moe_sort(ids, experts), ids.shape[0], ids.shape[1])
+
+
+def _check_rows(t: torch.Tensor, order: TokenOrder, rows: int) -> None:
+    require_cuda(t)
+    if t.dim() != 2 or t.shape[0] != rows or t.device != order.device:
+        raise P2PError(f"rows of {tuple(t.shape)} on {t.device}, wanted [{rows}, ..] on {order.device}")
+    dtype_code(t)
+
+
+def to_experts(x: torch.Tensor, order: TokenOrder) -> torch.Tensor:
+    """[T K, H]: x's rows in the order's places, zero behind the last pair. bfloat16, float16 or float32. The gradient
+    of x is the sum over its slots, in slot order and fp32."""
+    _check_rows(x, order, order.tokens)
+    return _lib.ops().moe_spread(x, order.where, order.offsets, order.topk)
+
+
+def from_experts(y: torch.Tensor, order: TokenOrder, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """[T, H]: per token the sum over its slots, in slot order and fp32, of weights[t, j] times the slot's row of
+    y [T K, H] (no weights: 1); slots routed nowhere add nothing. Gradients for y (zero behind the last pair) and for
+    weights [T, K] (bfloat16, float16 or float32)."""
+    _check_rows(y, order, order.tokens * order.topk)
+    if weights is not None:
+        require_cuda(weights)
+        if tuple(weights.shape) != (order.tokens, order.topk) or weights.device != order.device:
+            raise P2PError(f"weights of {tuple(weights.shape)} on {weights.device}, wanted "
+                           f"{(order.tokens, order.topk)} on {order.device}")
+        dtype_code(weights)
+    return _lib.ops().moe_sum(y, order.where, order.offsets, weights, order.topk)
+
+
+class Int4Experts:
+    """A routed-expert tensor [E, rows, cols] from 4-bit row blocks with a leading expert dimension, laid out once at
+    load. Calling it multiplies a sorted pass: with gather the rows of x [T, cols] go to the order's places as they are
+    read, without it x [T K, cols] lies in that order already. Returns [T K, rows], gated [T K, rows / 2] =
+    dtype(silu(gate) * up). Rows behind the last pair are zero, or in a given `out` left as they were. Nothing is read
+    back. Inference only."""
+
+    def __init__(self, blocks: list, gated: bool = False):
+        self.int4 = int4.Layout(blocks, gated)
+        if blocks[0][1].dim() != 3:
+            raise P2PError("routed experts' blocks have a leading expert dimension")
+        if self.int4.experts > 1024:
+            raise P2PError(f"{self.int4.experts} experts: 1 to 1024")
+        self.gated, self.experts = gated, self.int4.experts
+        self.rows, self.cols, self.dtype, self.device = (self.int4.rows, self.int4.cols, self.int4.dtype,
+                                                         self.int4.device)
+
+    def __call__(self, x: torch.Tensor, order: TokenOrder, gather: bool = False,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        q = self.int4
+        q.check_x(x)
+        pairs = order.tokens * order.topk
+        _check_rows(x, order, order.tokens if gather else pairs)
+        if order.experts != self.experts:
+            raise P2PError(f"an order of {order.experts} experts, weights of {self.experts}")
+        args = (x, q.words, q.scales, q.zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order, order.offsets,
+                order.items, order.n_items, order.topk, gather)
+        if out is None:
+            return _lib.ops().int4_grouped(*args)
+        out = kernels._out(out, (pairs, q.rows // 2 if q.gated else q.rows), x)
+        _lib.ops().int4_grouped_into(*args, out)
+        return out
+
+    def nbytes(self) -> int:
+        return self.int4.nbytes()
+
+
 class GroupedMoE(torch.nn.Module):
     """A FusedMoE's quant_method for compact routed experts, gated SiLU: weights {"w13_weight": blocks of [E, 2R, H]
-    (gate rows, then up rows), "w2_weight": blocks of [E, H, R]}. apply(layer, dispatch_output) returns the layer's
+    (gate rows, then up rows), "w2_weight": blocks of [E, H, R]}, all of them 4-bit blocks or none. apply(layer, dispatch_output) returns the layer's
     output [T, H] in x's dtype. Other attributes are the layer's own method's."""
 
     def __init__(self, method, weights: dict):
         super().__init__()
         self.method = method
         two_r = sum(b[1].shape[-2] for b in weights["w13_weight"])
+        kinds = {b[0] == "int4" for blocks in weights.values() for b in blocks}
+        if len(kinds) > 1:
+            raise P2PError("routed experts are all 4-bit or none of them")
+        self.is_int4 = kinds == {True}
+        if self.is_int4:
+            self.w13 = Int4Experts(weights["w13_weight"], gated=True)
+            self.w2 = Int4Experts(weights["w2_weight"])
+            self._check()
+            return
         # SiLU(gate) * up inside the gate/up launch when the rows allow it (R a multiple of 64, one k)
         try:
             self.w13 = ExpertTiles(weights["w13_weight"], gated=two_r % 128 == 0)
         except P2PError:
             self.w13 = ExpertTiles(weights["w13_weight"])
         self.w2 = ExpertTiles(weights["w2_weight"])
+        self._check()
+
+    def _check(self) -> None:
         if self.w13.rows % 2 or self.w2.cols != self.w13.rows // 2 or self.w2.rows != self.w13.cols:
             raise P2PError("w13 [E, 2R, H] and w2 [E, H, R] do not match")
 
@@ -136,6 +255,10 @@ class GroupedMoE(torch.nn.Module):
         x2 = x.reshape(-1, x.shape[-1])
         if x2.dtype != self.w13.dtype:
             raise P2PError(f"x is {x2.dtype}, the experts {self.w13.dtype}")
+        if self.is_int4:                            # four launches, no read back: the pass can be captured
+            order = sort_tokens(ids if ids.dtype in (torch.int32, torch.int64) else ids.long(), self.w13.experts)
+            down = self.w2(self.w13(x2, order, gather=True), order)
+            return from_experts(down, order, weights).reshape(*x.shape[:-1], self.w2.rows)
         r = route(ids, self.w13.experts)
         P = r["order"].numel()
         out = torch.empty(T, self.w2.rows, dtype=x2.dtype, device=x.device)

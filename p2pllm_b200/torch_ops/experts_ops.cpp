@@ -1,0 +1,372 @@
+// The 4-bit products and the token shuffle around routed experts as torch custom operators (namespace p2p_b200). The
+// products are for inference: an x that needs a gradient is refused. The shuffle's two directions are differentiable;
+// their gradients are the library's own kernels, one level deep (second derivatives of the weighted sum are refused).
+#include <torch/csrc/autograd/custom_function.h>
+
+#include <algorithm>
+
+#include "op_common.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+constexpr int64_t kItemTokens = 32;                   // places of one item: what a block of the grouped product takes
+
+// t [rows, cols] with unit column stride and rows that do not overlap (an expanded gradient's do).
+at::Tensor rows2d(const at::Tensor& t) {
+    const bool cols_ok = t.size(1) <= 1 || t.stride(1) == 1, rows_ok = t.size(0) <= 1 || t.stride(0) >= t.size(1);
+    return cols_ok && rows_ok ? t : t.contiguous();
+}
+int64_t row_stride(const at::Tensor& t) { return std::max(t.size(0) <= 1 ? (int64_t)0 : t.stride(0), t.size(1)); }
+
+void check_matrix(const at::Tensor& t, const char* what) {
+    TORCH_CHECK(t.is_cuda(), "p2p_b200: ", what, ": CUDA tensors only (the replica path has no CPU fallback)");
+    TORCH_CHECK(t.dim() == 2, "p2p_b200: ", what, " of ", t.sizes(), " is not a matrix");
+}
+
+const int32_t* ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* what) {
+    TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() >= n,
+                "p2p_b200: ", what, " is not a contiguous int32 tensor of ", n, " on ", like.device());
+    return t.data_ptr<int32_t>();
+}
+
+// ---- 4-bit products --------------------------------------------------------------------------------------------------
+
+void check_int4(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
+                const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols, int64_t group,
+                bool gated) {
+    check_matrix(x, "x");
+    TORCH_CHECK(x.size(1) == cols, "p2p_b200: x of ", x.sizes(), " does not have ", cols, " columns");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()),
+                "p2p_b200: 4-bit weights are for inference: x must not need a gradient");
+    TORCH_CHECK(group == 32 || group == 64 || group == 128, "p2p_b200: groups of ", group, " columns, not 32, 64 or 128");
+    const int64_t rbs = experts * p2p_int4_row_blocks(rows, gated);
+    TORCH_CHECK(words.device() == x.device() && words.is_contiguous() && words.nbytes() >= (size_t)(rbs * ((cols + 63) / 64) * 512),
+                "p2p_b200: 4-bit words do not hold ", rows, " x ", cols);
+    const int64_t n = rbs * ((cols + group - 1) / group) * 16;
+    TORCH_CHECK(scales.device() == x.device() && scales.is_contiguous() && scales.scalar_type() == x.scalar_type() &&
+                    scales.numel() >= n, "p2p_b200: scales are not ", n, " of ", x.scalar_type(), " on ", x.device());
+    TORCH_CHECK(!zeros || (zeros->device() == x.device() && zeros->is_contiguous() && zeros->scalar_type() == at::kByte &&
+                           zeros->numel() >= n), "p2p_b200: zero points are not ", n, " bytes on ", x.device());
+}
+
+void check_rows_out(const at::Tensor& out, const at::Tensor& x, int64_t rows, int64_t cols) {
+    TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type() && out.dim() == 2 &&
+                    out.size(0) == rows && out.size(1) == cols &&
+                    (out.numel() == 0 || ((cols == 1 || out.stride(1) == 1) && (rows == 1 || out.stride(0) >= cols))),
+                "p2p_b200: out of ", out.sizes(), " ", out.scalar_type(), " does not take y [", rows, ", ", cols, "] ",
+                x.scalar_type());
+}
+
+const uint8_t* bytes(const std::optional<at::Tensor>& t) { return t ? t->data_ptr<uint8_t>() : nullptr; }
+
+void int4_mm_into(const at::Tensor& x_in, const at::Tensor& words, const at::Tensor& scales,
+                  const std::optional<at::Tensor>& zeros, int64_t rows, int64_t cols, int64_t group, bool gated,
+                  const at::Tensor& out) {
+    check_int4(x_in, words, scales, zeros, 1, rows, cols, group, gated);
+    check_rows_out(out, x_in, x_in.size(0), gated ? rows / 2 : rows);
+    const c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = rows2d(x_in);
+    check(p2p_int4_mm(x.data_ptr(), dtype_code(x), x.size(0), cols, row_stride(x), words.data_ptr(), scales.data_ptr(),
+                      bytes(zeros), rows, (int)group, gated, out.data_ptr(), row_stride(out), stream_of(x)),
+          "p2p_int4_mm");
+}
+
+at::Tensor int4_mm(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
+                   const std::optional<at::Tensor>& zeros, int64_t rows, int64_t cols, int64_t group, bool gated) {
+    check_matrix(x, "x");
+    at::Tensor out = at::empty({x.size(0), gated ? rows / 2 : rows}, x.options());
+    int4_mm_into(x, words, scales, zeros, rows, cols, group, gated, out);
+    return out;
+}
+
+void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& words, const at::Tensor& scales,
+                      const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
+                      int64_t group, bool gated, const at::Tensor& order, const at::Tensor& offsets,
+                      const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
+                      const at::Tensor& out, bool zero_behind) {
+    check_int4(x_in, words, scales, zeros, experts, rows, cols, group, gated);
+    const int64_t pairs = order.numel();
+    TORCH_CHECK(topk >= 1 && x_in.size(0) == (gather ? pairs / topk : pairs) && pairs % topk == 0, "p2p_b200: x has ",
+                x_in.size(0), " rows, the order is of ", pairs, " pairs, ", topk, " a token");
+    check_rows_out(out, x_in, pairs, gated ? rows / 2 : rows);
+    const c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = rows2d(x_in);
+    const int32_t* at_order = ints(order, x, pairs, "order");
+    const int32_t* at_offsets = ints(offsets, x, experts + 1, "offsets");
+    TORCH_CHECK(offsets.numel() == experts + 1, "p2p_b200: the order is of ", offsets.numel() - 1, " experts, the weights of ",
+                experts);
+    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, row_stride(x), words.data_ptr(), scales.data_ptr(),
+                           bytes(zeros), rows, (int)group, gated, ints(items, x, 0, "items"),
+                           ints(n_items, x, 1, "n_items"), items.numel() / 4, std::min(pairs, kItemTokens),
+                           gather ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
+                           out.data_ptr(), row_stride(out), stream_of(x)),
+          "p2p_int4_grouped");
+}
+
+void int4_grouped_into(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
+                       const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
+                       int64_t group, bool gated, const at::Tensor& order, const at::Tensor& offsets,
+                       const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
+                       const at::Tensor& out) {
+    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, offsets, items, n_items, topk,
+                     gather, out, false);
+}
+
+at::Tensor int4_grouped(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
+                        const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
+                        int64_t group, bool gated, const at::Tensor& order, const at::Tensor& offsets,
+                        const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather) {
+    check_matrix(x, "x");
+    at::Tensor out = at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
+    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, offsets, items, n_items, topk,
+                     gather, out, true);
+    return out;
+}
+
+// ---- tokens sorted by expert and back --------------------------------------------------------------------------------
+
+int64_t max_items(int64_t pairs, int64_t experts) {
+    return std::min(pairs, (pairs + kItemTokens - 1) / kItemTokens + experts);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& ids_in, int64_t experts) {
+    TORCH_CHECK(ids_in.is_cuda(), "p2p_b200: CUDA tensors only (the replica path has no CPU fallback)");
+    TORCH_CHECK(ids_in.scalar_type() == at::kInt || ids_in.scalar_type() == at::kLong, "p2p_b200: ids are int32 or int64");
+    TORCH_CHECK(experts >= 1 && experts <= 1024, "p2p_b200: ", experts, " experts, 1 to 1024");
+    const c10::cuda::CUDAGuard guard(ids_in.device());
+    const at::Tensor ids = ids_in.contiguous();
+    const int64_t n = ids.numel(), most = std::max<int64_t>(max_items(n, experts), 1);
+    // one allocation: items (16-byte aligned), order, where, offsets, n_items
+    at::Tensor all = at::empty({4 * most + 2 * n + experts + 2}, ids.options().dtype(at::kInt));
+    at::Tensor items = all.narrow(0, 0, 4 * most), order = all.narrow(0, 4 * most, n),
+               where = all.narrow(0, 4 * most + n, n), offsets = all.narrow(0, 4 * most + 2 * n, experts + 1),
+               n_items = all.narrow(0, 4 * most + 2 * n + experts + 1, 1);
+    check(p2p_moe_sort(ids.data_ptr(), (int)ids.element_size(), n, (int)experts, order.data_ptr<int32_t>(),
+                       where.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), items.data_ptr<int32_t>(), most,
+                       (int)kItemTokens, n_items.data_ptr<int32_t>(), stream_of(ids)),
+          "p2p_moe_sort");
+    return {order, where, offsets, items, n_items};
+}
+
+const int32_t* routed_of(const at::Tensor& offsets, const at::Tensor& like) {
+    return ints(offsets, like, 1, "offsets") + offsets.numel() - 1;
+}
+
+at::Tensor moe_spread(const at::Tensor& x_in, const at::Tensor& where, const at::Tensor& offsets, int64_t topk) {
+    check_matrix(x_in, "x");
+    const c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = rows2d(x_in);
+    TORCH_CHECK(topk >= 1 && where.numel() == x.size(0) * topk, "p2p_b200: x has ", x.size(0), " rows, the order is of ",
+                where.numel(), " pairs, ", topk, " a token");
+    at::Tensor out = at::empty({where.numel(), x.size(1)}, x.options());
+    if (out.numel() == 0) return out;
+    check(p2p_moe_spread(x.data_ptr(), dtype_code(x), x.size(0), (int)topk, x.size(1), row_stride(x),
+                         ints(where, x, where.numel(), "where"), routed_of(offsets, x), out.data_ptr(), out.size(1),
+                         stream_of(x)),
+          "p2p_moe_spread");
+    return out;
+}
+
+void check_sum(const at::Tensor& y, const at::Tensor& where, const std::optional<at::Tensor>& weights, int64_t topk) {
+    check_matrix(y, "y");
+    TORCH_CHECK(topk >= 1 && where.numel() % topk == 0 && y.size(0) == where.numel(), "p2p_b200: y has ", y.size(0),
+                " rows, the order is of ", where.numel(), " pairs, ", topk, " a token");
+    TORCH_CHECK(!weights || (weights->device() == y.device() && weights->numel() == where.numel()),
+                "p2p_b200: weights are not ", where.numel(), " on ", y.device());
+}
+
+at::Tensor moe_sum(const at::Tensor& y_in, const at::Tensor& where, const at::Tensor&,
+                   const std::optional<at::Tensor>& weights, int64_t topk) {
+    check_sum(y_in, where, weights, topk);
+    const c10::cuda::CUDAGuard guard(y_in.device());
+    const at::Tensor y = rows2d(y_in);
+    at::Tensor out = at::empty({where.numel() / topk, y.size(1)}, y.options());
+    if (out.numel() == 0) return out;
+    const at::Tensor w = weights ? weights->contiguous() : at::Tensor();
+    check(p2p_moe_sum(y.data_ptr(), dtype_code(y), out.size(0), (int)topk, y.size(1), row_stride(y),
+                      ints(where, y, where.numel(), "where"), weights ? w.data_ptr() : nullptr,
+                      weights ? dtype_code(w) : P2P_F32, out.data_ptr(), out.size(1), stream_of(y)),
+          "p2p_moe_sum");
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_sum_back(const at::Tensor& dout_in, const at::Tensor& y_in,
+                                                const at::Tensor& where, const at::Tensor& offsets,
+                                                const at::Tensor& weights_in, int64_t topk) {
+    check_sum(y_in, where, weights_in, topk);
+    check_matrix(dout_in, "the gradient");
+    TORCH_CHECK(dout_in.device() == y_in.device() && dout_in.scalar_type() == y_in.scalar_type() &&
+                    dout_in.size(0) == where.numel() / topk && dout_in.size(1) == y_in.size(1),
+                "p2p_b200: a gradient of ", dout_in.sizes(), " ", dout_in.scalar_type(), " for rows of ", y_in.sizes(), " ",
+                y_in.scalar_type());
+    const c10::cuda::CUDAGuard guard(y_in.device());
+    const at::Tensor y = rows2d(y_in), dout = rows2d(dout_in), w = weights_in.contiguous();
+    at::Tensor dy = at::empty({y.size(0), y.size(1)}, y.options()), dw = at::empty(weights_in.sizes(), w.options());
+    if (y.size(0) == 0) return {dy, dw};
+    if (y.size(1) == 0) return {dy, dw.zero_()};
+    check(p2p_moe_sum_back(dout.data_ptr(), y.data_ptr(), dtype_code(y), dout.size(0), (int)topk, y.size(1),
+                           row_stride(dout), row_stride(y), ints(where, y, where.numel(), "where"),
+                           routed_of(offsets, y), w.data_ptr(), dtype_code(w), dy.data_ptr(), y.size(1), dw.data_ptr(),
+                           stream_of(y)),
+          "p2p_moe_sum_back");
+    return {dy, dw};
+}
+
+// The operators as the dispatcher sees them, for the gradients below.
+at::Tensor call_spread(const at::Tensor& x, const at::Tensor& where, const at::Tensor& offsets, int64_t topk) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::moe_spread", "").typed<decltype(moe_spread)>();
+    return op.call(x, where, offsets, topk);
+}
+at::Tensor call_sum(const at::Tensor& y, const at::Tensor& where, const at::Tensor& offsets,
+                    const std::optional<at::Tensor>& weights, int64_t topk) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::moe_sum", "").typed<decltype(moe_sum)>();
+    return op.call(y, where, offsets, weights, topk);
+}
+std::tuple<at::Tensor, at::Tensor> call_sum_back(const at::Tensor& dout, const at::Tensor& y, const at::Tensor& where,
+                                                 const at::Tensor& offsets, const at::Tensor& weights, int64_t topk) {
+    static const auto op =
+        c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::moe_sum_back", "").typed<decltype(moe_sum_back)>();
+    return op.call(dout, y, where, offsets, weights, topk);
+}
+
+bool needs_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+struct Spread : torch::autograd::Function<Spread> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& where,
+                              const at::Tensor& offsets, int64_t topk) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({where, offsets});
+        ctx->saved_data["topk"] = topk;
+        return call_spread(x, where, offsets, topk);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list s = ctx->get_saved_variables();
+        at::Tensor dx;
+        if (grads[0].defined()) dx = call_sum(grads[0], s[0], s[1], std::nullopt, ctx->saved_data["topk"].toInt());
+        return {dx, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+struct Sum : torch::autograd::Function<Sum> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& where,
+                              const at::Tensor& offsets, const std::optional<at::Tensor>& weights, int64_t topk) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->saved_data["topk"] = topk;
+        ctx->saved_data["weighted"] = weights.has_value();
+        if (weights) ctx->save_for_backward({where, offsets, y, *weights});
+        else ctx->save_for_backward({where, offsets});
+        return call_sum(y, where, offsets, weights, topk);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const int64_t topk = ctx->saved_data["topk"].toInt();
+        at::Tensor dy, dw;
+        if (grads[0].defined()) {
+            if (!ctx->saved_data["weighted"].toBool()) dy = call_spread(grads[0], s[0], s[1], topk);
+            else std::tie(dy, dw) = call_sum_back(grads[0], s[2], s[0], s[1], s[3], topk);
+        }
+        return {dy, at::Tensor(), at::Tensor(), dw, at::Tensor()};
+    }
+};
+
+at::Tensor moe_spread_grad(const at::Tensor& x, const at::Tensor& where, const at::Tensor& offsets, int64_t topk) {
+    if (needs_grad(x)) return Spread::apply(x, where, offsets, topk);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_spread(x, where, offsets, topk);
+}
+at::Tensor moe_sum_grad(const at::Tensor& y, const at::Tensor& where, const at::Tensor& offsets,
+                        const std::optional<at::Tensor>& weights, int64_t topk) {
+    if (needs_grad(y) || (weights && needs_grad(*weights))) return Sum::apply(y, where, offsets, weights, topk);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_sum(y, where, offsets, weights, topk);
+}
+std::tuple<at::Tensor, at::Tensor> moe_sum_back_grad(const at::Tensor& dout, const at::Tensor& y,
+                                                     const at::Tensor& where, const at::Tensor& offsets,
+                                                     const at::Tensor& weights, int64_t topk) {
+    TORCH_CHECK(!(needs_grad(dout) || needs_grad(y) || needs_grad(weights)),
+                "p2p_b200: second derivatives of the weighted sum are not offered");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_sum_back(dout, y, where, offsets, weights, topk);
+}
+
+// ---- shapes ----------------------------------------------------------------------------------------------------------
+
+at::Tensor int4_mm_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                        int64_t rows, int64_t, int64_t, bool gated) {
+    return at::empty({x.size(0), gated ? rows / 2 : rows}, x.options());
+}
+void int4_mm_into_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                       int64_t, int64_t, int64_t, bool, const at::Tensor&) {}
+at::Tensor int4_grouped_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                             int64_t, int64_t rows, int64_t, int64_t, bool gated, const at::Tensor& order,
+                             const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool) {
+    return at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
+}
+void int4_grouped_into_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                            int64_t, int64_t, int64_t, int64_t, bool, const at::Tensor&, const at::Tensor&,
+                            const at::Tensor&, const at::Tensor&, int64_t, bool, const at::Tensor&) {}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort_meta(const at::Tensor& ids, int64_t experts) {
+    const auto o = ids.options().dtype(at::kInt);
+    const int64_t n = ids.numel();
+    return {at::empty({n}, o), at::empty({n}, o), at::empty({experts + 1}, o),
+            at::empty({4 * std::max<int64_t>(max_items(n, experts), 1)}, o), at::empty({1}, o)};
+}
+at::Tensor moe_spread_meta(const at::Tensor& x, const at::Tensor& where, const at::Tensor&, int64_t) {
+    return at::empty({where.numel(), x.size(1)}, x.options());
+}
+at::Tensor moe_sum_meta(const at::Tensor& y, const at::Tensor& where, const at::Tensor&, const std::optional<at::Tensor>&,
+                        int64_t topk) {
+    return at::empty({where.numel() / topk, y.size(1)}, y.options());
+}
+std::tuple<at::Tensor, at::Tensor> moe_sum_back_meta(const at::Tensor&, const at::Tensor& y, const at::Tensor&,
+                                                     const at::Tensor&, const at::Tensor& weights, int64_t) {
+    return {at::empty(y.sizes(), y.options()), at::empty(weights.sizes(), weights.options())};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(p2p_b200, m) {
+    m.def("int4_mm(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int rows, int cols, int group, bool gated) -> Tensor");
+    m.def("int4_mm_into(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int rows, int cols, int group, bool gated, "
+          "Tensor(a!) out) -> ()");
+    m.def("int4_grouped(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int experts, int rows, int cols, int group, "
+          "bool gated, Tensor order, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather) -> Tensor");
+    m.def("int4_grouped_into(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int experts, int rows, int cols, "
+          "int group, bool gated, Tensor order, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather, "
+          "Tensor(a!) out) -> ()");
+    m.def("moe_sort(Tensor ids, int experts) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("moe_spread(Tensor x, Tensor where, Tensor offsets, int topk) -> Tensor");
+    m.def("moe_sum(Tensor y, Tensor where, Tensor offsets, Tensor? weights, int topk) -> Tensor");
+    m.def("moe_sum_back(Tensor dout, Tensor y, Tensor where, Tensor offsets, Tensor weights, int topk) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(p2p_b200, CUDA, m) {
+    m.impl("int4_mm", &int4_mm);
+    m.impl("int4_mm_into", &int4_mm_into);
+    m.impl("int4_grouped", &int4_grouped);
+    m.impl("int4_grouped_into", &int4_grouped_into);
+    m.impl("moe_sort", &moe_sort);
+    m.impl("moe_spread", &moe_spread);
+    m.impl("moe_sum", &moe_sum);
+    m.impl("moe_sum_back", &moe_sum_back);
+}
+
+TORCH_LIBRARY_IMPL(p2p_b200, Autograd, m) {
+    m.impl("moe_spread", &moe_spread_grad);
+    m.impl("moe_sum", &moe_sum_grad);
+    m.impl("moe_sum_back", &moe_sum_back_grad);
+}
+
+TORCH_LIBRARY_IMPL(p2p_b200, Meta, m) {
+    m.impl("int4_mm", &int4_mm_meta);
+    m.impl("int4_mm_into", &int4_mm_into_meta);
+    m.impl("int4_grouped", &int4_grouped_meta);
+    m.impl("int4_grouped_into", &int4_grouped_into_meta);
+    m.impl("moe_sort", &moe_sort_meta);
+    m.impl("moe_spread", &moe_spread_meta);
+    m.impl("moe_sum", &moe_sum_meta);
+    m.impl("moe_sum_back", &moe_sum_back_meta);
+}

@@ -14,27 +14,9 @@
 #include <tuple>
 #include <vector>
 
-#include "p2p_b200.h"
+#include "op_common.h"
 
 namespace {
-
-int dtype_code(const at::Tensor& t) {
-    switch (t.scalar_type()) {
-        case at::kBFloat16: return P2P_BF16;
-        case at::kHalf: return P2P_F16;
-        case at::kFloat: return P2P_F32;
-        default: TORCH_CHECK(false, "p2p_b200: bfloat16, float16 or float32, got ", t.scalar_type());
-    }
-    return -1;
-}
-
-void check(int status, const char* what) {
-    TORCH_CHECK(status == P2P_OK, what, ": ", p2p_last_error(), " (status ", status, ")");
-}
-
-void* stream_of(const at::Tensor& t) {
-    return reinterpret_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
-}
 
 // A zeroed scratch buffer per device, purpose and stream, kept for the process (the kernels leave it zeroed again;
 // launches on one stream run in order and may share it, launches on two streams may overlap and must not).
