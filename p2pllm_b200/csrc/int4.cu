@@ -9,7 +9,9 @@
 //   p2p_int4_mm         y = x W^T
 //   p2p_int4_grouped    the same for the rows of one expert after the other, rows gathered by token or in place, with
 //                       silu(gate) * up applied on the way out of a gated module
+#include <stdlib.h>
 #include "int4.cuh"
+#include "int4_run.cuh"
 
 namespace p2p {
 namespace {
@@ -480,39 +482,81 @@ int int4_params(Int4Params& p, const char* what, const void* x, int dtype, int64
 }
 }  // namespace
 
+namespace {
+// Calls of up to this many tokens stay with the kernel above.
+bool use_tc(int64_t tokens, int64_t rows, int64_t cols) {
+    static const char* e = getenv("P2P_INT4_TC");
+    if (e) return tokens >= atoi(e);
+    return tokens > 8;
+}
+bool tc_aligned(const void* x, int64_t ldx) { return aligned16(x) && ldx % 8 == 0; }
+}  // namespace
+
+extern "C" size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated) {
+    if (tokens <= 0 || rows <= 0 || cols <= 0 || !use_tc(tokens, rows, cols)) return 0;
+    return int4_tc_workspace(tokens, rows, cols, gated);
+}
+
 extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* words,
                            const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated, void* y,
-                           int64_t ldy, void* stream) {
+                           int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
     P2P_REQUIRE(tokens >= 0 && rows >= 0 && tokens <= 0x7fffffff, "p2p_int4_mm: bad shape");
     if (tokens == 0 || rows == 0) return P2P_OK;
     Int4Params p;
     if (int e = int4_params(p, "p2p_int4_mm", x, dtype, cols, ldx, words, scales, zeros, rows, group, gated, y, ldy))
         return e;
+    cudaStream_t st = as_stream(stream);
+    if (use_tc(tokens, rows, cols)) {
+        P2P_REQUIRE(tc_aligned(x, ldx), "p2p_int4_mm: %lld tokens need x rows of 16-byte alignment", (long long)tokens);
+        const size_t need = p2p_int4_workspace(tokens, rows, cols, gated);
+        P2P_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+                    "p2p_int4_mm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+        Int4Call c = {};
+        c.x = x; c.dtype = dtype; c.tokens = tokens; c.cols = cols; c.ldx = ldx;
+        c.words = words; c.scales = scales; c.zeros = zeros;
+        c.rows = rows; c.group = group; c.gated = gated; c.y = y; c.ldy = ldy;
+        return int4_tc_run(c, workspace, st, "p2p_int4_mm");
+    }
     p.tokens = (int)tokens;
-    return dtype == P2P_BF16 ? run_int4<__nv_bfloat16>(p, tokens, 0, as_stream(stream), "p2p_int4_mm")
-                             : run_int4<__half>(p, tokens, 0, as_stream(stream), "p2p_int4_mm");
+    return dtype == P2P_BF16 ? run_int4<__nv_bfloat16>(p, tokens, 0, st, "p2p_int4_mm")
+                             : run_int4<__half>(p, tokens, 0, st, "p2p_int4_mm");
 }
 
 extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* words,
                                 const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated,
-                                const int32_t* items, const int32_t* n_items, int64_t max_items, int64_t max_tokens,
+                                const int32_t* items, const int32_t* n_items, int64_t max_items, int64_t item_tokens,
                                 const int32_t* order, int topk, const int32_t* routed, int64_t pairs, void* y,
                                 int64_t ldy, void* stream) {
-    P2P_REQUIRE(max_items >= 0 && rows >= 0 && max_tokens >= 0 && pairs >= 0, "p2p_int4_grouped: bad shape");
-    if (max_items == 0 || rows == 0 || max_tokens == 0) return P2P_OK;
-    P2P_REQUIRE(max_tokens <= 32, "p2p_int4_grouped: items of up to %lld tokens, at most 32", (long long)max_tokens);
+    P2P_REQUIRE(max_items >= 0 && rows >= 0 && item_tokens >= 0 && pairs >= 0 && pairs <= 0x7fffffff,
+                "p2p_int4_grouped: bad shape");
+    if (max_items == 0 || rows == 0 || item_tokens == 0 || pairs == 0) return P2P_OK;
+    const bool tc = item_tokens > 8;
+    P2P_REQUIRE(item_tokens <= kInt4TileTokens, "p2p_int4_grouped: items of up to %lld tokens, at most %d",
+                (long long)item_tokens, kInt4TileTokens);
     P2P_REQUIRE(items && n_items && topk >= 1, "p2p_int4_grouped: null pointer or topk %d", topk);
     P2P_REQUIRE(aligned16(items), "p2p_int4_grouped: items must start on a 16-byte boundary");
     Int4Params p;
     if (int e = int4_params(p, "p2p_int4_grouped", x, dtype, cols, ldx, words, scales, zeros, rows, group, gated, y,
                             ldy))
         return e;
+    cudaStream_t st = as_stream(stream);
+    if (tc) {
+        P2P_REQUIRE(!order, "p2p_int4_grouped: items of more than 8 tokens take x in the order's places");
+        P2P_REQUIRE(tc_aligned(x, ldx), "p2p_int4_grouped: items of more than 8 tokens need x rows of 16-byte alignment");
+        Int4Call c = {};
+        c.x = x; c.dtype = dtype; c.cols = cols; c.ldx = ldx;
+        c.words = words; c.scales = scales; c.zeros = zeros;
+        c.rows = rows; c.group = group; c.gated = gated; c.y = y; c.ldy = ldy;
+        c.items = items; c.n_items = n_items; c.max_items = max_items; c.item_tokens = item_tokens; c.pairs = pairs;
+        c.routed = routed;
+        return int4_tc_run(c, nullptr, st, "p2p_int4_grouped");
+    }
     p.items = items;
     p.n_items = n_items;
     p.order = order;
     p.topk = topk;
     p.routed = routed;
     p.pairs = pairs;
-    return dtype == P2P_BF16 ? run_int4<__nv_bfloat16>(p, max_tokens, max_items, as_stream(stream), "p2p_int4_grouped")
-                             : run_int4<__half>(p, max_tokens, max_items, as_stream(stream), "p2p_int4_grouped");
+    return dtype == P2P_BF16 ? run_int4<__nv_bfloat16>(p, item_tokens, max_items, st, "p2p_int4_grouped")
+                             : run_int4<__half>(p, item_tokens, max_items, st, "p2p_int4_grouped");
 }

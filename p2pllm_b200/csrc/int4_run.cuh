@@ -1,0 +1,29 @@
+// A 4-bit product as its C entries take it, handed to the tensor-core kernel (int4_tc.cu).
+#pragma once
+#include "common.cuh"
+
+namespace p2p {
+
+constexpr int kInt4TileTokens = 272;    // most tokens of a tile: its accumulator and three A tiles fill tensor memory
+
+struct Int4Call {
+    const void* x;
+    int dtype;
+    int64_t tokens, cols, ldx;          // dense
+    const void *words, *scales;
+    const uint8_t* zeros;
+    int64_t rows;
+    int group, gated;
+    void* y;
+    int64_t ldy;
+    const int32_t *items, *n_items;     // routed: x's rows are the places
+    int64_t max_items, item_tokens, pairs;
+    const int32_t* routed;              // not null: y's rows from *routed to pairs become zero
+};
+
+// Bytes of workspace int4_tc_run needs for a dense call.
+size_t int4_tc_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated);
+// x: 16-byte aligned rows (ldx and the start).
+int int4_tc_run(const Int4Call& call, void* workspace, cudaStream_t st, const char* what);
+
+}  // namespace p2p

@@ -1,0 +1,638 @@
+// (2d) The 4-bit product on tcgen05 tensor cores: y[t, r] = sum_c (code[r, c] - zero[r, g]) scale[r, g] x[t, c] for
+// every token count at which the streams below stay busy (int4.cu keeps the small calls), dense or for routed experts.
+//
+// Scales stay out of the tensor cores: a group's sum of exact small integers times x goes to TMEM in fp32, and the
+// warps that read it out multiply it by the group's scale on the way into fp32 registers, so no weight is rounded (one
+// scaled weight rounded to bf16 would double the squared error of the result). A CTA, one an SM, takes a contiguous run
+// of units (128 rows x 128 columns), row tile after row tile:
+//
+//   warp 16 (weights)   streams the run's codes, 8 KB a unit, into a ring in shared memory by bulk copies, ahead of the
+//                       previous kernel's end and up to 8 units ahead of their use
+//   warp 17 (x)         TMA of each unit's x tile [tokens x 128] (two 64-column boxes, 128-byte swizzle)
+//   warps 8-15 (build)  warp w turns the codes of one 16-row block into bf16 / f16 integers and stores them into the
+//                       unit's A tile in tensor memory (two tcgen05.st.16x256b.x4: the layout is that store's order)
+//   warps 18, 19 (MMA)  one thread each issues tcgen05.mma kind::f16, A from TMEM, M = 128, for one half of the tokens:
+//                       a group's columns into a zeroed accumulator, then a commit
+//   warps 0-3, 4-7      read the two halves' accumulators out, group after group, acc += scale * sum (packed fp32
+//                       pairs), and write the finished row tile: y itself, silu(gate) * up of it, or, where the tile
+//                       is shared with the neighbouring run, an fp32 partial that int4_join_kernel adds in run order
+//
+// Every wait is bounded (2 s): a launch that gives up records where, issues nothing more, drains what it issued and
+// exits (p2p_int4_status reads the site).
+#include <atomic>
+
+#include "int4.cuh"
+#include "int4_run.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
+
+namespace p2p {
+namespace {
+
+using namespace sm100;
+
+constexpr int kPromoteWarps = 8, kBuildWarps = 8;
+constexpr int kBuildWarp = kPromoteWarps;               // 8..15
+constexpr int kWeightWarp = kBuildWarp + kBuildWarps;   // 16
+constexpr int kXWarp = kWeightWarp + 1;                 // 17
+constexpr int kMmaWarp = kWeightWarp + 2;               // 18, 19
+constexpr int kThreads = 640;
+constexpr int kUnitBytes = 8 * 2 * q4::kBlockBytes;     // 128 rows x 128 columns of codes
+constexpr int kACols = 64;                              // TMEM columns of one unit's A tile
+constexpr int kTmemCols = 512;
+constexpr int kMaxW = 8, kMaxX = 8, kMaxA = 6, kMaxBuf = 2;
+constexpr int kSmemLimit = 227 * 1024 - 1024;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+__device__ int g_int4_error;            // site of the first wait that gave up since the last reset (0: none)
+__device__ unsigned g_int4_failed_seq;  // sequence number of the last launch in which a wait gave up
+
+struct TcParams {
+    const uint8_t* words;
+    const uint16_t* scales;
+    const uint8_t* zeros;               // null: 8
+    int rows, out_rows, rbs, row_tiles, kbs, units, groups, group_shift, gated;   // units: 128-column steps a row tile
+    int tokens, tile_tokens, token_tiles;                                         // dense
+    const int32_t* items;                                                         // routed
+    const int32_t* n_items;
+    void* y;
+    int64_t ldy;
+    const int32_t* routed;              // not null: output rows from *routed to pairs become zero
+    int64_t pairs;
+    float* partial;                     // [ctas][2][n_max][128]; null: every CTA takes whole row tiles
+    int n_max, ctas;
+    int x_rows, box_rows, w_slots, x_slots, a_slots, bufs, a_col0;
+    uint64_t wait_ns;
+    unsigned seq;
+};
+
+__device__ __forceinline__ void ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// Waits for this thread's TMEM loads; r passes through so that nothing reads it earlier.
+__device__ __forceinline__ void ld16_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// Two fp32 products and sums at once: acc.{lo,hi} += s.{lo,hi} * {lo, hi}.
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t s, uint32_t lo, uint32_t hi) {
+    asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%2, %3};\n\tfma.rn.f32x2 %0, %1, v, %0;\n\t}" : "+l"(acc) : "l"(s), "r"(lo), "r"(hi));
+}
+__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(v >> (32 * i))); }
+
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, site, wc));
+}
+
+// A row tile of the run: its row blocks, its tokens, the steps of it that this CTA takes.
+struct Tile {
+    int64_t rb0;                        // first row block, of all experts
+    int rt;                             // row tile within the module
+    int first, n;                       // first x row (and y row), tokens
+    int k0, k1;                         // steps [k0, k1) of p.units
+};
+
+__device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t u, int64_t u1) {
+    Tile t;
+    const int64_t id = u / p.units;
+    t.k0 = (int)(u - id * p.units);
+    t.k1 = (int)min((int64_t)p.units, t.k0 + (u1 - u));
+    if (p.items) {
+        const int item = (int)(id / p.row_tiles);
+        t.rt = (int)(id - (int64_t)item * p.row_tiles);
+        const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + item);
+        t.rb0 = (int64_t)it.x * p.rbs + t.rt * 8;
+        t.first = it.y;
+        t.n = min(it.z, p.n_max);
+    } else {
+        t.rt = (int)(id / p.token_tiles);
+        t.first = (int)(id - (int64_t)t.rt * p.token_tiles) * p.tile_tokens;
+        t.n = min(p.tile_tokens, p.tokens - t.first);
+        t.rb0 = t.rt * 8;
+    }
+    return t;
+}
+// Tokens of the first half (a multiple of 16) and of both.
+__device__ __forceinline__ int n_total(int n) { return (n + 15) & ~15; }
+__device__ __forceinline__ int n_first(int n) { return (n_total(n) / 2 + 15) & ~15; }
+
+__device__ __forceinline__ int64_t run_begin(int64_t units_all, int units, int64_t b, int ctas, bool split) {
+    return split ? units_all * b / ctas : units_all / units * b / ctas * units;
+}
+
+// NH: columns of the larger half's accumulator, in registers of the warps that promote it.
+template <typename T, int NH>
+__global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
+                                                              const __grid_constant__ TcParams p) {
+    // 640 threads start with 96 registers each; the promoting warps need an accumulator of up to 144 and take what the
+    // others give back: 256 x 176 + 256 x 48 + 128 x 32 = 640 x 96.
+    constexpr bool kSplitRegs = NH >= 64;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t s_tmem;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int SW = p.w_slots, SX = p.x_slots, SA = p.a_slots, NB = p.bufs;
+    const uint32_t sub_bytes = (uint32_t)p.x_rows * 128u, x_bytes = 2u * sub_bytes;
+    const uint32_t x_ring = base, w_ring = x_ring + SX * x_bytes, bars = w_ring + SW * kUnitBytes;
+    auto wfull = [&](int s) { return bars + 8u * s; };
+    auto wempty = [&](int s) { return bars + 8u * (kMaxW + s); };
+    auto xfull = [&](int s) { return bars + 8u * (2 * kMaxW + s); };
+    auto xempty = [&](int s) { return bars + 8u * (2 * kMaxW + kMaxX + s); };
+    auto afull = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + s); };
+    auto aempty = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + kMaxA + s); };
+    auto dfull = [&](int h, int b) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * b + h); };
+    auto dempty = [&](int h, int b) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * kMaxBuf + 2 * b + h); };
+    const uint32_t done = bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtl wc{&g_int4_error, &g_int4_failed_seq, p.wait_ns, p.seq};
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < SW; ++s) { mbar_init(wfull(s), 1); mbar_init(wempty(s), kBuildWarps); }
+        for (int s = 0; s < SX; ++s) { mbar_init(xfull(s), 1); mbar_init(xempty(s), 2); }
+        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kBuildWarps); mbar_init(aempty(s), 2); }
+        for (int b = 0; b < NB; ++b)
+            for (int h = 0; h < 2; ++h) { mbar_init(dfull(h, b), 1); mbar_init(dempty(h, b), 4); }
+        mbar_init(done, 2);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == kXWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    // The items are the previous kernel's; dense weights wait for nobody, and everything else for that kernel's end.
+    if (p.items || (warp != kWeightWarp && (warp < kBuildWarp || warp >= kWeightWarp)))
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t tiles = p.items ? (int64_t)*p.n_items * p.row_tiles : (int64_t)p.row_tiles * p.token_tiles;
+    const int64_t units_all = tiles * p.units;
+    const bool split = p.partial != nullptr;
+    const int64_t u0 = run_begin(units_all, p.units, blockIdx.x, p.ctas, split);
+    const int64_t u1 = run_begin(units_all, p.units, blockIdx.x + 1, p.ctas, split);
+    const int subs = 128 >> p.group_shift;               // groups a unit
+    // TMEM column of buffer b of half h: the same for every tile, so that one half may run ahead into the next tile
+    auto d_col = [&](int h, int b) { return (uint32_t)(b * p.n_max + h * n_first(p.n_max)); };
+
+    if (warp >= kWeightWarp) {
+        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == kWeightWarp) {
+            int slot = 0, used = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int64_t u = u0; u < u1 && ok;) {
+                const Tile t = tile_at(p, u, u1);
+                const int blocks = min(8, p.rbs - t.rt * 8);
+                const uint8_t* src = p.words + (t.rb0 + lane) * p.kbs * q4::kBlockBytes;
+                for (int k = t.k0; k < t.k1; ++k) {
+                    if (used >= SW && !(ok = wait_all(wempty(slot), ph ^ 1u, 1, wc))) break;
+                    const uint32_t bytes = 2 * k + 1 < p.kbs ? 2u * q4::kBlockBytes : (uint32_t)q4::kBlockBytes;
+                    if (lane == 0) mbar_expect_tx(wfull(slot), bytes * blocks);
+                    __syncwarp();
+                    if (lane < blocks)
+                        bulk_load(w_ring + slot * kUnitBytes + lane * 2 * q4::kBlockBytes,
+                                  src + (int64_t)k * 2 * q4::kBlockBytes, bytes, wfull(slot));
+                    ++used;
+                    advance(slot, ph, 1, SW);
+                }
+                u += t.k1 - t.k0;
+            }
+            // every copy issued must have landed before the CTA may exit: each slot's last one
+            for (int i = max(0, used - SW); i < used; ++i) mbar_drain(wfull(i % SW), (uint32_t)((i / SW) & 1), 2, wc);
+        } else if (warp == kXWarp) {
+            if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_x)) : "memory");
+            int slot = 0, used = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int64_t u = u0; u < u1 && ok;) {
+                const Tile t = tile_at(p, u, u1);
+                const int boxes = (n_total(t.n) + p.box_rows - 1) / p.box_rows;
+                for (int k = t.k0; k < t.k1; ++k) {
+                    if (used >= SX && !(ok = wait_all(xempty(slot), ph ^ 1u, 3, wc))) break;
+                    if (lane == 0) mbar_expect_tx(xfull(slot), (uint32_t)(2 * boxes * p.box_rows) * 128u);
+                    __syncwarp();
+                    for (int i = lane; i < 2 * boxes; i += 32) {
+                        const int s = i & 1, b = i >> 1;
+                        tma_load_2d(x_ring + slot * x_bytes + s * sub_bytes + b * p.box_rows * 128, &tmap_x,
+                                    k * 128 + s * 64, t.first + b * p.box_rows, xfull(slot));
+                    }
+                    ++used;
+                    advance(slot, ph, 1, SX);
+                }
+                u += t.k1 - t.k0;
+            }
+            for (int i = max(0, used - SX); i < used; ++i) mbar_drain(xfull(i % SX), (uint32_t)((i / SX) & 1), 4, wc);
+        } else {
+            const int h = warp - kMmaWarp;
+            if (lane == 0) {
+                int sa = 0, sx = 0, sb = 0, jobs = 0;
+                uint32_t pha = 0, phx = 0, phb = 0;
+                bool ok = true;
+                const int steps = 8 / subs;              // K = 16 products a group
+                for (int64_t u = u0; u < u1 && ok;) {
+                    const Tile t = tile_at(p, u, u1);
+                    const int n0 = n_first(t.n), n = h ? n_total(t.n) - n0 : n0;
+                    const uint32_t id = idesc_f16<T>(n ? n : 16);
+                    for (int k = t.k0; k < t.k1 && ok; ++k) {
+                        if (!(ok = mbar_wait(afull(sa), pha, 5, wc))) break;
+                        if (!(ok = mbar_wait(xfull(sx), phx, 6, wc))) break;
+                        tc_fence_after();
+                        const uint32_t a = tmem + (uint32_t)(p.a_col0 + sa * kACols);
+                        const uint64_t b0 = sw128_desc(x_ring + sx * x_bytes) + (uint64_t)((h * n0 * 128) >> 4);
+                        const uint64_t b1 = b0 + (uint64_t)(sub_bytes >> 4);
+                        for (int s = 0; s < subs; ++s) {
+                            if (jobs >= NB && !(ok = mbar_wait(dempty(h, sb), phb ^ 1u, 7, wc))) break;
+                            tc_fence_after();
+                            if (n) {
+                                const uint32_t d = tmem + d_col(h, sb);
+                                for (int i = 0; i < steps; ++i) {
+                                    const int kk = s * steps + i;
+                                    umma_f16_ts(d, a + 8u * kk, (kk < 4 ? b0 : b1) + 2 * (kk & 3), id, i ? 1u : 0u);
+                                }
+                            }
+                            umma_commit(dfull(h, sb));
+                            ++jobs;
+                            advance(sb, phb, 1, NB);
+                        }
+                        umma_commit(aempty(sa));
+                        umma_commit(xempty(sx));
+                        advance(sa, pha, 1, SA);
+                        advance(sx, phx, 1, SX);
+                    }
+                    u += t.k1 - t.k0;
+                }
+                umma_commit(done);
+                mbar_drain(done, 0, 8, wc);              // both issuers' products complete before TMEM is freed
+            }
+            __syncwarp();
+        }
+    } else if (warp >= kBuildWarp) {
+        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        const int w = warp - kBuildWarp, blk = 2 * (w & 3) + (w >> 2);          // lanes 32 (w % 4).. are this warp's
+        const uint32_t lanes = (uint32_t)(16 * blk) << 16;
+        int sw = 0, sa = 0, used = 0;
+        uint32_t phw = 0, pha = 0;
+        bool ok = true;
+        for (int64_t u = u0; u < u1 && ok;) {
+            const Tile t = tile_at(p, u, u1);
+            const int64_t rb = t.rb0 + min(blk, p.rbs - t.rt * 8 - 1);          // past the module: any codes do
+            const uint16_t* zrow = reinterpret_cast<const uint16_t*>(p.zeros) + rb * p.groups * 8 + (lane >> 2);
+            uint32_t z[4] = {0x0808u, 0x0808u, 0x0808u, 0x0808u};
+            auto load_zeros = [&](int k) {
+                if (!p.zeros) return;
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    if (s < subs) z[s] = __ldg(zrow + min(k * subs + s, p.groups - 1) * 8);
+            };
+            load_zeros(t.k0);
+            for (int k = t.k0; k < t.k1; ++k) {
+                if (!(ok = wait_all(wfull(sw), phw, 9, wc))) break;
+                const uint32_t at = w_ring + sw * kUnitBytes + blk * 2 * q4::kBlockBytes + lane * 16;
+                const uint4 c[2] = {lds_v4(at), lds_v4(at + q4::kBlockBytes)};
+                uint32_t zs[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) zs[s] = z[s];
+                if (k + 1 < t.k1) load_zeros(k + 1);
+                if (used >= SA && !(ok = wait_all(aempty(sa), pha ^ 1u, 10, wc))) break;
+                tc_fence_after();
+                q4::Codes<T> codes;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t words[4] = {c[half].x, c[half].y, c[half].z, c[half].w};
+                    uint32_t r[16];
+                    // groups of 128: one zero point a unit, 64: one a half, 32: one a quarter
+                    const uint32_t z0 = p.group_shift == 5 ? zs[2 * half] : p.group_shift == 6 ? zs[half] : zs[0];
+                    codes.zeros(z0 & 15u, z0 >> 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i == 2 && p.group_shift == 5) codes.zeros(zs[2 * half + 1] & 15u, zs[2 * half + 1] >> 8);
+                        uint32_t a[4];
+                        codes.expand(words[i], a);
+                        r[4 * i] = a[0]; r[4 * i + 1] = a[2]; r[4 * i + 2] = a[1]; r[4 * i + 3] = a[3];
+                    }
+                    tmem_st_16x256b_x4(tmem + lanes + (uint32_t)(p.a_col0 + sa * kACols + half * 32), r);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(wempty(sw));
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(afull(sa));
+                ++used;
+                advance(sw, phw, 1, SW);
+                advance(sa, pha, 1, SA);
+            }
+            u += t.k1 - t.k0;
+        }
+    } else {
+        if (kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int h = warp >> 2, q = warp & 3, row_in = 32 * q + lane;
+        T* y = reinterpret_cast<T*>(p.y);
+        int sb = 0;
+        uint32_t phb = 0;
+        bool ok = true;
+        for (int64_t u = u0; u < u1 && ok;) {
+            const Tile t = tile_at(p, u, u1);
+            const int n0 = n_first(t.n), nh = h ? n_total(t.n) - n0 : n0;
+            const int64_t rb = t.rb0 + min(row_in >> 4, p.rbs - t.rt * 8 - 1);
+            const uint16_t* srow = p.scales + rb * p.groups * 16 + 2 * (row_in & 7) + ((row_in >> 3) & 1);
+            uint64_t acc[NH / 2];
+#pragma unroll
+            for (int i = 0; i < NH / 2; ++i) acc[i] = 0;
+            const int g0 = t.k0 * subs, g1 = t.k1 * subs;
+            uint16_t sbits = __ldg(srow + (int64_t)min(g0, p.groups - 1) * 16);
+            for (int g = g0; g < g1; ++g) {
+                const float s = to_f32(*reinterpret_cast<const T*>(&sbits));
+                uint64_t s2;
+                asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(s)));
+                if (g + 1 < g1) sbits = __ldg(srow + (int64_t)min(g + 1, p.groups - 1) * 16);
+                if (!(ok = wait_all(dfull(h, sb), phb, 11, wc))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + d_col(h, sb);
+                uint32_t v[2][16];
+                if (nh > 0) ld16_async(d, v[0]);
+#pragma unroll
+                for (int c = 0; c < NH / 16; ++c) {
+                    if (c * 16 < nh) {
+                        ld16_wait(v[c & 1]);
+                        if ((c + 1) * 16 < nh) ld16_async(d + (c + 1) * 16, v[(c + 1) & 1]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], s2, v[c & 1][2 * i], v[c & 1][2 * i + 1]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(dempty(h, sb));
+                advance(sb, phb, 1, NB);
+            }
+            if (!ok) break;
+            const int left = min(nh, t.n - h * n0);      // this half's tokens
+            if (t.k1 - t.k0 < p.units) {                 // shared with the neighbouring run
+                float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 +
+                              (int64_t)h * n0 * 128 + row_in;
+#pragma unroll
+                for (int c = 0; c < NH; ++c)
+                    if (c < left) part[c * 128] = half_of(acc[c / 2], c & 1);
+            } else if (p.gated) {
+                // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each pair of
+                // lanes exchanges one of two columns and finishes the other.
+                const int64_t row = (int64_t)t.rt * 64 + 16 * q + (lane & 15);
+#pragma unroll
+                for (int c = 0; c < NH; c += 2) {
+                    if (c >= left) continue;
+                    const float mine = half_of(acc[c / 2], lane >> 4), send = half_of(acc[c / 2], (lane >> 4) ^ 1);
+                    const float other = __shfl_xor_sync(0xffffffffu, send, 16);
+                    const float gate = lane < 16 ? mine : other, up = lane < 16 ? other : mine;
+                    const int col = c + (lane >> 4);
+                    if (col < left && row < p.out_rows)
+                        y[(int64_t)(t.first + h * n0 + col) * p.ldy + row] =
+                            from_f32<T>(gate / (1.f + expf(-gate)) * up);
+                }
+            } else {
+                const int64_t row = (int64_t)t.rt * 128 + row_in;
+                if (row < p.out_rows) {
+                    T* out = y + (int64_t)(t.first + h * n0) * p.ldy + row;
+#pragma unroll
+                    for (int c = 0; c < NH; ++c)
+                        if (c < left) out[c * p.ldy] = from_f32<T>(half_of(acc[c / 2], c & 1));
+                }
+            }
+            u += t.k1 - t.k0;
+        }
+        if (p.routed) {                                  // what lies behind the last pair
+            for (int64_t r = *p.routed + blockIdx.x; r < p.pairs; r += p.ctas)
+                for (int c = threadIdx.x; c < p.out_rows; c += kPromoteWarps * 32) y[r * p.ldy + c] = from_f32<T>(0.f);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kXWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+}
+
+// Row tiles that several runs share: their fp32 partials added in run order. A block takes one row tile and 8 tokens,
+// a thread one row.
+constexpr int kJoinTokens = 8;
+template <typename T> __global__ void __launch_bounds__(128) int4_join_kernel(const __grid_constant__ TcParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t tile = blockIdx.x, units_all = (int64_t)p.row_tiles * p.token_tiles * p.units;
+    const int64_t a = tile * p.units, z = a + p.units;
+    const auto begin = [&](int64_t b) { return run_begin(units_all, p.units, b, p.ctas, true); };
+    // the run that holds unit u: the last b whose begin is at most u
+    const auto run_of = [&](int64_t u) { return ((u + 1) * p.ctas + units_all - 1) / units_all - 1; };
+    const int64_t b0 = run_of(a), b1 = run_of(z - 1);
+    if (b0 == b1) return;                                // one run wrote y itself
+    const Tile t = tile_at(p, a, z);
+    const int row_in = threadIdx.x, lane = threadIdx.x & 31, q = threadIdx.x >> 5;
+    const int c0 = blockIdx.y * kJoinTokens;
+    float acc[kJoinTokens];
+#pragma unroll
+    for (int c = 0; c < kJoinTokens; ++c) acc[c] = 0.f;
+    for (int64_t b = b0; b <= b1; ++b) {
+        const float* part = p.partial + (b * 2 + (begin(b) >= a ? 0 : 1)) * p.n_max * 128 + row_in;
+#pragma unroll
+        for (int c = 0; c < kJoinTokens; ++c)
+            if (c0 + c < t.n) acc[c] += __ldcg(part + (int64_t)(c0 + c) * 128);
+    }
+    T* y = reinterpret_cast<T*>(p.y);
+#pragma unroll
+    for (int c = 0; c < kJoinTokens; ++c) {
+        if (c0 + c >= t.n) break;
+        T* out = y + (int64_t)(t.first + c0 + c) * p.ldy;
+        if (p.gated) {
+            const float up = __shfl_xor_sync(0xffffffffu, acc[c], 16);
+            const int64_t row = (int64_t)t.rt * 64 + 16 * q + (lane & 15);
+            if (lane < 16 && row < p.out_rows) out[row] = from_f32<T>(acc[c] / (1.f + expf(-acc[c])) * up);
+        } else {
+            const int64_t row = (int64_t)t.rt * 128 + row_in;
+            if (row < p.out_rows) out[row] = from_f32<T>(acc[c]);
+        }
+    }
+}
+
+unsigned next_seq() {
+    static std::atomic<unsigned> counter{0};
+    unsigned v = ++counter;
+    while (v == 0) v = ++counter;
+    return v;
+}
+
+// What a launch of at most `most` tokens a tile takes: accumulator columns, rings.
+struct TcPlan {
+    int nh, n_max, x_rows, box_rows, bufs, a_col0, a_slots, x_slots, w_slots, smem;
+};
+
+int bucket(int n_half) { return n_half <= 16 ? 16 : n_half <= 32 ? 32 : n_half <= 64 ? 64 : n_half <= 96 ? 96 : 144; }
+
+TcPlan plan_tc(int most, bool routed) {
+    TcPlan pl;
+    const int total = (most + 15) / 16 * 16, half = (total / 2 + 15) / 16 * 16;
+    pl.nh = bucket(half);
+    pl.n_max = total;
+    pl.x_rows = total;
+    // a routed item's x rows end anywhere: boxes of 16 rows follow it; a dense tile is one box, or two above 256 rows
+    pl.box_rows = routed ? 16 : total <= 256 ? total : total / 2;
+    pl.bufs = 2 * total + 2 * kACols <= kTmemCols ? 2 : 1;
+    pl.a_col0 = (pl.bufs * total + 31) / 32 * 32;
+    pl.a_slots = (kTmemCols - pl.a_col0) / kACols;
+    if (pl.a_slots > kMaxA) pl.a_slots = kMaxA;
+    const int x_bytes = 2 * pl.x_rows * 128, bar_bytes = 8 * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + 1);
+    pl.w_slots = kMaxW;
+    int room = kSmemLimit - 1024 - bar_bytes - pl.w_slots * kUnitBytes;
+    pl.x_slots = room / x_bytes;
+    if (pl.x_slots > kMaxX) pl.x_slots = kMaxX;
+    pl.smem = 1024 + pl.x_slots * x_bytes + pl.w_slots * kUnitBytes + bar_bytes;
+    return pl;
+}
+
+template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
+    auto kernel = int4_tc_kernel<T, NH>;
+    if (int e = allow_smem((const void*)kernel, smem, what)) return e;
+    if (NH >= 64) {                                      // the register split needs what it was written for
+        static std::atomic<int> regs{0};
+        if (regs == 0) {
+            cudaFuncAttributes a;
+            if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess)
+                return fail(P2P_ECUDA, "%s: %s", what, cudaGetErrorString(cudaGetLastError()));
+            regs = a.numRegs;
+        }
+        if (regs * kThreads < 256 * 176 + 256 * 48 + 128 * 32)
+            return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread, 96 needed", what, regs.load());
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)p.ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, map, p);
+    if (int e = launch_status(what)) return e;
+    if (!p.partial) return P2P_OK;
+    cfg.gridDim = dim3((unsigned)(p.row_tiles * p.token_tiles), (unsigned)((p.tile_tokens + kJoinTokens - 1) / kJoinTokens));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cudaLaunchKernelEx(&cfg, int4_join_kernel<T>, p);
+    return launch_status(what);
+}
+
+template <typename T> int launch_nh(int nh, const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
+    switch (nh) {
+        case 16: return launch_tc<T, 16>(map, p, smem, st, what);
+        case 32: return launch_tc<T, 32>(map, p, smem, st, what);
+        case 64: return launch_tc<T, 64>(map, p, smem, st, what);
+        case 96: return launch_tc<T, 96>(map, p, smem, st, what);
+        default: return launch_tc<T, 144>(map, p, smem, st, what);
+    }
+}
+
+// Token tiles of a dense call: as even as they divide, at most 272 tokens each.
+int64_t token_tiles(int64_t tokens) { return (tokens + kInt4TileTokens - 1) / kInt4TileTokens; }
+int tile_tokens(int64_t tokens) {
+    const int64_t n = token_tiles(tokens);
+    return (int)((tokens + n - 1) / n);
+}
+// CTAs of a dense call, and whether they split row tiles: not where whole tiles leave at most a tenth of them idle.
+int dense_ctas(int64_t tiles, int64_t units, bool* split) {
+    const int64_t sms = sm_count(), waves = (tiles + sms - 1) / sms;
+    *split = waves * sms * 10 > tiles * 11;
+    const int64_t most = *split ? tiles * units : tiles;
+    return (int)(most < sms ? most : sms);
+}
+
+}  // namespace
+
+size_t int4_tc_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated) {
+    const int64_t row_tiles = q4::div_up(q4::row_blocks(rows, gated), 8), units = q4::div_up(cols, 128);
+    bool split;
+    const int ctas = dense_ctas(row_tiles * token_tiles(tokens), units, &split);
+    if (!split) return 0;
+    return (size_t)ctas * 2 * ((tile_tokens(tokens) + 15) / 16 * 16) * 128 * sizeof(float);
+}
+
+int int4_tc_run(const Int4Call& c, void* workspace, cudaStream_t st, const char* what) {
+    TcParams p = {};
+    const bool routed = c.items != nullptr;
+    const int most = routed ? (int)c.item_tokens : tile_tokens(c.tokens);
+    const TcPlan pl = plan_tc(most, routed);
+    p.words = reinterpret_cast<const uint8_t*>(c.words);
+    p.scales = reinterpret_cast<const uint16_t*>(c.scales);
+    p.zeros = c.zeros;
+    p.rows = (int)c.rows;
+    p.out_rows = (int)(c.gated ? c.rows / 2 : c.rows);
+    p.rbs = (int)q4::row_blocks(c.rows, c.gated);
+    p.row_tiles = (int)q4::div_up(p.rbs, 8);
+    p.kbs = (int)q4::div_up(c.cols, q4::kCols);
+    p.units = (int)q4::div_up(c.cols, 128);
+    p.groups = (int)q4::div_up(c.cols, c.group);
+    p.group_shift = c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
+    p.gated = c.gated;
+    p.tokens = (int)c.tokens;
+    p.tile_tokens = routed ? most : tile_tokens(c.tokens);
+    p.token_tiles = routed ? 1 : (int)token_tiles(c.tokens);
+    p.items = c.items;
+    p.n_items = c.n_items;
+    p.routed = c.routed;
+    p.pairs = c.pairs;
+    p.y = c.y;
+    p.ldy = c.ldy;
+    p.n_max = pl.n_max;
+    bool split = false;
+    if (routed) {
+        const int64_t tiles = c.max_items * p.row_tiles;
+        p.ctas = (int)(tiles < sm_count() ? tiles : sm_count());
+    } else {
+        p.ctas = dense_ctas((int64_t)p.row_tiles * p.token_tiles, p.units, &split);
+    }
+    p.partial = split ? reinterpret_cast<float*>(workspace) : nullptr;
+    p.x_rows = pl.x_rows;
+    p.box_rows = pl.box_rows;
+    p.w_slots = pl.w_slots;
+    p.x_slots = pl.x_slots;
+    p.a_slots = pl.a_slots;
+    p.bufs = pl.bufs;
+    p.a_col0 = pl.a_col0;
+    p.wait_ns = kWaitNs;
+    p.seq = next_seq();
+    CUtensorMap map;
+    if (int e = encode_x_map(&map, c.x, c.dtype, routed ? c.pairs : c.tokens, c.cols, c.ldx, pl.box_rows)) return e;
+    return c.dtype == P2P_BF16 ? launch_nh<__nv_bfloat16>(pl.nh, map, p, pl.smem, st, what)
+                               : launch_nh<__half>(pl.nh, map, p, pl.smem, st, what);
+}
+
+}  // namespace p2p
+
+using namespace p2p;
+
+extern "C" int p2p_int4_status(int reset, void* stream) {
+    cudaStream_t st = as_stream(stream);
+    int v = 0;
+    if (cudaMemcpyFromSymbolAsync(&v, g_int4_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+        cudaStreamSynchronize(st) != cudaSuccess)
+        return fail(P2P_ECUDA, "p2p_int4_status: %s", cudaGetErrorString(cudaGetLastError()));
+    if (reset && v) {
+        const int zero = 0;
+        cudaMemcpyToSymbolAsync(g_int4_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+        cudaStreamSynchronize(st);
+    }
+    if (v) return fail(P2P_ECUDA, "p2p_int4: a pipeline wait timed out (site %d)", v);
+    return P2P_OK;
+}

@@ -121,7 +121,7 @@ class TokenOrder:
     order: torch.Tensor           # int32 [T K]: the pair token * K + slot at each place, -1 behind the last
     where: torch.Tensor           # int32 [T K]: each pair's place, -1 if it is routed nowhere
     offsets: torch.Tensor         # int32 [experts + 1]: each expert's first place, then the number of routed pairs
-    items: torch.Tensor           # int32 [.., 4]: {expert, first place, places, 0}, runs of at most 32 places
+    items: torch.Tensor           # int32 [.., 4]: {expert, first place, places, 0}, runs of one expert's places
     n_items: torch.Tensor         # int32 [1]
     tokens: int
     topk: int
@@ -199,8 +199,8 @@ class Int4Experts:
         _check_rows(x, order, order.tokens if gather else pairs)
         if order.experts != self.experts:
             raise P2PError(f"an order of {order.experts} experts, weights of {self.experts}")
-        args = (x, q.words, q.scales, q.zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order, order.offsets,
-                order.items, order.n_items, order.topk, gather)
+        args = (x, q.words, q.scales, q.zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order, order.where,
+                order.offsets, order.items, order.n_items, order.topk, gather)
         if out is None:
             return _lib.ops().int4_grouped(*args)
         out = kernels._out(out, (pairs, q.rows // 2 if q.gated else q.rows), x)

@@ -12,14 +12,32 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr int64_t kItemTokens = 32;                   // places of one item: what a block of the grouped product takes
+constexpr int64_t kSmallTokens = 8;                   // up to here the products take x rows of any alignment and order
+
+// Places of one item, what one pass over an expert's weights takes: few where experts have few pairs on average, so
+// that a tile is not mostly empty; otherwise as many as keep the weights' codes from being turned twice.
+int64_t item_tokens(int64_t pairs, int64_t experts) {
+    if (pairs <= kSmallTokens) return kSmallTokens;
+    const int64_t mean = pairs / experts;
+    return mean <= 8 ? 32 : mean <= 64 ? 128 : 256;
+}
 
 // t [rows, cols] with unit column stride and rows that do not overlap (an expanded gradient's do).
 at::Tensor rows2d(const at::Tensor& t) {
     const bool cols_ok = t.size(1) <= 1 || t.stride(1) == 1, rows_ok = t.size(0) <= 1 || t.stride(0) >= t.size(1);
     return cols_ok && rows_ok ? t : t.contiguous();
 }
+// t with rows that start on 16-byte boundaries; the columns that a copy's stride adds are never read.
+at::Tensor aligned_rows(const at::Tensor& t) {
+    const at::Tensor r = rows2d(t);
+    if (reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 && (r.size(0) <= 1 || r.stride(0) % 8 == 0)) return r;
+    at::Tensor copy = at::empty({r.size(0), (r.size(1) + 7) / 8 * 8}, r.options()).narrow(1, 0, r.size(1));
+    copy.copy_(r);
+    return copy;
+}
 int64_t row_stride(const at::Tensor& t) { return std::max(t.size(0) <= 1 ? (int64_t)0 : t.stride(0), t.size(1)); }
+// The same, rounded up to 8 elements where one row stands alone.
+int64_t aligned_stride(const at::Tensor& t) { return t.size(0) <= 1 ? (t.size(1) + 7) / 8 * 8 : t.stride(0); }
 
 void check_matrix(const at::Tensor& t, const char* what) {
     TORCH_CHECK(t.is_cuda(), "p2p_b200: ", what, ": CUDA tensors only (the replica path has no CPU fallback)");
@@ -31,6 +49,8 @@ const int32_t* ints(const at::Tensor& t, const at::Tensor& like, int64_t n, cons
                 "p2p_b200: ", what, " is not a contiguous int32 tensor of ", n, " on ", like.device());
     return t.data_ptr<int32_t>();
 }
+
+at::Tensor moe_spread(const at::Tensor& x_in, const at::Tensor& where, const at::Tensor& offsets, int64_t topk);
 
 // ---- 4-bit products --------------------------------------------------------------------------------------------------
 
@@ -68,9 +88,13 @@ void int4_mm_into(const at::Tensor& x_in, const at::Tensor& words, const at::Ten
     check_int4(x_in, words, scales, zeros, 1, rows, cols, group, gated);
     check_rows_out(out, x_in, x_in.size(0), gated ? rows / 2 : rows);
     const c10::cuda::CUDAGuard guard(x_in.device());
-    const at::Tensor x = rows2d(x_in);
-    check(p2p_int4_mm(x.data_ptr(), dtype_code(x), x.size(0), cols, row_stride(x), words.data_ptr(), scales.data_ptr(),
-                      bytes(zeros), rows, (int)group, gated, out.data_ptr(), row_stride(out), stream_of(x)),
+    const bool small = x_in.size(0) <= kSmallTokens;
+    const at::Tensor x = small ? rows2d(x_in) : aligned_rows(x_in);
+    const size_t need = p2p_int4_workspace(x.size(0), rows, cols, gated);
+    const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte)) : at::Tensor();
+    check(p2p_int4_mm(x.data_ptr(), dtype_code(x), x.size(0), cols, small ? row_stride(x) : aligned_stride(x),
+                      words.data_ptr(), scales.data_ptr(), bytes(zeros), rows, (int)group, gated, out.data_ptr(),
+                      row_stride(out), need ? ws.data_ptr() : nullptr, need, stream_of(x)),
           "p2p_int4_mm");
 }
 
@@ -84,7 +108,7 @@ at::Tensor int4_mm(const at::Tensor& x, const at::Tensor& words, const at::Tenso
 
 void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& words, const at::Tensor& scales,
                       const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
-                      int64_t group, bool gated, const at::Tensor& order, const at::Tensor& offsets,
+                      int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
                       const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
                       const at::Tensor& out, bool zero_behind) {
     check_int4(x_in, words, scales, zeros, experts, rows, cols, group, gated);
@@ -93,35 +117,38 @@ void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& words, const at:
                 x_in.size(0), " rows, the order is of ", pairs, " pairs, ", topk, " a token");
     check_rows_out(out, x_in, pairs, gated ? rows / 2 : rows);
     const c10::cuda::CUDAGuard guard(x_in.device());
-    const at::Tensor x = rows2d(x_in);
-    const int32_t* at_order = ints(order, x, pairs, "order");
-    const int32_t* at_offsets = ints(offsets, x, experts + 1, "offsets");
+    const int32_t* at_order = ints(order, x_in, pairs, "order");
+    const int32_t* at_offsets = ints(offsets, x_in, experts + 1, "offsets");
     TORCH_CHECK(offsets.numel() == experts + 1, "p2p_b200: the order is of ", offsets.numel() - 1, " experts, the weights of ",
                 experts);
-    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, row_stride(x), words.data_ptr(), scales.data_ptr(),
+    if (pairs == 0) return;
+    const int64_t most = item_tokens(pairs, experts);
+    const bool small = most <= kSmallTokens, in_place = small || !gather;
+    const at::Tensor x = small ? rows2d(x_in) : aligned_rows(gather ? moe_spread(x_in, where, offsets, topk) : x_in);
+    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, small ? row_stride(x) : aligned_stride(x), words.data_ptr(), scales.data_ptr(),
                            bytes(zeros), rows, (int)group, gated, ints(items, x, 0, "items"),
-                           ints(n_items, x, 1, "n_items"), items.numel() / 4, std::min(pairs, kItemTokens),
-                           gather ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
+                           ints(n_items, x, 1, "n_items"), items.numel() / 4, most,
+                           gather && in_place ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
                            out.data_ptr(), row_stride(out), stream_of(x)),
           "p2p_int4_grouped");
 }
 
 void int4_grouped_into(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
                        const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
-                       int64_t group, bool gated, const at::Tensor& order, const at::Tensor& offsets,
+                       int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
                        const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
                        const at::Tensor& out) {
-    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, offsets, items, n_items, topk,
+    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk,
                      gather, out, false);
 }
 
 at::Tensor int4_grouped(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
                         const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
-                        int64_t group, bool gated, const at::Tensor& order, const at::Tensor& offsets,
+                        int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
                         const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather) {
     check_matrix(x, "x");
     at::Tensor out = at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
-    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, offsets, items, n_items, topk,
+    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk,
                      gather, out, true);
     return out;
 }
@@ -129,7 +156,8 @@ at::Tensor int4_grouped(const at::Tensor& x, const at::Tensor& words, const at::
 // ---- tokens sorted by expert and back --------------------------------------------------------------------------------
 
 int64_t max_items(int64_t pairs, int64_t experts) {
-    return std::min(pairs, (pairs + kItemTokens - 1) / kItemTokens + experts);
+    const int64_t most = item_tokens(pairs, experts);
+    return std::min(pairs, (pairs + most - 1) / most + experts);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& ids_in, int64_t experts) {
@@ -146,7 +174,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(
                n_items = all.narrow(0, 4 * most + 2 * n + experts + 1, 1);
     check(p2p_moe_sort(ids.data_ptr(), (int)ids.element_size(), n, (int)experts, order.data_ptr<int32_t>(),
                        where.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), items.data_ptr<int32_t>(), most,
-                       (int)kItemTokens, n_items.data_ptr<int32_t>(), stream_of(ids)),
+                       (int)item_tokens(n, experts), n_items.data_ptr<int32_t>(), stream_of(ids)),
           "p2p_moe_sort");
     return {order, where, offsets, items, n_items};
 }
@@ -302,12 +330,12 @@ void int4_mm_into_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, 
                        int64_t, int64_t, int64_t, bool, const at::Tensor&) {}
 at::Tensor int4_grouped_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
                              int64_t, int64_t rows, int64_t, int64_t, bool gated, const at::Tensor& order,
-                             const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool) {
+                             const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool) {
     return at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
 }
 void int4_grouped_into_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
                             int64_t, int64_t, int64_t, int64_t, bool, const at::Tensor&, const at::Tensor&,
-                            const at::Tensor&, const at::Tensor&, int64_t, bool, const at::Tensor&) {}
+                            const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool, const at::Tensor&) {}
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort_meta(const at::Tensor& ids, int64_t experts) {
     const auto o = ids.options().dtype(at::kInt);
     const int64_t n = ids.numel();
@@ -333,9 +361,9 @@ TORCH_LIBRARY_FRAGMENT(p2p_b200, m) {
     m.def("int4_mm_into(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int rows, int cols, int group, bool gated, "
           "Tensor(a!) out) -> ()");
     m.def("int4_grouped(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int experts, int rows, int cols, int group, "
-          "bool gated, Tensor order, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather) -> Tensor");
+          "bool gated, Tensor order, Tensor where, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather) -> Tensor");
     m.def("int4_grouped_into(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int experts, int rows, int cols, "
-          "int group, bool gated, Tensor order, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather, "
+          "int group, bool gated, Tensor order, Tensor where, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather, "
           "Tensor(a!) out) -> ()");
     m.def("moe_sort(Tensor ids, int experts) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("moe_spread(Tensor x, Tensor where, Tensor offsets, int topk) -> Tensor");

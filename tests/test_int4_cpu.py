@@ -31,18 +31,24 @@ def test_row_blocks(lib):
     (lambda l: l.p2p_int4_layout(FAKE, FAKE, None, 1, 3, 64, 64, 1, FAKE, FAKE, None, None), -1, b"shape"),
     (lambda l: l.p2p_int4_layout(FAKE, FAKE, FAKE, 1, 4, 64, 64, 0, FAKE, FAKE, None, None), -1, b"null"),
     (lambda l: l.p2p_int4_layout(FAKE, FAKE, None, 1, 4, 64, 64, 0, FAKE + 8, FAKE, None, None), -1, b"16-byte"),
-    (lambda l: l.p2p_int4_mm(FAKE, 2, 4, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None), -2, b"bf16 or f16"),
-    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 63, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None), -1, b"stride"),
-    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 15, None), -1, b"stride"),
-    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE, FAKE, None, 15, 64, 1, FAKE, 16, None), -1, b"gated"),
-    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE + 4, FAKE, None, 16, 64, 0, FAKE, 16, None), -1, b"16-byte"),
-    (lambda l: l.p2p_int4_mm(None, 0, 4, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None), -1, b"null"),
-    (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, FAKE, 4, 33, None, 1, None, 4,
-                                  FAKE, 16, None), -1, b"at most 32"),
+    (lambda l: l.p2p_int4_mm(FAKE, 2, 4, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None, 0, None), -2, b"bf16 or f16"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 63, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"stride"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 15, None, 0, None), -1, b"stride"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE, FAKE, None, 15, 64, 1, FAKE, 16, None, 0, None), -1, b"gated"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE + 4, FAKE, None, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"16-byte"),
+    (lambda l: l.p2p_int4_mm(None, 0, 4, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"null"),
+    (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, FAKE, 4, 273, None, 1, None, 4,
+                                  FAKE, 16, None), -1, b"at most 272"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE + 4, FAKE, 4, 8, None, 1, None, 4,
                                   FAKE, 16, None), -1, b"16-byte"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, FAKE, 4, 8, FAKE, 0, None, 4,
                                   FAKE, 16, None), -1, b"topk"),
+    (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, FAKE, 4, 9, FAKE, 1, None, 4,
+                                  FAKE, 16, None), -1, b"in the order's places"),
+    (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 68, FAKE, FAKE, None, 16, 64, 0, FAKE, FAKE, 4, 9, None, 1, None, 4,
+                                  FAKE, 16, None), -1, b"16-byte"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 9, 64, 68, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"16-byte"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 9, 64, 64, FAKE, FAKE, None, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"workspace"),
     (lambda l: l.p2p_moe_sort(FAKE, 4, 64, 1025, FAKE, FAKE, FAKE, FAKE, 2000, 32, FAKE, None), -2, b"at most 1024"),
     (lambda l: l.p2p_moe_sort(FAKE, 2, 64, 8, FAKE, FAKE, FAKE, FAKE, 64, 32, FAKE, None), -1, b"4 or 8"),
     (lambda l: l.p2p_moe_sort(FAKE, 4, 64, 8, FAKE, FAKE, FAKE, FAKE, 9, 32, FAKE, None), -1, b"10 needed"),
@@ -62,7 +68,7 @@ def test_entries_refuse_bad_arguments(lib, call, status, needle):
 
 def test_empty_work_launches_nothing(lib):
     assert lib.p2p_int4_quantize(None, 0, 0, 64, 64, 64, None, None, None, None) == 0
-    assert lib.p2p_int4_mm(None, 0, 0, 64, 64, None, None, None, 16, 64, 0, None, 16, None) == 0
+    assert lib.p2p_int4_mm(None, 0, 0, 64, 64, None, None, None, 16, 64, 0, None, 16, None, 0, None) == 0
     assert lib.p2p_int4_grouped(None, 0, 64, 64, None, None, None, 16, 64, 0, None, None, 0, 0, None, 1, None, 0, None,
                                 16, None) == 0
     assert lib.p2p_moe_spread(None, 0, 0, 2, 8, 8, None, None, None, 8, None) == 0
@@ -77,7 +83,7 @@ def test_operators_propagate_shapes_on_meta_tensors(lib):
     assert ops.int4_mm(meta(17, 64), w, s, None, 40, 64, 64, True).shape == (17, 20)
     order, where, offsets, items, n = ops.moe_sort(meta(17, 8, dtype=torch.int64), 128)
     assert order.shape == where.shape == (136,) and offsets.shape == (129,) and items.shape == (4 * 133,) and n.shape == (1,)
-    assert ops.int4_grouped(meta(17, 64), w, s, None, 128, 40, 64, 64, True, order, offsets, items, n, 8, True).shape == (136, 20)
+    assert ops.int4_grouped(meta(17, 64), w, s, None, 128, 40, 64, 64, True, order, where, offsets, items, n, 8, True).shape == (136, 20)
     x = meta(17, 96).requires_grad_(True)
     xs = ops.moe_spread(x, where, offsets, 8)
     assert xs.shape == (136, 96) and xs.requires_grad
