@@ -342,17 +342,14 @@ int p2p_int4_quantize(const void* w, int dtype, int64_t rows, int64_t cols, int6
 int p2p_int4_expand(const uint8_t* codes, const void* scales, const uint8_t* zeros, int dtype, int64_t rows,
                     int64_t cols, int group, void* dense, void* stream);
 
-/* Row blocks (16 rows) of one expert in the layout: ceil(rows / 16), of a gated module 2 ceil(rows / 2 / 16); -1 for
- * rows below zero or an odd gated count. */
-int64_t p2p_int4_row_blocks(int64_t rows, int gated);
+/* Bytes of the layout that the products read, codes, scales and zero points in one; -1 for arguments out of range. */
+int64_t p2p_int4_layout_bytes(int64_t experts, int64_t rows, int64_t cols, int group, int has_zeros, int gated);
 
-/* Codes, scales and zero points (contiguous, [experts, rows, ..]) into the layout that the products read: words of
- * experts x row blocks x ceil(cols / 64) x 512 bytes (16-byte aligned), out_scales and out_zeros of experts x row
- * blocks x ceil(cols / group) x 16. gated: the first half of an expert's rows is the gate, the second the up
- * projection. Load time; synchronise before the layout is used. */
+/* Codes, scales and zero points (contiguous, [experts, rows, ..]) into that layout (16-byte aligned). gated: the first
+ * half of an expert's rows is the gate, the second the up projection. Load time; synchronise before the layout is
+ * used. */
 int p2p_int4_layout(const uint8_t* codes, const void* scales, const uint8_t* zeros, int64_t experts, int64_t rows,
-                    int64_t cols, int group, int gated, void* words, void* out_scales, uint8_t* out_zeros,
-                    void* stream);
+                    int64_t cols, int group, int gated, void* layout, void* stream);
 
 /* Bytes of workspace p2p_int4_mm needs (0: none). Calls that share one must not overlap on the GPU; it needs no
  * zeroing. */
@@ -363,17 +360,16 @@ size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated)
  * fp32; no weight is rounded. Any tokens, rows and cols; above 8 tokens x's rows start on 16-byte boundaries (ldx a
  * multiple of 8). As the other GEMMs, a programmatic dependent of the stream's previous kernel that reads its weights
  * before that kernel completes. */
-int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* words,
-                const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated, void* y, int64_t ldy,
-                void* workspace, size_t workspace_bytes, void* stream);
+int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout, int has_zeros,
+                int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                void* stream);
 
 /* The same for routed experts: y [pairs, rows] (gated: rows / 2), row p being x's row times the weights of the expert
  * whose item holds place p. items, n_items: p2p_moe_sort's, of at most item_tokens <= 272 places each. x's row of
  * place p is p itself, or with items of at most 8 places, where order is not null, order[p] / topk; above 8 places x's
  * rows start on 16-byte boundaries. routed: null, or the number of routed pairs on the device: rows from there to
  * `pairs` become zero (null: they stay as they were). */
-int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* words, const void* scales,
-                     const uint8_t* zeros, int64_t rows, int group, int gated, const int32_t* items,
+int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout, int has_zeros, int64_t rows, int group, int gated, const int32_t* items,
                      const int32_t* n_items, int64_t max_items, int64_t item_tokens, const int32_t* order, int topk,
                      const int32_t* routed, int64_t pairs, void* y, int64_t ldy, void* stream);
 

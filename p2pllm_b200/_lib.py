@@ -80,13 +80,13 @@ SIGNATURES = {
     "p2p_moe_combine": ([_vp, _int, _i64, _vp, _vp, _i64, _int, _i64, _vp, _i64, _vp], _int),
     "p2p_int4_quantize": ([_vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp], _int),
     "p2p_int4_expand": ([_vp, _vp, _vp, _int, _i64, _i64, _int, _vp, _vp], _int),
-    "p2p_int4_row_blocks": ([_i64, _int], _i64),
-    "p2p_int4_layout": ([_vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp], _int),
+    "p2p_int4_layout_bytes": ([_i64, _i64, _i64, _int, _int, _int], _i64),
+    "p2p_int4_layout": ([_vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp], _int),
     "p2p_int4_workspace": ([_i64, _i64, _i64, _int], _sz),
-    "p2p_int4_mm": ([_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _int, _int, _vp, _i64, _vp, _sz, _vp], _int),
+    "p2p_int4_mm": ([_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _i64, _vp, _sz, _vp], _int),
     "p2p_int4_status": ([_int, _vp], _int),
-    "p2p_int4_grouped": ([_vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _int, _int, _vp, _vp, _i64, _i64, _vp, _int, _vp,
-                          _i64, _vp, _i64, _vp], _int),
+    "p2p_int4_grouped": ([_vp, _int, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _vp, _i64, _i64, _vp, _int, _vp, _i64,
+                          _vp, _i64, _vp], _int),
     "p2p_moe_sort": ([_vp, _int, _i64, _int, _vp, _vp, _vp, _vp, _i64, _int, _vp, _vp], _int),
     "p2p_moe_spread": ([_vp, _int, _i64, _int, _i64, _i64, _vp, _vp, _vp, _i64, _vp], _int),
     "p2p_moe_sum": ([_vp, _int, _i64, _int, _i64, _i64, _vp, _vp, _int, _vp, _i64, _vp], _int),

@@ -90,50 +90,54 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* __restrict__
     }
 }
 
-// One thread a word of the layout; the threads past the words take the scales.
+// One thread a 32-bit word of the layout: eight codes, four zero points or two scales.
 __global__ void __launch_bounds__(256) layout_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales,
                                                      const uint8_t* __restrict__ zeros, int64_t experts, int64_t rows,
-                                                     int cols, int group, int gated, uint32_t* __restrict__ words,
-                                                     uint16_t* __restrict__ out_scales, uint8_t* __restrict__ out_zeros) {
-    const int64_t rbs = q4::row_blocks(rows, gated), kbs = q4::div_up(cols, q4::kCols);
-    const int64_t groups = q4::div_up(cols, group), n_bytes = q4::div_up(cols, 2);
-    const int64_t n_words = experts * rbs * kbs * 128, n_scales = experts * rbs * groups * 16;
-    const int64_t half = rows / 2;
+                                                     int cols, int group, int gated, uint32_t* __restrict__ out) {
+    const int64_t tiles = q4::row_tiles(rows, gated), units = q4::div_up(cols, q4::kUnitCols);
+    const int64_t groups = q4::div_up(cols, group), n_bytes = q4::div_up(cols, 2), half = rows / 2;
+    const int subs = q4::kUnitCols / group, zero_words = q4::unit_zero_bytes(group, zeros != nullptr) / 4;
+    const int code_words = q4::kCodeBytes / 4, record = q4::unit_bytes(group, zeros != nullptr) / 4;
     // the source row of row `in` of row block rb, or -1 for padding
     auto source = [&](int64_t rb, int in) -> int64_t {
         const int64_t r = (gated ? rb / 2 : rb) * q4::kRows + in;
         if (gated) return r < half ? r + (rb & 1) * half : -1;
         return r < rows ? r : -1;
     };
-    const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n_words + n_scales; i += stride) {
-        if (i < n_words) {
-            const int r = (int)(i & 3), lane = (int)((i >> 2) & 31);
-            const int64_t blk = i >> 7, kb = blk % kbs, rb = blk / kbs % rbs, e = blk / kbs / rbs;
-            const int64_t k = kb * q4::kCols + 16 * r + 4 * (lane & 3);
-            uint32_t w = 0;
+    const int64_t n = experts * tiles * units * record, stride = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += stride) {
+        const int64_t rec = i / record, unit = rec % units, tile = rec / units % tiles, e = rec / units / tiles;
+        int w = (int)(i % record);
+        uint32_t v = 0;
+        if (w < code_words) {
+            const int r = w & 3, lane = (w >> 2) & 31, kb = (w >> 7) & 1, blk = w >> 8;
+            const int64_t k = unit * q4::kUnitCols + kb * q4::kCols + 16 * r + 4 * (lane & 3);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int64_t row = source(rb, (lane >> 2) + 8 * h);
+                const int64_t row = source(tile * q4::kTileBlocks + blk, (lane >> 2) + 8 * h);
                 if (row < 0) continue;
                 const uint8_t* p = codes + (e * rows + row) * n_bytes;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (k + c >= cols) continue;
                     const uint32_t q = (p[(k + c) >> 1] >> (4 * (c & 1))) & 15u;
-                    w |= q << (4 * (2 * h + (c >> 1)) + 16 * (c & 1));
+                    v |= q << (4 * (2 * h + (c >> 1)) + 16 * (c & 1));
                 }
             }
-            words[i] = w;
         } else {
-            const int64_t s = i - n_words;
-            const int in = (int)((s >> 1) & 7) + 8 * (int)(s & 1);
-            const int64_t blk = s >> 4, g = blk % groups, rb = blk / groups % rbs, e = blk / groups / rbs;
-            const int64_t row = source(rb, in);
-            const int64_t at = (e * rows + row) * groups + g;
-            out_scales[s] = row < 0 ? (uint16_t)0 : scales[at];
-            if (zeros) out_zeros[s] = row < 0 ? (uint8_t)8 : (uint8_t)(zeros[at] & 15);
+            w -= code_words;
+            const bool is_zero = w < zero_words;
+            if (!is_zero) w -= zero_words;
+            const int per = is_zero ? 4 : 2;             // values a word; 16 values a row block
+            for (int c = 0; c < per; ++c) {
+                const int at = w * per + c, in = ((at >> 1) & 7) + 8 * (at & 1), blk = (at >> 4) & 7;
+                const int64_t g = unit * subs + (at >> 7), row = source(tile * q4::kTileBlocks + blk, in);
+                if (row < 0 || g >= groups) continue;
+                const int64_t from = (e * rows + row) * groups + g;
+                v |= (is_zero ? (uint32_t)(zeros[from] & 15) : (uint32_t)scales[from]) << (c * (32 / per));
+            }
         }
+        out[i] = v;
     }
 }
 
@@ -141,11 +145,11 @@ struct Int4Params {
     const void* x;
     int64_t ldx;
     int vec;                          // x's rows start on 8 bytes and cols is a multiple of 4: 8-byte loads
-    const uint4* words;
-    const uint32_t* scales;
-    const uint16_t* zeros;            // null: 8 everywhere
-    int tokens, cols, kbs, groups, group_shift;
-    int64_t rows, rbs;                // output rows (a gated module's: both halves) and row blocks, of one expert
+    const uint8_t* layout;
+    int record, scales_at;            // bytes of a unit's record, and where its scales start
+    int zeros;                        // it holds zero points (else 8 everywhere)
+    int tokens, cols, kbs, units, group_shift;
+    int64_t rows, rbs, tiles;         // rows (a gated module's: both halves), row blocks and row tiles of one expert
     int gated;
     void* y;
     int64_t ldy;
@@ -214,7 +218,9 @@ __global__ void __launch_bounds__(WARPS * 32) int4_kernel(const __grid_constant_
     } else {
         count = (int)min((int64_t)(NT * 8), p.tokens - first);
     }
-    const int64_t rb0 = (int64_t)blockIdx.x * RB, base = expert * p.rbs + rb0;
+    const int64_t rb0 = (int64_t)blockIdx.x * RB;                    // RB divides a tile's 8 blocks
+    const uint8_t* base = p.layout + (expert * p.tiles + rb0 / 8) * p.units * p.record;
+    const int blk = (int)(rb0 & 7);
     const int n_rb = (int)min((int64_t)RB, p.rbs - rb0);
     struct Stage {
         uint4 w[U][RB];
@@ -231,15 +237,18 @@ __global__ void __launch_bounds__(WARPS * 32) int4_kernel(const __grid_constant_
                 st.s[u][b][0] = st.s[u][b][1] = 0u;
                 st.z[u][b][0] = st.z[u][b][1] = 0x0808;
                 if (kb < p.kbs && b < n_rb) {
-                    st.w[u][b] = __ldg(p.words + ((base + b) * p.kbs + kb) * 32 + lane);
-                    const int g0 = (kb * 64) >> p.group_shift;
-                    const int64_t at = (base + b) * p.groups;
-                    st.s[u][b][0] = __ldg(p.scales + (at + g0) * 8 + n);
-                    if (p.zeros) st.z[u][b][0] = __ldg(p.zeros + (at + g0) * 8 + n);
+                    const uint8_t* rec = base + (int64_t)(kb >> 1) * p.record;
+                    st.w[u][b] = __ldg(reinterpret_cast<const uint4*>(rec + ((blk + b) * 2 + (kb & 1)) * q4::kBlockBytes) + lane);
+                    // the block's first group in its unit, and with groups of 32 the next
+                    const int g = p.group_shift == 7 ? 0 : p.group_shift == 6 ? kb & 1 : 2 * (kb & 1);
+                    const int at = (g * 8 + blk + b) * 8 + n;
+                    const uint32_t* sc = reinterpret_cast<const uint32_t*>(rec + p.scales_at) + at;
+                    const uint16_t* ze = reinterpret_cast<const uint16_t*>(rec + q4::kCodeBytes) + at;
+                    st.s[u][b][0] = __ldg(sc);
+                    if (p.zeros) st.z[u][b][0] = __ldg(ze);
                     if (p.group_shift == 5) {
-                        const int g1 = min(g0 + 1, p.groups - 1);
-                        st.s[u][b][1] = __ldg(p.scales + (at + g1) * 8 + n);
-                        if (p.zeros) st.z[u][b][1] = __ldg(p.zeros + (at + g1) * 8 + n);
+                        st.s[u][b][1] = __ldg(sc + 64);
+                        if (p.zeros) st.z[u][b][1] = __ldg(ze + 64);
                     }
                 }
             }
@@ -429,48 +438,51 @@ extern "C" int p2p_int4_expand(const uint8_t* codes, const void* scales, const u
     return launch_status("p2p_int4_expand");
 }
 
-extern "C" int64_t p2p_int4_row_blocks(int64_t rows, int gated) {
-    return rows < 0 || (gated && rows % 2) ? -1 : q4::row_blocks(rows, gated);
+extern "C" int64_t p2p_int4_layout_bytes(int64_t experts, int64_t rows, int64_t cols, int group, int has_zeros,
+                                         int gated) {
+    if (experts < 1 || rows < 1 || cols < 1 || (gated && rows % 2) || group_shift(group) < 0) return -1;
+    return q4::layout_bytes(experts, rows, cols, group, has_zeros != 0, gated);
 }
 
 extern "C" int p2p_int4_layout(const uint8_t* codes, const void* scales, const uint8_t* zeros, int64_t experts,
-                               int64_t rows, int64_t cols, int group, int gated, void* words, void* out_scales,
-                               uint8_t* out_zeros, void* stream) {
+                               int64_t rows, int64_t cols, int group, int gated, void* layout, void* stream) {
     P2P_REQUIRE(experts >= 1 && rows >= 1 && cols >= 1 && cols <= 0x7fffffff && !(gated && rows % 2),
                 "p2p_int4_layout: bad shape");
     P2P_REQUIRE(group_shift(group) > 0, "p2p_int4_layout: groups of %d columns, not 32, 64 or 128", group);
-    P2P_REQUIRE(codes && scales && words && out_scales && (!zeros || out_zeros), "p2p_int4_layout: null pointer");
-    P2P_REQUIRE(aligned16(words), "p2p_int4_layout: the layout must start on a 16-byte boundary");
-    layout_kernel<<<sm_count() * 16, 256, 0, as_stream(stream)>>>(
-        codes, reinterpret_cast<const uint16_t*>(scales), zeros, experts, rows, (int)cols, group, gated,
-        reinterpret_cast<uint32_t*>(words), reinterpret_cast<uint16_t*>(out_scales), out_zeros);
+    P2P_REQUIRE(codes && scales && layout, "p2p_int4_layout: null pointer");
+    P2P_REQUIRE(aligned16(layout), "p2p_int4_layout: the layout must start on a 16-byte boundary");
+    layout_kernel<<<sm_count() * 16, 256, 0, as_stream(stream)>>>(codes, reinterpret_cast<const uint16_t*>(scales), zeros,
+                                                                  experts, rows, (int)cols, group, gated,
+                                                                  reinterpret_cast<uint32_t*>(layout));
     return launch_status("p2p_int4_layout");
 }
 
 namespace {
 // What both products check and fill in.
-int int4_params(Int4Params& p, const char* what, const void* x, int dtype, int64_t cols, int64_t ldx, const void* words,
-                const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated, void* y, int64_t ldy) {
+int int4_params(Int4Params& p, const char* what, const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout,
+                int has_zeros, int64_t rows, int group, int gated, void* y, int64_t ldy) {
     if (dtype != P2P_BF16 && dtype != P2P_F16) return fail(P2P_EUNSUPPORTED, "%s: bf16 or f16", what);
     P2P_REQUIRE(rows <= 0x7fffffff && cols >= 1 && cols <= 0x7fffff00, "%s: bad shape", what);
     P2P_REQUIRE(group_shift(group) > 0, "%s: groups of %d columns, not 32, 64 or 128", what, group);
     P2P_REQUIRE(!(gated && rows % 2), "%s: a gated module has as many gate rows as up rows", what);
-    P2P_REQUIRE(x && words && scales && y, "%s: null pointer", what);
-    P2P_REQUIRE(aligned16(words), "%s: the layout must start on a 16-byte boundary", what);
+    P2P_REQUIRE(x && layout && y, "%s: null pointer", what);
+    P2P_REQUIRE(aligned16(layout), "%s: the layout must start on a 16-byte boundary", what);
     P2P_REQUIRE(ldx >= cols && ldy >= (gated ? rows / 2 : rows), "%s: a row stride below the row", what);
     p.x = x;
     p.ldx = ldx;
     p.vec = cols % 4 == 0 && ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 7u) == 0;
-    p.words = reinterpret_cast<const uint4*>(words);
-    p.scales = reinterpret_cast<const uint32_t*>(scales);
-    p.zeros = reinterpret_cast<const uint16_t*>(zeros);
+    p.layout = reinterpret_cast<const uint8_t*>(layout);
+    p.record = q4::unit_bytes(group, has_zeros != 0);
+    p.scales_at = q4::kCodeBytes + q4::unit_zero_bytes(group, has_zeros != 0);
+    p.zeros = has_zeros != 0;
     p.tokens = 0;
     p.cols = (int)cols;
     p.kbs = (int)q4::div_up(cols, q4::kCols);
-    p.groups = (int)q4::div_up(cols, group);
+    p.units = (int)q4::div_up(cols, q4::kUnitCols);
     p.group_shift = group_shift(group);
     p.rows = rows;
     p.rbs = q4::row_blocks(rows, gated);
+    p.tiles = q4::row_tiles(rows, gated);
     p.gated = gated;
     p.y = y;
     p.ldy = ldy;
@@ -497,13 +509,13 @@ extern "C" size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols,
     return int4_tc_workspace(tokens, rows, cols, gated);
 }
 
-extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* words,
-                           const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated, void* y,
-                           int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout,
+                           int has_zeros, int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace,
+                           size_t workspace_bytes, void* stream) {
     P2P_REQUIRE(tokens >= 0 && rows >= 0 && tokens <= 0x7fffffff, "p2p_int4_mm: bad shape");
     if (tokens == 0 || rows == 0) return P2P_OK;
     Int4Params p;
-    if (int e = int4_params(p, "p2p_int4_mm", x, dtype, cols, ldx, words, scales, zeros, rows, group, gated, y, ldy))
+    if (int e = int4_params(p, "p2p_int4_mm", x, dtype, cols, ldx, layout, has_zeros, rows, group, gated, y, ldy))
         return e;
     cudaStream_t st = as_stream(stream);
     if (use_tc(tokens, rows, cols)) {
@@ -513,7 +525,7 @@ extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t col
                     "p2p_int4_mm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         Int4Call c = {};
         c.x = x; c.dtype = dtype; c.tokens = tokens; c.cols = cols; c.ldx = ldx;
-        c.words = words; c.scales = scales; c.zeros = zeros;
+        c.layout = layout; c.has_zeros = has_zeros != 0;
         c.rows = rows; c.group = group; c.gated = gated; c.y = y; c.ldy = ldy;
         return int4_tc_run(c, workspace, st, "p2p_int4_mm");
     }
@@ -522,8 +534,8 @@ extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t col
                              : run_int4<__half>(p, tokens, 0, st, "p2p_int4_mm");
 }
 
-extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* words,
-                                const void* scales, const uint8_t* zeros, int64_t rows, int group, int gated,
+extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout,
+                                int has_zeros, int64_t rows, int group, int gated,
                                 const int32_t* items, const int32_t* n_items, int64_t max_items, int64_t item_tokens,
                                 const int32_t* order, int topk, const int32_t* routed, int64_t pairs, void* y,
                                 int64_t ldy, void* stream) {
@@ -536,8 +548,7 @@ extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t 
     P2P_REQUIRE(items && n_items && topk >= 1, "p2p_int4_grouped: null pointer or topk %d", topk);
     P2P_REQUIRE(aligned16(items), "p2p_int4_grouped: items must start on a 16-byte boundary");
     Int4Params p;
-    if (int e = int4_params(p, "p2p_int4_grouped", x, dtype, cols, ldx, words, scales, zeros, rows, group, gated, y,
-                            ldy))
+    if (int e = int4_params(p, "p2p_int4_grouped", x, dtype, cols, ldx, layout, has_zeros, rows, group, gated, y, ldy))
         return e;
     cudaStream_t st = as_stream(stream);
     if (tc) {
@@ -545,7 +556,7 @@ extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t 
         P2P_REQUIRE(tc_aligned(x, ldx), "p2p_int4_grouped: items of more than 8 tokens need x rows of 16-byte alignment");
         Int4Call c = {};
         c.x = x; c.dtype = dtype; c.cols = cols; c.ldx = ldx;
-        c.words = words; c.scales = scales; c.zeros = zeros;
+        c.layout = layout; c.has_zeros = has_zeros != 0;
         c.rows = rows; c.group = group; c.gated = gated; c.y = y; c.ldy = ldy;
         c.items = items; c.n_items = n_items; c.max_items = max_items; c.item_tokens = item_tokens; c.pairs = pairs;
         c.routed = routed;

@@ -1,16 +1,19 @@
 // The 4-bit weight layout (p2p_int4_layout), shared by the kernels that read it.
 //
-// A module's rows are cut into blocks of 16, its columns into blocks of 64. A (row block, column block) is 512 bytes:
-// lane t = 4 n + j of a warp owns the 16 bytes at 16 t, word r of them (r = 0..3) holding the codes of rows n and n + 8
-// at columns 16 r + 4 j .. + 3, as four pairs of neighbouring columns whose low column is nibble i and high column
-// nibble i + 4:
+// A module is cut into units of 128 rows by 128 columns, each a record of consecutive bytes, the units of a row tile one
+// after the other: a run of units is one linear stream.
+//   record   codes [8 row blocks of 16][2 column blocks of 64][512 bytes]
+//            zero points [groups of the unit][8 row blocks][8][2], a byte each: rows n and n + 8 (only if there are any)
+//            scales [groups of the unit][8 row blocks][8][2], 16 bits each, the same order
+//   layout   [experts][row tiles][units of 128 columns][record]
+// Of a (row block, column block)'s 512 bytes lane t = 4 n + j of a warp owns the 16 at 16 t, word r of them (r = 0..3)
+// holding the codes of rows n and n + 8 at columns 16 r + 4 j .. + 3, as four pairs of neighbouring columns whose low
+// column is nibble i and high column nibble i + 4:
 //   i = 0: row n, columns 0 and 1    i = 1: row n, columns 2 and 3    i = 2, 3: the same of row n + 8
 // so that one mask leaves a pair in the low bits of both halves of the word, ready to become two 16-bit floats. That is
 // a lane's A fragment of four m16n8k16 products whose k runs 4 j .. 4 j + 3 instead of {2 j, 2 j + 1, 2 j + 8, 2 j + 9}
 // (the sum over k does not mind, B's fragment takes the same columns: one 8-byte load of x), and also a lane's part of
 // a tcgen05.st.16x256b.x4 of 16 rows by 64 columns into tensor memory.
-//   blocks   [experts][row blocks][column blocks][512]
-//   scales   [experts][row blocks][groups][8][2]: rows n and n + 8, 16-bit; zeros the same in bytes (absent: 8)
 // Of a gated module the even row blocks are gate rows, the odd ones the same units' up rows.
 #pragma once
 #include "common.cuh"
@@ -21,11 +24,24 @@ namespace q4 {
 constexpr int kRows = 16;
 constexpr int kCols = 64;
 constexpr int kBlockBytes = 512;
+constexpr int kUnitCols = 128;
+constexpr int kTileBlocks = 8;                         // row blocks of a unit
+constexpr int kCodeBytes = kTileBlocks * 2 * kBlockBytes;
 
 __host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Row blocks of one expert; a gated module's halves are padded to whole blocks each.
 __host__ __device__ inline int64_t row_blocks(int64_t rows, int gated) {
     return gated ? 2 * div_up(rows / 2, kRows) : div_up(rows, kRows);
+}
+
+__host__ __device__ inline int64_t row_tiles(int64_t rows, int gated) { return div_up(row_blocks(rows, gated), kTileBlocks); }
+__host__ __device__ inline int unit_zero_bytes(int group, bool zeros) { return zeros ? kUnitCols / group * 128 : 0; }
+__host__ __device__ inline int unit_scale_bytes(int group) { return kUnitCols / group * 256; }
+__host__ __device__ inline int unit_bytes(int group, bool zeros) {
+    return kCodeBytes + unit_zero_bytes(group, zeros) + unit_scale_bytes(group);
+}
+inline int64_t layout_bytes(int64_t experts, int64_t rows, int64_t cols, int group, bool zeros, int gated) {
+    return experts * row_tiles(rows, gated) * div_up(cols, kUnitCols) * unit_bytes(group, zeros);
 }
 
 template <typename T> struct Codes;

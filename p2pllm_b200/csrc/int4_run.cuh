@@ -10,8 +10,8 @@ struct Int4Call {
     const void* x;
     int dtype;
     int64_t tokens, cols, ldx;          // dense
-    const void *words, *scales;
-    const uint8_t* zeros;
+    const void* layout;
+    bool has_zeros;
     int64_t rows;
     int group, gated;
     void* y;

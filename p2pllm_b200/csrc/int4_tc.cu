@@ -6,8 +6,9 @@
 // scaled weight rounded to bf16 would double the squared error of the result). A CTA, one an SM, takes a contiguous run
 // of units (128 rows x 128 columns), row tile after row tile:
 //
-//   warp 16 (weights)   streams the run's codes, 8 KB a unit, into a ring in shared memory by bulk copies, ahead of the
-//                       previous kernel's end and up to 8 units ahead of their use
+//   warp 16 (weights)   streams the run's records, 8.4 KB a unit and one linear range of the layout a row tile, into
+//                       rings in shared memory by bulk copies (codes and zero points in one, scales, which are used
+//                       later, in another), ahead of the previous kernel's end and up to 12 units ahead of their use
 //   warp 17 (x)         TMA of each unit's x tile [tokens x 128] (two 64-column boxes, 128-byte swizzle)
 //   warps 8-15 (build)  warp w turns the codes of one 16-row block into bf16 / f16 integers and stores them into the
 //                       unit's A tile in tensor memory (two tcgen05.st.16x256b.x4: the layout is that store's order)
@@ -37,10 +38,12 @@ constexpr int kWeightWarp = kBuildWarp + kBuildWarps;   // 16
 constexpr int kXWarp = kWeightWarp + 1;                 // 17
 constexpr int kMmaWarp = kWeightWarp + 2;               // 18, 19
 constexpr int kThreads = 640;
-constexpr int kUnitBytes = 8 * 2 * q4::kBlockBytes;     // 128 rows x 128 columns of codes
+constexpr int kWSlotBytes = q4::kCodeBytes + 512;       // codes and up to four groups' zero points
+constexpr int kSSlotBytes = 1024;                       // up to four groups' scales
 constexpr int kACols = 64;                              // TMEM columns of one unit's A tile
 constexpr int kTmemCols = 512;
-constexpr int kMaxW = 8, kMaxX = 8, kMaxA = 6, kMaxBuf = 2;
+constexpr int kMaxW = 12, kMaxX = 8, kMaxA = 6, kMaxBuf = 2;
+constexpr int kSSlots = 16;                             // scales wait for the rings before them: more than W + A slots hold
 constexpr int kSmemLimit = 227 * 1024 - 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
@@ -48,10 +51,9 @@ __device__ int g_int4_error;            // site of the first wait that gave up s
 __device__ unsigned g_int4_failed_seq;  // sequence number of the last launch in which a wait gave up
 
 struct TcParams {
-    const uint8_t* words;
-    const uint16_t* scales;
-    const uint8_t* zeros;               // null: 8
-    int rows, out_rows, rbs, row_tiles, kbs, units, groups, group_shift, gated;   // units: 128-column steps a row tile
+    const uint8_t* layout;
+    int record, zero_bytes, scale_bytes;                // of a unit
+    int out_rows, row_tiles, units, group_shift, gated; // units: 128-column steps a row tile
     int tokens, tile_tokens, token_tiles;                                         // dense
     const int32_t* items;                                                         // routed
     const int32_t* n_items;
@@ -88,13 +90,31 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t s, uint32_t lo, uin
 }
 __device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(v >> (32 * i))); }
 
+// mbar_wait, with many tests of the phase between two looks at the clock and the failure flag: each look takes about a
+// microsecond, which a hand-over between two roles cannot wait for.
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
+#pragma unroll 1
+    for (int i = 0; i < 4096; ++i)
+        if (mbar_try(bar, parity)) return true;
+    return mbar_wait(bar, parity, site, wc);
+}
+
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, site, wc));
+    return __all_sync(0xffffffffu, wait_one(bar, parity, site, wc));
+}
+
+// One thread of the warp, the same one every time. A branch on elect.sync, unlike one on the lane number, tells the
+// compiler that a single thread runs it: tensor-core and copy instructions then take their operands straight from
+// uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 // A row tile of the run: its row blocks, its tokens, the steps of it that this CTA takes.
 struct Tile {
-    int64_t rb0;                        // first row block, of all experts
+    const uint8_t* records;             // its units' records
     int rt;                             // row tile within the module
     int first, n;                       // first x row (and y row), tokens
     int k0, k1;                         // steps [k0, k1) of p.units
@@ -109,14 +129,14 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t u, int64_t u1
         const int item = (int)(id / p.row_tiles);
         t.rt = (int)(id - (int64_t)item * p.row_tiles);
         const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + item);
-        t.rb0 = (int64_t)it.x * p.rbs + t.rt * 8;
+        t.records = p.layout + ((int64_t)it.x * p.row_tiles + t.rt) * p.units * p.record;
         t.first = it.y;
         t.n = min(it.z, p.n_max);
     } else {
         t.rt = (int)(id / p.token_tiles);
         t.first = (int)(id - (int64_t)t.rt * p.token_tiles) * p.tile_tokens;
         t.n = min(p.tile_tokens, p.tokens - t.first);
-        t.rb0 = t.rt * 8;
+        t.records = p.layout + (int64_t)t.rt * p.units * p.record;
     }
     return t;
 }
@@ -140,7 +160,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int SW = p.w_slots, SX = p.x_slots, SA = p.a_slots, NB = p.bufs;
     const uint32_t sub_bytes = (uint32_t)p.x_rows * 128u, x_bytes = 2u * sub_bytes;
-    const uint32_t x_ring = base, w_ring = x_ring + SX * x_bytes, bars = w_ring + SW * kUnitBytes;
+    const uint32_t x_ring = base, w_ring = x_ring + SX * x_bytes, s_ring = w_ring + SW * kWSlotBytes;
+    const uint32_t bars = s_ring + kSSlots * kSSlotBytes;
     auto wfull = [&](int s) { return bars + 8u * s; };
     auto wempty = [&](int s) { return bars + 8u * (kMaxW + s); };
     auto xfull = [&](int s) { return bars + 8u * (2 * kMaxW + s); };
@@ -149,9 +170,11 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     auto aempty = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + kMaxA + s); };
     auto dfull = [&](int h, int b) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * b + h); };
     auto dempty = [&](int h, int b) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * kMaxBuf + 2 * b + h); };
-    const uint32_t done = bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf);
+    auto sfull = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + s); };
+    auto sempty = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + kSSlots + s); };
+    const uint32_t done = bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + 2 * kSSlots);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const WaitCtl wc{&g_int4_error, &g_int4_failed_seq, p.wait_ns, p.seq};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
@@ -160,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kBuildWarps); mbar_init(aempty(s), 2); }
         for (int b = 0; b < NB; ++b)
             for (int h = 0; h < 2; ++h) { mbar_init(dfull(h, b), 1); mbar_init(dempty(h, b), 4); }
+        for (int s = 0; s < kSSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), kPromoteWarps); }
         mbar_init(done, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -173,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     // The items are the previous kernel's; dense weights wait for nobody, and everything else for that kernel's end.
     if (p.items || (warp != kWeightWarp && (warp < kBuildWarp || warp >= kWeightWarp)))
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -189,54 +213,61 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     if (warp >= kWeightWarp) {
         if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
         if (warp == kWeightWarp) {
-            int slot = 0, used = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int64_t u = u0; u < u1 && ok;) {
-                const Tile t = tile_at(p, u, u1);
-                const int blocks = min(8, p.rbs - t.rt * 8);
-                const uint8_t* src = p.words + (t.rb0 + lane) * p.kbs * q4::kBlockBytes;
-                for (int k = t.k0; k < t.k1; ++k) {
-                    if (used >= SW && !(ok = wait_all(wempty(slot), ph ^ 1u, 1, wc))) break;
-                    const uint32_t bytes = 2 * k + 1 < p.kbs ? 2u * q4::kBlockBytes : (uint32_t)q4::kBlockBytes;
-                    if (lane == 0) mbar_expect_tx(wfull(slot), bytes * blocks);
-                    __syncwarp();
-                    if (lane < blocks)
-                        bulk_load(w_ring + slot * kUnitBytes + lane * 2 * q4::kBlockBytes,
-                                  src + (int64_t)k * 2 * q4::kBlockBytes, bytes, wfull(slot));
-                    ++used;
-                    advance(slot, ph, 1, SW);
+            if (elect_one()) {
+                int slot = 0, ss = 0, used = 0;
+                uint32_t ph = 0, phs = 0;
+                bool ok = true;
+                const uint32_t w_bytes = (uint32_t)(q4::kCodeBytes + p.zero_bytes);
+                for (int64_t u = u0; u < u1 && ok;) {
+                    const Tile t = tile_at(p, u, u1);
+                    const uint8_t* src = t.records + (int64_t)t.k0 * p.record;
+                    for (int k = t.k0; k < t.k1; ++k, src += p.record) {
+                        if (used >= SW && !(ok = wait_one(wempty(slot), ph ^ 1u, 1, wc))) break;
+                        if (used >= kSSlots && !(ok = wait_one(sempty(ss), phs ^ 1u, 12, wc))) break;
+                        mbar_expect_tx(wfull(slot), w_bytes);
+                        bulk_load(w_ring + slot * kWSlotBytes, src, w_bytes, wfull(slot));
+                        mbar_expect_tx(sfull(ss), (uint32_t)p.scale_bytes);
+                        bulk_load(s_ring + ss * kSSlotBytes, src + w_bytes, (uint32_t)p.scale_bytes, sfull(ss));
+                        ++used;
+                        advance(slot, ph, 1, SW);
+                        advance(ss, phs, 1, kSSlots);
+                    }
+                    u += t.k1 - t.k0;
                 }
-                u += t.k1 - t.k0;
+                // every copy issued must have landed before the CTA may exit: each slot's last one
+                for (int i = max(0, used - SW); i < used; ++i) mbar_drain(wfull(i % SW), (uint32_t)((i / SW) & 1), 2, wc);
+                for (int i = max(0, used - kSSlots); i < used; ++i)
+                    mbar_drain(sfull(i % kSSlots), (uint32_t)((i / kSSlots) & 1), 2, wc);
             }
-            // every copy issued must have landed before the CTA may exit: each slot's last one
-            for (int i = max(0, used - SW); i < used; ++i) mbar_drain(wfull(i % SW), (uint32_t)((i / SW) & 1), 2, wc);
+            __syncwarp();
         } else if (warp == kXWarp) {
             if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_x)) : "memory");
-            int slot = 0, used = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int64_t u = u0; u < u1 && ok;) {
-                const Tile t = tile_at(p, u, u1);
-                const int boxes = (n_total(t.n) + p.box_rows - 1) / p.box_rows;
-                for (int k = t.k0; k < t.k1; ++k) {
-                    if (used >= SX && !(ok = wait_all(xempty(slot), ph ^ 1u, 3, wc))) break;
-                    if (lane == 0) mbar_expect_tx(xfull(slot), (uint32_t)(2 * boxes * p.box_rows) * 128u);
-                    __syncwarp();
-                    for (int i = lane; i < 2 * boxes; i += 32) {
-                        const int s = i & 1, b = i >> 1;
-                        tma_load_2d(x_ring + slot * x_bytes + s * sub_bytes + b * p.box_rows * 128, &tmap_x,
-                                    k * 128 + s * 64, t.first + b * p.box_rows, xfull(slot));
+            if (elect_one()) {
+                int slot = 0, used = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                for (int64_t u = u0; u < u1 && ok;) {
+                    const Tile t = tile_at(p, u, u1);
+                    const int boxes = (n_total(t.n) + p.box_rows - 1) / p.box_rows;
+                    for (int k = t.k0; k < t.k1; ++k) {
+                        if (used >= SX && !(ok = wait_one(xempty(slot), ph ^ 1u, 3, wc))) break;
+                        mbar_expect_tx(xfull(slot), (uint32_t)(2 * boxes * p.box_rows) * 128u);
+                        for (int b = 0; b < boxes; ++b)
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+                                tma_load_2d(x_ring + slot * x_bytes + s * sub_bytes + b * p.box_rows * 128, &tmap_x,
+                                            k * 128 + s * 64, t.first + b * p.box_rows, xfull(slot));
+                        ++used;
+                        advance(slot, ph, 1, SX);
                     }
-                    ++used;
-                    advance(slot, ph, 1, SX);
+                    u += t.k1 - t.k0;
                 }
-                u += t.k1 - t.k0;
+                for (int i = max(0, used - SX); i < used; ++i) mbar_drain(xfull(i % SX), (uint32_t)((i / SX) & 1), 4, wc);
             }
-            for (int i = max(0, used - SX); i < used; ++i) mbar_drain(xfull(i % SX), (uint32_t)((i / SX) & 1), 4, wc);
+            __syncwarp();
         } else {
             const int h = warp - kMmaWarp;
-            if (lane == 0) {
+            if (elect_one()) {
                 int sa = 0, sx = 0, sb = 0, jobs = 0;
                 uint32_t pha = 0, phx = 0, phb = 0;
                 bool ok = true;
@@ -246,14 +277,14 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                     const int n0 = n_first(t.n), n = h ? n_total(t.n) - n0 : n0;
                     const uint32_t id = idesc_f16<T>(n ? n : 16);
                     for (int k = t.k0; k < t.k1 && ok; ++k) {
-                        if (!(ok = mbar_wait(afull(sa), pha, 5, wc))) break;
-                        if (!(ok = mbar_wait(xfull(sx), phx, 6, wc))) break;
+                        if (!(ok = wait_one(afull(sa), pha, 5, wc))) break;
+                        if (!(ok = wait_one(xfull(sx), phx, 6, wc))) break;
                         tc_fence_after();
                         const uint32_t a = tmem + (uint32_t)(p.a_col0 + sa * kACols);
                         const uint64_t b0 = sw128_desc(x_ring + sx * x_bytes) + (uint64_t)((h * n0 * 128) >> 4);
                         const uint64_t b1 = b0 + (uint64_t)(sub_bytes >> 4);
                         for (int s = 0; s < subs; ++s) {
-                            if (jobs >= NB && !(ok = mbar_wait(dempty(h, sb), phb ^ 1u, 7, wc))) break;
+                            if (jobs >= NB && !(ok = wait_one(dempty(h, sb), phb ^ 1u, 7, wc))) break;
                             tc_fence_after();
                             if (n) {
                                 const uint32_t d = tmem + d_col(h, sb);
@@ -287,24 +318,16 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         bool ok = true;
         for (int64_t u = u0; u < u1 && ok;) {
             const Tile t = tile_at(p, u, u1);
-            const int64_t rb = t.rb0 + min(blk, p.rbs - t.rt * 8 - 1);          // past the module: any codes do
-            const uint16_t* zrow = reinterpret_cast<const uint16_t*>(p.zeros) + rb * p.groups * 8 + (lane >> 2);
-            uint32_t z[4] = {0x0808u, 0x0808u, 0x0808u, 0x0808u};
-            auto load_zeros = [&](int k) {
-                if (!p.zeros) return;
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    if (s < subs) z[s] = __ldg(zrow + min(k * subs + s, p.groups - 1) * 8);
-            };
-            load_zeros(t.k0);
             for (int k = t.k0; k < t.k1; ++k) {
                 if (!(ok = wait_all(wfull(sw), phw, 9, wc))) break;
-                const uint32_t at = w_ring + sw * kUnitBytes + blk * 2 * q4::kBlockBytes + lane * 16;
+                const uint32_t rec = w_ring + sw * kWSlotBytes, at = rec + blk * 2 * q4::kBlockBytes + lane * 16;
                 const uint4 c[2] = {lds_v4(at), lds_v4(at + q4::kBlockBytes)};
-                uint32_t zs[4];
+                uint32_t zs[4] = {0x0808u, 0x0808u, 0x0808u, 0x0808u};
+                if (p.zero_bytes) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) zs[s] = z[s];
-                if (k + 1 < t.k1) load_zeros(k + 1);
+                    for (int s = 0; s < 4; ++s)
+                        if (s < subs) zs[s] = lds_u16(rec + q4::kCodeBytes + ((s * 8 + blk) * 8 + (lane >> 2)) * 2);
+                }
                 if (used >= SA && !(ok = wait_all(aempty(sa), pha ^ 1u, 10, wc))) break;
                 tc_fence_after();
                 q4::Codes<T> codes;
@@ -340,24 +363,29 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         if (kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         const int h = warp >> 2, q = warp & 3, row_in = 32 * q + lane;
         T* y = reinterpret_cast<T*>(p.y);
-        int sb = 0;
-        uint32_t phb = 0;
+        const uint32_t scale_at = (uint32_t)(((row_in >> 4) * 8 + (row_in & 7)) * 2 + ((row_in >> 3) & 1)) * 2u;
+        int sb = 0, ss = 0;
+        uint32_t phb = 0, phs = 0;
         bool ok = true;
         for (int64_t u = u0; u < u1 && ok;) {
             const Tile t = tile_at(p, u, u1);
             const int n0 = n_first(t.n), nh = h ? n_total(t.n) - n0 : n0;
-            const int64_t rb = t.rb0 + min(row_in >> 4, p.rbs - t.rt * 8 - 1);
-            const uint16_t* srow = p.scales + rb * p.groups * 16 + 2 * (row_in & 7) + ((row_in >> 3) & 1);
             uint64_t acc[NH / 2];
 #pragma unroll
             for (int i = 0; i < NH / 2; ++i) acc[i] = 0;
-            const int g0 = t.k0 * subs, g1 = t.k1 * subs;
-            uint16_t sbits = __ldg(srow + (int64_t)min(g0, p.groups - 1) * 16);
-            for (int g = g0; g < g1; ++g) {
-                const float s = to_f32(*reinterpret_cast<const T*>(&sbits));
+            for (int k = t.k0; k < t.k1 && ok; ++k) {
+                if (!(ok = wait_all(sfull(ss), phs, 13, wc))) break;
+#pragma unroll 1
+                for (int sub = 0; sub < subs; ++sub) {
+                const uint16_t sb16 = (uint16_t)lds_u16(s_ring + ss * kSSlotBytes + sub * 256 + scale_at);
+                if (sub == subs - 1) {                   // the unit's scales are read
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sempty(ss));
+                    advance(ss, phs, 1, kSSlots);
+                }
+                const float s = to_f32(*reinterpret_cast<const T*>(&sb16));
                 uint64_t s2;
                 asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(s)));
-                if (g + 1 < g1) sbits = __ldg(srow + (int64_t)min(g + 1, p.groups - 1) * 16);
                 if (!(ok = wait_all(dfull(h, sb), phb, 11, wc))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + d_col(h, sb);
@@ -376,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(dempty(h, sb));
                 advance(sb, phb, 1, NB);
+                }
             }
             if (!ok) break;
             const int left = min(nh, t.n - h * n0);      // this half's tokens
@@ -491,12 +520,14 @@ TcPlan plan_tc(int most, bool routed) {
     pl.a_col0 = (pl.bufs * total + 31) / 32 * 32;
     pl.a_slots = (kTmemCols - pl.a_col0) / kACols;
     if (pl.a_slots > kMaxA) pl.a_slots = kMaxA;
-    const int x_bytes = 2 * pl.x_rows * 128, bar_bytes = 8 * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + 1);
-    pl.w_slots = kMaxW;
-    int room = kSmemLimit - 1024 - bar_bytes - pl.w_slots * kUnitBytes;
-    pl.x_slots = room / x_bytes;
+    const int x_bytes = 2 * pl.x_rows * 128;
+    const int fixed = 1024 + kSSlots * kSSlotBytes + 8 * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + 2 * kSSlots + 1);
+    // eight units of weights in flight at least, then x, then as much again as is left for weights
+    pl.x_slots = (kSmemLimit - fixed - 8 * kWSlotBytes) / x_bytes;
     if (pl.x_slots > kMaxX) pl.x_slots = kMaxX;
-    pl.smem = 1024 + pl.x_slots * x_bytes + pl.w_slots * kUnitBytes + bar_bytes;
+    pl.w_slots = (kSmemLimit - fixed - pl.x_slots * x_bytes) / kWSlotBytes;
+    if (pl.w_slots > kMaxW) pl.w_slots = kMaxW;
+    pl.smem = fixed + pl.x_slots * x_bytes + pl.w_slots * kWSlotBytes;
     return pl;
 }
 
@@ -561,7 +592,7 @@ int dense_ctas(int64_t tiles, int64_t units, bool* split) {
 }  // namespace
 
 size_t int4_tc_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated) {
-    const int64_t row_tiles = q4::div_up(q4::row_blocks(rows, gated), 8), units = q4::div_up(cols, 128);
+    const int64_t row_tiles = q4::row_tiles(rows, gated), units = q4::div_up(cols, q4::kUnitCols);
     bool split;
     const int ctas = dense_ctas(row_tiles * token_tiles(tokens), units, &split);
     if (!split) return 0;
@@ -573,16 +604,13 @@ int int4_tc_run(const Int4Call& c, void* workspace, cudaStream_t st, const char*
     const bool routed = c.items != nullptr;
     const int most = routed ? (int)c.item_tokens : tile_tokens(c.tokens);
     const TcPlan pl = plan_tc(most, routed);
-    p.words = reinterpret_cast<const uint8_t*>(c.words);
-    p.scales = reinterpret_cast<const uint16_t*>(c.scales);
-    p.zeros = c.zeros;
-    p.rows = (int)c.rows;
+    p.layout = reinterpret_cast<const uint8_t*>(c.layout);
+    p.record = q4::unit_bytes(c.group, c.has_zeros);
+    p.zero_bytes = q4::unit_zero_bytes(c.group, c.has_zeros);
+    p.scale_bytes = q4::unit_scale_bytes(c.group);
     p.out_rows = (int)(c.gated ? c.rows / 2 : c.rows);
-    p.rbs = (int)q4::row_blocks(c.rows, c.gated);
-    p.row_tiles = (int)q4::div_up(p.rbs, 8);
-    p.kbs = (int)q4::div_up(c.cols, q4::kCols);
-    p.units = (int)q4::div_up(c.cols, 128);
-    p.groups = (int)q4::div_up(c.cols, c.group);
+    p.row_tiles = (int)q4::row_tiles(c.rows, c.gated);
+    p.units = (int)q4::div_up(c.cols, q4::kUnitCols);
     p.group_shift = c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
     p.gated = c.gated;
     p.tokens = (int)c.tokens;

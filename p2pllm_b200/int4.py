@@ -106,19 +106,17 @@ class Layout:
         self.experts = codes.shape[0] if codes.dim() == 3 else 1
         self.rows, self.cols, self.group, self.gated = codes.shape[-2], cols, group, gated
         self.dtype, self.device = scales.dtype, scales.device
-        blocks_of = _lib.load().p2p_int4_row_blocks(self.rows, int(gated))
-        if blocks_of < 0:
-            raise P2PError(f"a gated module has as many gate rows as up rows, not {self.rows} in all")
         if self.rows == 0 or self.experts == 0:
             raise P2PError("a 4-bit module needs at least one row")
-        row_blocks, groups = self.experts * blocks_of, -(-cols // group)
-        self.words = torch.empty(row_blocks * -(-cols // 64) * 128, dtype=torch.int32, device=self.device)
-        self.scales = torch.empty(row_blocks * groups * 16, dtype=self.dtype, device=self.device)
-        self.zeros = None if zeros is None else torch.empty(row_blocks * groups * 16, dtype=torch.uint8, device=self.device)
+        self.has_zeros = zeros is not None
+        nbytes = _lib.load().p2p_int4_layout_bytes(self.experts, self.rows, cols, group, self.has_zeros, gated)
+        if nbytes < 0:
+            raise P2PError(f"a gated module has as many gate rows as up rows, not {self.rows} in all")
+        self.data = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         codes, scales, zeros = codes.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
         with torch.cuda.device(self.device):
             call("p2p_int4_layout", ptr(codes), ptr(scales), ptr(zeros), self.experts, self.rows, cols, group,
-                 int(gated), ptr(self.words), ptr(self.scales), ptr(self.zeros), stream_of(codes))
+                 int(gated), ptr(self.data), stream_of(codes))
             torch.cuda.current_stream(self.device).synchronize()   # the products read weights ahead of their stream
 
     def check_x(self, x: torch.Tensor) -> None:
@@ -136,11 +134,11 @@ class Layout:
         """x [T, cols] W^T: [T, rows], gated [T, rows / 2] (p2p_int4_mm through the torch operator)."""
         self.check_x(x)
         if out is None:
-            return _lib.ops().int4_mm(x, self.words, self.scales, self.zeros, self.rows, self.cols, self.group, self.gated)
+            return _lib.ops().int4_mm(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated)
         from .kernels import _out
         out = _out(out, (x.shape[0], self.rows // 2 if self.gated else self.rows), x)
-        _lib.ops().int4_mm_into(x, self.words, self.scales, self.zeros, self.rows, self.cols, self.group, self.gated, out)
+        _lib.ops().int4_mm_into(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated, out)
         return out
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.words, self.scales, self.zeros) if t is not None)
+        return self.data.numel()

@@ -199,7 +199,7 @@ class Int4Experts:
         _check_rows(x, order, order.tokens if gather else pairs)
         if order.experts != self.experts:
             raise P2PError(f"an order of {order.experts} experts, weights of {self.experts}")
-        args = (x, q.words, q.scales, q.zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order, order.where,
+        args = (x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order, order.where,
                 order.offsets, order.items, order.n_items, order.topk, gather)
         if out is None:
             return _lib.ops().int4_grouped(*args)

@@ -54,22 +54,16 @@ at::Tensor moe_spread(const at::Tensor& x_in, const at::Tensor& where, const at:
 
 // ---- 4-bit products --------------------------------------------------------------------------------------------------
 
-void check_int4(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
-                const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols, int64_t group,
+void check_int4(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols, int64_t group,
                 bool gated) {
     check_matrix(x, "x");
     TORCH_CHECK(x.size(1) == cols, "p2p_b200: x of ", x.sizes(), " does not have ", cols, " columns");
     TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()),
                 "p2p_b200: 4-bit weights are for inference: x must not need a gradient");
     TORCH_CHECK(group == 32 || group == 64 || group == 128, "p2p_b200: groups of ", group, " columns, not 32, 64 or 128");
-    const int64_t rbs = experts * p2p_int4_row_blocks(rows, gated);
-    TORCH_CHECK(words.device() == x.device() && words.is_contiguous() && words.nbytes() >= (size_t)(rbs * ((cols + 63) / 64) * 512),
-                "p2p_b200: 4-bit words do not hold ", rows, " x ", cols);
-    const int64_t n = rbs * ((cols + group - 1) / group) * 16;
-    TORCH_CHECK(scales.device() == x.device() && scales.is_contiguous() && scales.scalar_type() == x.scalar_type() &&
-                    scales.numel() >= n, "p2p_b200: scales are not ", n, " of ", x.scalar_type(), " on ", x.device());
-    TORCH_CHECK(!zeros || (zeros->device() == x.device() && zeros->is_contiguous() && zeros->scalar_type() == at::kByte &&
-                           zeros->numel() >= n), "p2p_b200: zero points are not ", n, " bytes on ", x.device());
+    const int64_t need = p2p_int4_layout_bytes(experts, rows, cols, (int)group, zeros, gated);
+    TORCH_CHECK(need > 0 && layout.device() == x.device() && layout.scalar_type() == at::kByte && layout.is_contiguous() &&
+                    layout.numel() >= need, "p2p_b200: the 4-bit layout does not hold ", rows, " x ", cols, " weights");
 }
 
 void check_rows_out(const at::Tensor& out, const at::Tensor& x, int64_t rows, int64_t cols) {
@@ -80,12 +74,9 @@ void check_rows_out(const at::Tensor& out, const at::Tensor& x, int64_t rows, in
                 x.scalar_type());
 }
 
-const uint8_t* bytes(const std::optional<at::Tensor>& t) { return t ? t->data_ptr<uint8_t>() : nullptr; }
-
-void int4_mm_into(const at::Tensor& x_in, const at::Tensor& words, const at::Tensor& scales,
-                  const std::optional<at::Tensor>& zeros, int64_t rows, int64_t cols, int64_t group, bool gated,
+void int4_mm_into(const at::Tensor& x_in, const at::Tensor& layout, bool zeros, int64_t rows, int64_t cols, int64_t group, bool gated,
                   const at::Tensor& out) {
-    check_int4(x_in, words, scales, zeros, 1, rows, cols, group, gated);
+    check_int4(x_in, layout, zeros, 1, rows, cols, group, gated);
     check_rows_out(out, x_in, x_in.size(0), gated ? rows / 2 : rows);
     const c10::cuda::CUDAGuard guard(x_in.device());
     const bool small = x_in.size(0) <= kSmallTokens;
@@ -93,25 +84,23 @@ void int4_mm_into(const at::Tensor& x_in, const at::Tensor& words, const at::Ten
     const size_t need = p2p_int4_workspace(x.size(0), rows, cols, gated);
     const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte)) : at::Tensor();
     check(p2p_int4_mm(x.data_ptr(), dtype_code(x), x.size(0), cols, small ? row_stride(x) : aligned_stride(x),
-                      words.data_ptr(), scales.data_ptr(), bytes(zeros), rows, (int)group, gated, out.data_ptr(),
+                      layout.data_ptr(), zeros, rows, (int)group, gated, out.data_ptr(),
                       row_stride(out), need ? ws.data_ptr() : nullptr, need, stream_of(x)),
           "p2p_int4_mm");
 }
 
-at::Tensor int4_mm(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
-                   const std::optional<at::Tensor>& zeros, int64_t rows, int64_t cols, int64_t group, bool gated) {
+at::Tensor int4_mm(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t rows, int64_t cols, int64_t group, bool gated) {
     check_matrix(x, "x");
     at::Tensor out = at::empty({x.size(0), gated ? rows / 2 : rows}, x.options());
-    int4_mm_into(x, words, scales, zeros, rows, cols, group, gated, out);
+    int4_mm_into(x, layout, zeros, rows, cols, group, gated, out);
     return out;
 }
 
-void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& words, const at::Tensor& scales,
-                      const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
+void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols,
                       int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
                       const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
                       const at::Tensor& out, bool zero_behind) {
-    check_int4(x_in, words, scales, zeros, experts, rows, cols, group, gated);
+    check_int4(x_in, layout, zeros, experts, rows, cols, group, gated);
     const int64_t pairs = order.numel();
     TORCH_CHECK(topk >= 1 && x_in.size(0) == (gather ? pairs / topk : pairs) && pairs % topk == 0, "p2p_b200: x has ",
                 x_in.size(0), " rows, the order is of ", pairs, " pairs, ", topk, " a token");
@@ -125,30 +114,27 @@ void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& words, const at:
     const int64_t most = item_tokens(pairs, experts);
     const bool small = most <= kSmallTokens, in_place = small || !gather;
     const at::Tensor x = small ? rows2d(x_in) : aligned_rows(gather ? moe_spread(x_in, where, offsets, topk) : x_in);
-    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, small ? row_stride(x) : aligned_stride(x), words.data_ptr(), scales.data_ptr(),
-                           bytes(zeros), rows, (int)group, gated, ints(items, x, 0, "items"),
+    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, small ? row_stride(x) : aligned_stride(x), layout.data_ptr(), zeros, rows, (int)group, gated, ints(items, x, 0, "items"),
                            ints(n_items, x, 1, "n_items"), items.numel() / 4, most,
                            gather && in_place ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
                            out.data_ptr(), row_stride(out), stream_of(x)),
           "p2p_int4_grouped");
 }
 
-void int4_grouped_into(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
-                       const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
+void int4_grouped_into(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols,
                        int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
                        const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
                        const at::Tensor& out) {
-    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk,
+    int4_grouped_run(x, layout, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk,
                      gather, out, false);
 }
 
-at::Tensor int4_grouped(const at::Tensor& x, const at::Tensor& words, const at::Tensor& scales,
-                        const std::optional<at::Tensor>& zeros, int64_t experts, int64_t rows, int64_t cols,
+at::Tensor int4_grouped(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols,
                         int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
                         const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather) {
     check_matrix(x, "x");
     at::Tensor out = at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
-    int4_grouped_run(x, words, scales, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk,
+    int4_grouped_run(x, layout, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk,
                      gather, out, true);
     return out;
 }
@@ -322,19 +308,15 @@ std::tuple<at::Tensor, at::Tensor> moe_sum_back_grad(const at::Tensor& dout, con
 
 // ---- shapes ----------------------------------------------------------------------------------------------------------
 
-at::Tensor int4_mm_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
-                        int64_t rows, int64_t, int64_t, bool gated) {
+at::Tensor int4_mm_meta(const at::Tensor& x, const at::Tensor&, bool, int64_t rows, int64_t, int64_t, bool gated) {
     return at::empty({x.size(0), gated ? rows / 2 : rows}, x.options());
 }
-void int4_mm_into_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
-                       int64_t, int64_t, int64_t, bool, const at::Tensor&) {}
-at::Tensor int4_grouped_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
-                             int64_t, int64_t rows, int64_t, int64_t, bool gated, const at::Tensor& order,
+void int4_mm_into_meta(const at::Tensor&, const at::Tensor&, bool, int64_t, int64_t, int64_t, bool, const at::Tensor&) {}
+at::Tensor int4_grouped_meta(const at::Tensor& x, const at::Tensor&, bool, int64_t, int64_t rows, int64_t, int64_t, bool gated, const at::Tensor& order,
                              const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool) {
     return at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
 }
-void int4_grouped_into_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
-                            int64_t, int64_t, int64_t, int64_t, bool, const at::Tensor&, const at::Tensor&,
+void int4_grouped_into_meta(const at::Tensor&, const at::Tensor&, bool, int64_t, int64_t, int64_t, int64_t, bool, const at::Tensor&, const at::Tensor&,
                             const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool, const at::Tensor&) {}
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort_meta(const at::Tensor& ids, int64_t experts) {
     const auto o = ids.options().dtype(at::kInt);
@@ -357,12 +339,12 @@ std::tuple<at::Tensor, at::Tensor> moe_sum_back_meta(const at::Tensor&, const at
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(p2p_b200, m) {
-    m.def("int4_mm(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int rows, int cols, int group, bool gated) -> Tensor");
-    m.def("int4_mm_into(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int rows, int cols, int group, bool gated, "
+    m.def("int4_mm(Tensor x, Tensor layout, bool zeros, int rows, int cols, int group, bool gated) -> Tensor");
+    m.def("int4_mm_into(Tensor x, Tensor layout, bool zeros, int rows, int cols, int group, bool gated, "
           "Tensor(a!) out) -> ()");
-    m.def("int4_grouped(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int experts, int rows, int cols, int group, "
+    m.def("int4_grouped(Tensor x, Tensor layout, bool zeros, int experts, int rows, int cols, int group, "
           "bool gated, Tensor order, Tensor where, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather) -> Tensor");
-    m.def("int4_grouped_into(Tensor x, Tensor words, Tensor scales, Tensor? zeros, int experts, int rows, int cols, "
+    m.def("int4_grouped_into(Tensor x, Tensor layout, bool zeros, int experts, int rows, int cols, "
           "int group, bool gated, Tensor order, Tensor where, Tensor offsets, Tensor items, Tensor n_items, int topk, bool gather, "
           "Tensor(a!) out) -> ()");
     m.def("moe_sort(Tensor ids, int experts) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
