@@ -357,8 +357,7 @@ size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated)
 
 /* y [tokens, rows] = x [tokens, cols] W^T of a module in the layout; gated: y [tokens, rows / 2] =
  * dtype(silu(gate) * up), from the fp32 sums. Each group's sum of exact code differences is multiplied by its scale in
- * fp32; no weight is rounded. Any tokens, rows and cols; above 8 tokens x's rows start on 16-byte boundaries (ldx a
- * multiple of 8). As the other GEMMs, a programmatic dependent of the stream's previous kernel that reads its weights
+ * fp32; no weight is rounded. Any tokens, rows and cols; x's rows start on 16-byte boundaries (ldx a multiple of 8). As the other GEMMs, a programmatic dependent of the stream's previous kernel that reads its weights
  * before that kernel completes. */
 int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout, int has_zeros,
                 int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
@@ -366,8 +365,8 @@ int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t 
 
 /* The same for routed experts: y [pairs, rows] (gated: rows / 2), row p being x's row times the weights of the expert
  * whose item holds place p. items, n_items: p2p_moe_sort's, of at most item_tokens <= 272 places each. x's row of
- * place p is p itself, or with items of at most 8 places, where order is not null, order[p] / topk; above 8 places x's
- * rows start on 16-byte boundaries. routed: null, or the number of routed pairs on the device: rows from there to
+ * place p is p itself, or with items of at most 8 places, where order is not null, order[p] / topk (x then has pairs / topk
+ * rows). routed: null, or the number of routed pairs on the device: rows from there to
  * `pairs` become zero (null: they stay as they were). */
 int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout, int has_zeros, int64_t rows, int group, int gated, const int32_t* items,
                      const int32_t* n_items, int64_t max_items, int64_t item_tokens, const int32_t* order, int topk,

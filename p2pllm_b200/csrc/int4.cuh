@@ -16,7 +16,7 @@
 // a tcgen05.st.16x256b.x4 of 16 rows by 64 columns into tensor memory.
 // Of a gated module the even row blocks are gate rows, the odd ones the same units' up rows.
 #pragma once
-#include "common.cuh"
+#include "sm100.cuh"
 
 namespace p2p {
 namespace q4 {
@@ -92,4 +92,25 @@ template <> struct Codes<__half> {
 };
 
 }  // namespace q4
+namespace sm100 {
+
+// mbar_wait, with many tests of the phase between two looks at the clock and the failure flag: each look takes about a
+// microsecond, which a hand-over between two roles cannot wait for.
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
+#pragma unroll 1
+    for (int i = 0; i < 4096; ++i)
+        if (mbar_try(bar, parity)) return true;
+    return mbar_wait(bar, parity, site, wc);
+}
+
+// One thread of the warp, the same one every time. A branch on elect.sync, unlike one on the lane number, tells the
+// compiler that a single thread runs it: tensor-core and copy instructions then take their operands straight from
+// uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+}  // namespace sm100
 }  // namespace p2p

@@ -26,4 +26,7 @@ size_t int4_tc_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated);
 // x: 16-byte aligned rows (ldx and the start).
 int int4_tc_run(const Int4Call& call, void* workspace, cudaStream_t st, const char* what);
 
+// The site of that kernel's first wait that gave up (0: none); reset != 0 clears it. Syncs the stream.
+int int4_tc_error(int* site, int reset, cudaStream_t st);
+
 }  // namespace p2p

@@ -90,26 +90,8 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t s, uint32_t lo, uin
 }
 __device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(v >> (32 * i))); }
 
-// mbar_wait, with many tests of the phase between two looks at the clock and the failure flag: each look takes about a
-// microsecond, which a hand-over between two roles cannot wait for.
-__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
-#pragma unroll 1
-    for (int i = 0; i < 4096; ++i)
-        if (mbar_try(bar, parity)) return true;
-    return mbar_wait(bar, parity, site, wc);
-}
-
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
     return __all_sync(0xffffffffu, wait_one(bar, parity, site, wc));
-}
-
-// One thread of the warp, the same one every time. A branch on elect.sync, unlike one on the lane number, tells the
-// compiler that a single thread runs it: tensor-core and copy instructions then take their operands straight from
-// uniform registers.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-    return r != 0;
 }
 
 // A row tile of the run: its row blocks, its tokens, the steps of it that this CTA takes.
@@ -128,7 +110,7 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t u, int64_t u1
     if (p.items) {
         const int item = (int)(id / p.row_tiles);
         t.rt = (int)(id - (int64_t)item * p.row_tiles);
-        const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + item);
+        const int4 it = __ldcg(reinterpret_cast<const int4*>(p.items) + item);
         t.records = p.layout + ((int64_t)it.x * p.row_tiles + t.rt) * p.units * p.record;
         t.first = it.y;
         t.n = min(it.z, p.n_max);
@@ -646,21 +628,16 @@ int int4_tc_run(const Int4Call& c, void* workspace, cudaStream_t st, const char*
                                : launch_nh<__half>(pl.nh, map, p, pl.smem, st, what);
 }
 
-}  // namespace p2p
-
-using namespace p2p;
-
-extern "C" int p2p_int4_status(int reset, void* stream) {
-    cudaStream_t st = as_stream(stream);
-    int v = 0;
-    if (cudaMemcpyFromSymbolAsync(&v, g_int4_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+int int4_tc_error(int* site, int reset, cudaStream_t st) {
+    if (cudaMemcpyFromSymbolAsync(site, g_int4_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
         cudaStreamSynchronize(st) != cudaSuccess)
         return fail(P2P_ECUDA, "p2p_int4_status: %s", cudaGetErrorString(cudaGetLastError()));
-    if (reset && v) {
+    if (reset && *site) {
         const int zero = 0;
         cudaMemcpyToSymbolAsync(g_int4_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
         cudaStreamSynchronize(st);
     }
-    if (v) return fail(P2P_ECUDA, "p2p_int4: a pipeline wait timed out (site %d)", v);
     return P2P_OK;
 }
+
+}  // namespace p2p

@@ -186,7 +186,7 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) spre
             const Vec<T, N> val = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
 #pragma unroll 4
             for (int j = 0; j < p.k; ++j) {
-                const int at = __ldg(p.where + t * p.k + j);
+                const int at = __ldcg(p.where + t * p.k + j);
                 if (at >= 0) store_vec<T, N>(p.out, at * p.ldo + (int64_t)v * N, val);
             }
         }
@@ -208,7 +208,7 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_
             int at[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                at[b] = j0 + b < p.k ? __ldg(p.where + t * p.k + j0 + b) : -1;
+                at[b] = j0 + b < p.k ? __ldcg(p.where + t * p.k + j0 + b) : -1;
                 if (at[b] >= 0) rows[b] = load_vec<T, N>(p.y, at[b] * p.ldy + (int64_t)v * N);
             }
 #pragma unroll
@@ -241,7 +241,7 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_
         for (int b = 0; b < kBatch; ++b) {
             const bool in = live && j0 + b < p.k;
             dot[b] = 0.f;
-            at[b] = in ? __ldg(p.where + t * p.k + j0 + b) : -1;
+            at[b] = in ? __ldcg(p.where + t * p.k + j0 + b) : -1;
             w[b] = at[b] >= 0 ? load_weight(p.w, p.w_dtype, t * p.k + j0 + b) : 0.f;
         }
         for (int v = threadIdx.x; live && v < p.vecs; v += blockDim.x) {

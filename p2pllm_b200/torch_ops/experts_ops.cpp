@@ -12,7 +12,7 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr int64_t kSmallTokens = 8;                   // up to here the products take x rows of any alignment and order
+constexpr int64_t kSmallTokens = 8;                   // items of up to here pick x's rows by the order
 
 // Places of one item, what one pass over an expert's weights takes: few where experts have few pairs on average, so
 // that a tile is not mostly empty; otherwise as many as keep the weights' codes from being turned twice.
@@ -79,11 +79,10 @@ void int4_mm_into(const at::Tensor& x_in, const at::Tensor& layout, bool zeros, 
     check_int4(x_in, layout, zeros, 1, rows, cols, group, gated);
     check_rows_out(out, x_in, x_in.size(0), gated ? rows / 2 : rows);
     const c10::cuda::CUDAGuard guard(x_in.device());
-    const bool small = x_in.size(0) <= kSmallTokens;
-    const at::Tensor x = small ? rows2d(x_in) : aligned_rows(x_in);
+    const at::Tensor x = aligned_rows(x_in);
     const size_t need = p2p_int4_workspace(x.size(0), rows, cols, gated);
     const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte)) : at::Tensor();
-    check(p2p_int4_mm(x.data_ptr(), dtype_code(x), x.size(0), cols, small ? row_stride(x) : aligned_stride(x),
+    check(p2p_int4_mm(x.data_ptr(), dtype_code(x), x.size(0), cols, aligned_stride(x),
                       layout.data_ptr(), zeros, rows, (int)group, gated, out.data_ptr(),
                       row_stride(out), need ? ws.data_ptr() : nullptr, need, stream_of(x)),
           "p2p_int4_mm");
@@ -112,11 +111,12 @@ void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& layout, bool zer
                 experts);
     if (pairs == 0) return;
     const int64_t most = item_tokens(pairs, experts);
-    const bool small = most <= kSmallTokens, in_place = small || !gather;
-    const at::Tensor x = small ? rows2d(x_in) : aligned_rows(gather ? moe_spread(x_in, where, offsets, topk) : x_in);
-    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, small ? row_stride(x) : aligned_stride(x), layout.data_ptr(), zeros, rows, (int)group, gated, ints(items, x, 0, "items"),
+    // few pairs: the product picks x's rows itself
+    const bool pick = gather && most <= kSmallTokens;
+    const at::Tensor x = aligned_rows(gather && !pick ? moe_spread(x_in, where, offsets, topk) : x_in);
+    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, aligned_stride(x), layout.data_ptr(), zeros, rows, (int)group, gated, ints(items, x, 0, "items"),
                            ints(n_items, x, 1, "n_items"), items.numel() / 4, most,
-                           gather && in_place ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
+                           pick ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
                            out.data_ptr(), row_stride(out), stream_of(x)),
           "p2p_int4_grouped");
 }

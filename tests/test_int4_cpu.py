@@ -52,7 +52,7 @@ def test_layout_bytes(lib):
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 68, FAKE, 0, 16, 64, 0, FAKE, FAKE, 4, 9, None, 1, None, 4,
                                   FAKE, 16, None), -1, b"16-byte"),
     (lambda l: l.p2p_int4_mm(FAKE, 0, 9, 64, 68, FAKE, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"16-byte"),
-    (lambda l: l.p2p_int4_mm(FAKE, 0, 9, 64, 64, FAKE, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"workspace"),
+    (lambda l: l.p2p_int4_mm(FAKE, 0, 33, 64, 64, FAKE, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"workspace"),
     (lambda l: l.p2p_moe_sort(FAKE, 4, 64, 1025, FAKE, FAKE, FAKE, FAKE, 2000, 32, FAKE, None), -2, b"at most 1024"),
     (lambda l: l.p2p_moe_sort(FAKE, 2, 64, 8, FAKE, FAKE, FAKE, FAKE, 64, 32, FAKE, None), -1, b"4 or 8"),
     (lambda l: l.p2p_moe_sort(FAKE, 4, 64, 8, FAKE, FAKE, FAKE, FAKE, 9, 32, FAKE, None), -1, b"10 needed"),
