@@ -370,7 +370,11 @@ int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t 
  * `pairs` become zero (null: they stay as they were). */
 int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout, int has_zeros, int64_t rows, int group, int gated, const int32_t* items,
                      const int32_t* n_items, int64_t max_items, int64_t item_tokens, const int32_t* order, int topk,
-                     const int32_t* routed, int64_t pairs, void* y, int64_t ldy, void* stream);
+                     const int32_t* routed, int64_t pairs, void* y, int64_t ldy, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace p2p_int4_grouped needs, as p2p_int4_workspace. */
+size_t p2p_int4_grouped_workspace(int64_t max_items, int64_t item_tokens, int64_t rows, int64_t cols, int gated);
 
 /* P2P_OK unless a pipeline wait of a 4-bit product gave up since the last reset (P2P_ECUDA, naming its site; that
  * launch's y is undefined); reset != 0 clears it. Syncs the stream. */

@@ -86,7 +86,8 @@ SIGNATURES = {
     "p2p_int4_mm": ([_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _i64, _vp, _sz, _vp], _int),
     "p2p_int4_status": ([_int, _vp], _int),
     "p2p_int4_grouped": ([_vp, _int, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _vp, _i64, _i64, _vp, _int, _vp, _i64,
-                          _vp, _i64, _vp], _int),
+                          _vp, _i64, _vp, _sz, _vp], _int),
+    "p2p_int4_grouped_workspace": ([_i64, _i64, _i64, _i64, _int], _sz),
     "p2p_moe_sort": ([_vp, _int, _i64, _int, _vp, _vp, _vp, _vp, _i64, _int, _vp, _vp], _int),
     "p2p_moe_spread": ([_vp, _int, _i64, _int, _i64, _i64, _vp, _vp, _vp, _i64, _vp], _int),
     "p2p_moe_sum": ([_vp, _int, _i64, _int, _i64, _i64, _vp, _vp, _int, _vp, _i64, _vp], _int),

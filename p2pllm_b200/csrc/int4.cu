@@ -10,6 +10,7 @@
 //   p2p_int4_grouped    the same for the rows of one expert after the other, rows gathered by token or in place, with
 //                       silu(gate) * up applied on the way out of a gated module
 #include <atomic>
+#include <stdlib.h>
 
 #include "int4.cuh"
 #include "int4_run.cuh"
@@ -158,9 +159,10 @@ __device__ unsigned g_small_failed_seq;  // sequence number of the last launch i
 struct SmallParams {
     const uint8_t* layout;
     int record, zeros, scales_at;       // bytes of a unit's record; whether it holds zero points; where its scales start
-    int units, row_tiles, group_shift, gated;
-    int tokens, out_rows;
-    int splits;                         // CTAs of a cluster, each with its share of the units
+    int units, row_tiles, col_tiles, group_shift, gated;
+    int tokens, n_max, out_rows;        // n_max: tokens of a tile, at most
+    int splits;                         // > 0: CTAs of a cluster, each with its share of one row tile; 0: runs
+    float* partial;                     // runs: [ctas][2][n_max][128], the row tiles a run shares with its neighbours
     int slots, slot_bytes, x_at, x_sub; // ring: record, then two x boxes of x_sub bytes at x_at
     void* y;
     int64_t ldy;
@@ -174,27 +176,35 @@ struct SmallParams {
     unsigned seq;
 };
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b, __nv_bfloat16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+// c += a b, or with Zero c = a b.
+template <bool Zero, typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    const float z = 0.f;
+    if constexpr (bf && Zero)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%10, %10, %10, %10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(z));
+    else if constexpr (bf)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+    else if constexpr (Zero)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%10, %10, %10, %10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(z));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b, __half) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
-}
-__device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
+// A value at byte `at` of shared memory: plain loads, which the compiler may move about between two barriers.
+template <typename V> __device__ __forceinline__ V lds(const uint8_t* smem, uint32_t at) {
+    return *reinterpret_cast<const V*>(smem + at);
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
@@ -202,21 +212,56 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 
-// A CTA takes a row tile (128 rows), up to 8 NT tokens and a share of the columns; the CTAs of a cluster hold the row
-// tile's shares and add them up over distributed shared memory, in column order. One warp streams the share's records
-// and x tiles into a ring of shared memory; warp w multiplies row block w: the codes become exact small integers, eight
-// m16n8k16 products a unit and 8 tokens add a group's columns in fp32, and the group's scale multiplies that sum on its
-// way into the fp32 accumulators: no weight is ever rounded.
-template <typename T, int NT>
-__global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 4 : 3) int4_small_kernel(const __grid_constant__ CUtensorMap tmap_x,
-                                                                                   const __grid_constant__ SmallParams p) {
+// Row tile `id` of a launch: whose rows, which tokens.
+struct SmallTile {
+    const uint8_t* records;
+    int rt, first, n;
+};
+__device__ __forceinline__ SmallTile small_tile(const SmallParams& p, int64_t id) {
+    SmallTile t;
+    const int col = (int)(id / p.row_tiles);             // an item, or a tile of the tokens
+    t.rt = (int)(id - (int64_t)col * p.row_tiles);
+    int64_t expert = 0;
+    if (p.items) {
+        const int4 it = __ldcg(reinterpret_cast<const int4*>(p.items) + col);
+        expert = it.x;
+        t.first = it.y;
+        t.n = min(it.z, p.n_max);
+    } else {
+        t.first = col * p.n_max;
+        t.n = min(p.n_max, p.tokens - t.first);
+    }
+    t.records = p.layout + (expert * p.row_tiles + t.rt) * p.units * p.record;
+    return t;
+}
+__device__ __forceinline__ int64_t small_tiles(const SmallParams& p) {
+    return (int64_t)(p.items ? *p.n_items : p.col_tiles) * p.row_tiles;
+}
+// Runs of a launch: no more than it has units (routed launches learn that here), so that none is empty; and where run b
+// begins.
+__device__ __forceinline__ int small_runs(int64_t units_all, int ctas) { return (int)min((int64_t)ctas, units_all); }
+__device__ __forceinline__ int64_t small_begin(int64_t units_all, int64_t b, int runs) { return units_all * b / runs; }
+
+// y of a finished pair of sums (gated) or sum.
+template <typename T> __device__ __forceinline__ T gate_up(float g, float u) { return from_f32<T>(g / (1.f + expf(-g)) * u); }
+
+// A CTA takes 128 x 128 units of a row tile and up to 8 NT tokens: its share of one row tile, the CTAs of a cluster adding
+// theirs up over distributed shared memory in column order, or (runs) a contiguous run of units across row tiles, the
+// sums of those it shares with its neighbours going to int4_small_join_kernel. One warp streams records and x tiles into
+// a ring of shared memory; warp w multiplies row blocks 2 (w % 4) and + 1 of column block w / 4 (two row blocks share a
+// fragment of x, whose reads would else bind): the codes become exact small integers, m16n8k16 products add a group's
+// columns in fp32, and the group's scale multiplies that sum on its way into the fp32 accumulators: no weight is ever
+// rounded. G32: groups of 32 columns, two a column block (else one holds the block or more).
+template <typename T, int NT, bool G32>
+__global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __grid_constant__ CUtensorMap tmap_x,
+                                                                      const __grid_constant__ SmallParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    const uint32_t bars = base + (uint32_t)(p.slots * p.slot_bytes);
+    float* red = reinterpret_cast<float*>(smem_raw + (base - raw) + p.slots * p.slot_bytes);   // [8 NT][kRowPad]
+    const uint32_t bars = smem_u32(red) + NT * 8 * kRowPad * 4;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (kMaxSlots + s); };
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
     const WaitCtl wc{&g_small_error, &g_small_failed_seq, p.wait_ns, p.seq};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
@@ -228,68 +273,73 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 4 : 3) int4_small_ker
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    int64_t expert = 0, first = (int64_t)blockIdx.y * (NT * 8);
-    int count = 0;
-    if (p.items) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");           // the items are the previous kernel's
-        const int n_items = *p.n_items;
-        if ((int)blockIdx.y >= n_items) {                            // no item left: zero what lies behind the last pair
-            const int64_t col = (int64_t)tile * (p.gated ? 64 : 128) + threadIdx.x;
-            if (p.routed && rank == 0 && threadIdx.x < (p.gated ? 64 : 128) && col < p.out_rows)
-                for (int64_t r = *p.routed + (blockIdx.y - n_items); r < p.pairs; r += gridDim.y - n_items)
-                    reinterpret_cast<T*>(p.y)[r * p.ldy + col] = from_f32<T>(0.f);
-            return;
-        }
-        const int4 it = reinterpret_cast<const int4*>(p.items)[blockIdx.y];
-        expert = it.x;
-        first = it.y;
-        count = min(it.z, NT * 8);
+    // The items are the previous kernel's. Dense weights wait for nobody; x (its input) and y (whose old values it may
+    // still read) for that kernel's end.
+    if (p.items || warp < kComputeWarps) asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t tiles = small_tiles(p), units_all = tiles * p.units;
+    const bool clustered = p.splits > 0;
+    int64_t u0, u1;
+    int rank = 0;
+    if (clustered) {
+        const int64_t tile = blockIdx.x / p.splits;
+        rank = blockIdx.x - (int)tile * p.splits;
+        u0 = tile < tiles ? tile * p.units + (int64_t)p.units * rank / p.splits : 0;
+        u1 = tile < tiles ? tile * p.units + (int64_t)p.units * (rank + 1) / p.splits : 0;
     } else {
-        count = (int)min((int64_t)(NT * 8), p.tokens - first);
+        const int runs = small_runs(units_all, gridDim.x);
+        u0 = blockIdx.x < runs ? small_begin(units_all, blockIdx.x, runs) : 0;
+        u1 = blockIdx.x < runs ? small_begin(units_all, blockIdx.x + 1, runs) : 0;
     }
-    const int k0 = (int)((int64_t)p.units * rank / p.splits), k1 = (int)((int64_t)p.units * (rank + 1) / p.splits);
-    float acc[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
 
     if (warp == kComputeWarps) {
         if (elect_one()) {
-            const uint8_t* src = p.layout + ((expert * p.row_tiles + tile) * p.units + k0) * p.record;
             const int n_slots = p.slots;
-            const uint32_t x_rows = p.order ? (uint32_t)count : (uint32_t)(NT * 8);
-            bool ok = true, first_x = true;
-            auto load_x = [&](int slot, int k) {
+            const uint32_t w_bytes = (uint32_t)p.record;
+            bool ok = true;
+            auto load_w = [&](int slot, const SmallTile& t, int k) {
+                const uint32_t x_rows = p.order ? (uint32_t)t.n : (uint32_t)(NT * 8);
+                mbar_expect_tx(full(slot), w_bytes + 2u * 128u * x_rows);
+                bulk_load(base + slot * p.slot_bytes, t.records + (int64_t)k * p.record, w_bytes, full(slot));
+            };
+            auto load_x = [&](int slot, const SmallTile& t, int k) {
                 const uint32_t at = base + slot * p.slot_bytes + p.x_at;
                 if (p.order) {                                       // a row at a time, from wherever its token lies
-                    for (int i = 0; i < count; ++i) {
-                        const int row = __ldcg(p.order + first + i) / p.topk;
+                    for (int i = 0; i < t.n; ++i) {
+                        const int row = __ldcg(p.order + t.first + i) / p.topk;
                         tma_load_2d(at + i * 128, &tmap_x, k * 128, row, full(slot));
                         tma_load_2d(at + p.x_sub + i * 128, &tmap_x, k * 128 + 64, row, full(slot));
                     }
                 } else {
-                    tma_load_2d(at, &tmap_x, k * 128, (int)first, full(slot));
-                    tma_load_2d(at + p.x_sub, &tmap_x, k * 128 + 64, (int)first, full(slot));
+                    tma_load_2d(at, &tmap_x, k * 128, t.first, full(slot));
+                    tma_load_2d(at + p.x_sub, &tmap_x, k * 128 + 64, t.first, full(slot));
                 }
             };
-            // the ring's first fill: all weights, then, once x is there, all x tiles
-            const int head = min(n_slots, k1 - k0);
-            for (int i = 0; i < head; ++i) {
-                mbar_expect_tx(full(i), (uint32_t)p.record + 2u * 128u * x_rows);
-                bulk_load(base + i * p.slot_bytes, src + (int64_t)i * p.record, (uint32_t)p.record, full(i));
-            }
-            if (!p.items) asm volatile("griddepcontrol.wait;" ::: "memory");   // x may be the previous kernel's output
-            for (int i = 0; i < head; ++i) load_x(i, k0 + i);
-            int slot = 0, used = head;
+            int slot = 0, used = 0;
             uint32_t ph = 0;
-            for (int k = k0 + head; k < k1; ++k) {
-                if (!(ok = wait_one(empty(slot), ph, 1, wc))) break;
-                mbar_expect_tx(full(slot), (uint32_t)p.record + 2u * 128u * x_rows);
-                bulk_load(base + slot * p.slot_bytes, src + (int64_t)(k - k0) * p.record, (uint32_t)p.record, full(slot));
-                load_x(slot, k);
-                ++used;
-                advance(slot, ph, 1, n_slots);
+            if (!p.items) {
+                // the ring's first fill: weights, then, once the previous kernel has ended, x
+                for (int pass = 0; pass < 2; ++pass) {
+                    int i = 0;
+                    for (int64_t u = u0; u < u1 && i < n_slots;) {
+                        const SmallTile t = small_tile(p, u / p.units);
+                        for (int k = (int)(u % p.units); k < p.units && u < u1 && i < n_slots; ++k, ++u, ++i)
+                            if (pass == 0) load_w(i, t, k); else load_x(i, t, k);
+                    }
+                    used = i;
+                    if (pass == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+                }
+                slot = used == n_slots ? 0 : used;
+                ph = used == n_slots ? 1u : 0u;
+            }
+            for (int64_t u = u0 + used; u < u1 && ok;) {
+                const SmallTile t = small_tile(p, u / p.units);
+                for (int k = (int)(u % p.units); k < p.units && u < u1; ++k, ++u) {
+                    if (used >= n_slots && !(ok = wait_one(empty(slot), ph ^ 1u, 1, wc))) break;
+                    load_w(slot, t, k);
+                    load_x(slot, t, k);
+                    ++used;
+                    advance(slot, ph, 1, n_slots);
+                }
             }
             // every copy issued must have landed before the CTA may exit: each slot's last one
             for (int i = max(0, used - n_slots); i < used; ++i)
@@ -297,110 +347,215 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 4 : 3) int4_small_ker
         }
         __syncwarp();
     } else {
-        if (!p.items) asm volatile("griddepcontrol.wait;" ::: "memory");       // y may be the previous kernel's input
-        const int j = lane & 3, n = lane >> 2;
+        const int j = lane & 3, n = lane >> 2, blk = 2 * (warp & 3), half = warp >> 2;
         // this lane's columns 4 j.. of a 16-column step, in the 128-byte swizzle: 16-byte chunk 2 r + j / 2, XOR row
-        const uint32_t x_row = (uint32_t)(p.x_at + n * 128 + (j & 1) * 8);
+        uint32_t x_off[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            x_off[r] = (uint32_t)(p.x_at + half * p.x_sub + n * 128 + (j & 1) * 8 + (((2 * r + (j >> 1)) ^ n) << 4));
+        const uint32_t code_off = (uint32_t)((blk * 2 + half) * q4::kBlockBytes + lane * 16);
+        // the column block's first group in its unit, this lane's pair of rows in it
+        const int group0 = G32 ? 2 * half : p.group_shift == 6 ? half : 0, mine = group0 * 64 + blk * 8 + n;
+        const uint32_t zero_off = (uint32_t)(q4::kCodeBytes + mine * 2), scale_off = (uint32_t)(p.scales_at + mine * 4);
         int slot = 0;
-        uint32_t ph = 0;
-        for (int k = k0; k < k1; ++k) {
-            if (!__all_sync(0xffffffffu, wait_one(full(slot), ph, 3, wc))) break;
-            const uint32_t rec = base + slot * p.slot_bytes;
-            const uint32_t mine = (uint32_t)(warp * 8 + n);           // of a group's 64 pairs of rows
-            q4::Codes<T> codes;
-            float part[NT][4];
-            auto clear = [&] {
+        uint32_t ph = 0, rec = 0;
+        bool ok = true;
+        const uint8_t* ring = smem_raw + (base - raw);
+        q4::Codes<T> codes[2];
+        codes[0].zeros(8u, 8u);
+        codes[1].zeros(8u, 8u);
+        for (int64_t u = u0; u < u1;) {
+            const SmallTile t = small_tile(p, u / p.units);
+            const int ka = (int)(u % p.units), kz = (int)min((int64_t)p.units, ka + (u1 - u));
+            float acc[2][NT][4];
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) part[t][i] = 0.f;
-            };
-            auto begin = [&](int g) {                                 // group g of the unit
-                const uint32_t z = p.zeros ? lds_u16(rec + q4::kCodeBytes + (g * 64 + mine) * 2) : 0x0808u;
-                codes.zeros(z & 15u, z >> 8);
-                clear();
-            };
-            auto end = [&](int g) {
-                const float2 s = unpack2<T>(lds_u32(rec + p.scales_at + (g * 64 + mine) * 4));
+                for (int c = 0; c < NT; ++c)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    acc[t][0] = fmaf(s.x, part[t][0], acc[t][0]);
-                    acc[t][1] = fmaf(s.x, part[t][1], acc[t][1]);
-                    acc[t][2] = fmaf(s.y, part[t][2], acc[t][2]);
-                    acc[t][3] = fmaf(s.y, part[t][3], acc[t][3]);
+                    for (int i = 0; i < 4; ++i) acc[b][c][i] = 0.f;
+            for (int k = ka; k < kz; ++k) {
+                // a warp that gave up multiplies nothing more, but keeps meeting the others at every row tile's end
+                if (!ok || !(ok = __all_sync(0xffffffffu, wait_one(full(slot), ph, 3, wc)))) break;
+                const uint8_t* at = ring + rec;
+                uint32_t w[2][4];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint4 c = lds<uint4>(at, code_off + b * 2 * q4::kBlockBytes);
+                    w[b][0] = c.x; w[b][1] = c.y; w[b][2] = c.z; w[b][3] = c.w;
                 }
-            };
-            begin(0);
+                // the two row blocks' products alternate: each waits for its own last one only
+                float part[2][NT][4];
+                auto begin = [&](int b, int g) {
+                    if (p.zeros) {
+                        const uint32_t z = lds<uint16_t>(at, zero_off + b * 16 + g * 128);
+                        codes[b].zeros(z & 15u, z >> 8);
+                    }
+                };
+                auto end = [&](int b, int g) {
+                    const float2 s = unpack2<T>(lds<uint32_t>(at, scale_off + b * 32 + g * 256));
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint4 c = lds_v4(rec + (warp * 2 + half) * q4::kBlockBytes + lane * 16);
-                const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-                if (half == 1 && p.group_shift < 7) {
-                    end(p.group_shift == 6 ? 0 : 1);
-                    begin(p.group_shift == 6 ? 1 : 2);
-                }
+                    for (int c = 0; c < NT; ++c) {
+                        acc[b][c][0] = fmaf(s.x, part[b][c][0], acc[b][c][0]);
+                        acc[b][c][1] = fmaf(s.x, part[b][c][1], acc[b][c][1]);
+                        acc[b][c][2] = fmaf(s.y, part[b][c][2], acc[b][c][2]);
+                        acc[b][c][3] = fmaf(s.y, part[b][c][3], acc[b][c][3]);
+                    }
+                };
+                begin(0, 0);
+                begin(1, 0);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (r == 2 && p.group_shift == 5) {
-                        end(2 * half);
-                        begin(2 * half + 1);
+                    if (G32 && r == 2) {
+                        end(0, 0);
+                        end(1, 0);
+                        begin(0, 1);
+                        begin(1, 1);
                     }
-                    uint32_t a[4];
-                    codes.expand(w[r], a);
-                    const uint32_t at = rec + x_row + half * p.x_sub + (((2 * r + (j >> 1)) ^ n) << 4);
+                    uint2 xf[NT];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) mma16816(part[t], a, lds_v2(at + t * 1024), T());
+                    for (int c = 0; c < NT; ++c) xf[c] = lds<uint2>(at, x_off[r] + c * 1024);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t a[4];
+                        codes[b].expand(w[b][r], a);
+#pragma unroll
+                        for (int c = 0; c < NT; ++c) {
+                            if (r == 0 || (G32 && r == 2)) mma16816<true, T>(part[b][c], a, xf[c]);
+                            else mma16816<false, T>(part[b][c], a, xf[c]);
+                        }
+                    }
+                }
+                end(0, G32 ? 1 : 0);
+                end(1, G32 ? 1 : 0);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty(slot));
+                rec += (uint32_t)p.slot_bytes;
+                if (++slot == p.slots) {
+                    slot = 0;
+                    ph ^= 1u;
+                    rec = 0;
                 }
             }
-            end(p.group_shift == 7 ? 0 : p.group_shift == 6 ? 1 : 3);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty(slot));
-            advance(slot, ph, 1, p.slots);
+            // The row tile's sums [token][row]: the second column block's first, the first one's added to them.
+#pragma unroll
+            for (int h = 1; h >= 0; --h) {
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (half == h) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float* at = red + (c * 8 + 2 * j + (i & 1)) * kRowPad + (blk + b) * 16 + n + 8 * (i >> 1);
+                                *at = h ? acc[b][c][i] : acc[b][c][i] + *at;
+                            }
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (!clustered) {
+                T* y = reinterpret_cast<T*>(p.y);
+                if (kz - ka < p.units) {                             // shared with the neighbouring run
+                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128;
+                    for (int i = threadIdx.x; i < t.n * 32; i += 256)
+                        *reinterpret_cast<float4*>(part + i * 4) =
+                            *reinterpret_cast<const float4*>(red + (i >> 5) * kRowPad + (i & 31) * 4);
+                } else if (p.gated) {
+                    for (int i = threadIdx.x; i < t.n * 64; i += 256) {
+                        const int in = i & 63, at = (i >> 6) * kRowPad + in / 16 * 32 + in % 16, row = t.rt * 64 + in;
+                        if (row < p.out_rows)
+                            y[(int64_t)(t.first + (i >> 6)) * p.ldy + row] = gate_up<T>(red[at], red[at + 16]);
+                    }
+                } else {
+                    for (int i = threadIdx.x; i < t.n * 128; i += 256) {
+                        const int row = t.rt * 128 + (i & 127);
+                        if (row < p.out_rows)
+                            y[(int64_t)(t.first + (i >> 7)) * p.ldy + row] = from_f32<T>(red[(i >> 7) * kRowPad + (i & 127)]);
+                    }
+                }
+            }
+            u += kz - ka;
         }
     }
-    // Each CTA's partial tile [token][row] goes to the front of its own ring, all of whose copies have been read.
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(smem_raw + (base - raw));
-    if (warp < kComputeWarps) {
-        const int j = lane & 3, n = lane >> 2;
+    if (clustered) {
+        // Sum over the cluster, in column order; CTA `rank` finishes its share of the outputs.
+        cluster_sync_all();
+        if (u0 < u1) {
+            const SmallTile t = small_tile(p, u0 / p.units);
+            auto total = [&](int tok, int row) {
+                const uint32_t at = smem_u32(red + tok * kRowPad + row);
+                float v[8];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+                for (int c = 0; c < 8; ++c)
+                    if (c < p.splits) v[c] = ld_cluster_f32(cluster_addr(at, c));
+                float sum = v[0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                red[(t * 8 + 2 * j + (i & 1)) * kRowPad + warp * 16 + n + 8 * (i >> 1)] = acc[t][i];
+                for (int c = 1; c < 8; ++c)
+                    if (c < p.splits) sum += v[c];
+                return sum;
+            };
+            T* y = reinterpret_cast<T*>(p.y);
+            const int width = p.gated ? 64 : 128;
+            const int begin = t.n * width * rank / p.splits, end = t.n * width * (rank + 1) / p.splits;
+            for (int i = begin + threadIdx.x; i < end; i += kSmallThreads) {
+                const int tok = i / width, in = i % width, row = t.rt * width + in;
+                if (row >= p.out_rows) continue;
+                y[(int64_t)(t.first + tok) * p.ldy + row] =
+                    p.gated ? gate_up<T>(total(tok, in / 16 * 32 + in % 16), total(tok, in / 16 * 32 + 16 + in % 16))
+                            : from_f32<T>(total(tok, in));           // even row blocks are gates, odd ones their ups
+            }
+        }
+        cluster_sync_all();                                          // nobody leaves while its tile may still be read
     }
-    if (p.splits > 1) cluster_sync_all(); else __syncthreads();
-    // Sum over the cluster, in column order: CTA `rank` finishes every splits-th token... of all rows.
-    auto total = [&](int tok, int row) {
-        const uint32_t at = smem_u32(red + tok * kRowPad + row);
-        if (p.splits == 1) return __uint_as_float(lds_u32(at));
-        float v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-            if (c < p.splits) v[c] = ld_cluster_f32(cluster_addr(at, c));
-        float sum = v[0];
-#pragma unroll
-        for (int c = 1; c < 8; ++c)
-            if (c < p.splits) sum += v[c];
-        return sum;
-    };
+    if (p.routed && warp < kComputeWarps) {                          // what lies behind the last pair
+        for (int64_t r = *p.routed + blockIdx.x; r < p.pairs; r += gridDim.x)
+            for (int c = threadIdx.x; c < p.out_rows; c += 256) reinterpret_cast<T*>(p.y)[r * p.ldy + c] = from_f32<T>(0.f);
+    }
+}
+
+// Row tiles that several runs share: their fp32 partials added in run order. A block takes a row tile, a warp a token at
+// a time, a thread four rows.
+template <typename T> __global__ void __launch_bounds__(256) int4_small_join_kernel(const __grid_constant__ SmallParams p, int ctas) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t tile = blockIdx.x, tiles = small_tiles(p), units_all = tiles * p.units;
+    if (tile >= tiles) return;
+    const int64_t a = tile * p.units, z = a + p.units;
+    // the run that holds unit u: the last b whose begin is at most u
+    const int runs = small_runs(units_all, ctas);
+    const auto run_of = [&](int64_t u) { return (int)(((u + 1) * runs + units_all - 1) / units_all - 1); };
+    const int b0 = run_of(a), b1 = run_of(z - 1);
+    if (b0 == b1) return;                                            // one run wrote y itself
+    const SmallTile t = small_tile(p, tile);
+    const int which0 = small_begin(units_all, b0, runs) >= a ? 0 : 1, lane = threadIdx.x & 31;
     T* y = reinterpret_cast<T*>(p.y);
-    const int width = p.gated ? 64 : 128;
-    const int begin = count * width * rank / p.splits, end = count * width * (rank + 1) / p.splits;
-    for (int i = begin + threadIdx.x; i < end; i += kSmallThreads) {
-        const int tok = i / width, in = i % width;
-        const int64_t row = (int64_t)tile * width + in;
-        if (row >= p.out_rows) continue;
-        float v;
-        if (p.gated) {                                               // even row blocks are gates, odd ones their ups
-            const float g = total(tok, in / 16 * 32 + in % 16), u = total(tok, in / 16 * 32 + 16 + in % 16);
-            v = g / (1.f + expf(-g)) * u;
-        } else {
-            v = total(tok, in);
+    for (int tok = threadIdx.x >> 5; tok < t.n; tok += 8) {
+        const float* part = p.partial + (int64_t)tok * 128 + lane * 4;
+        const int64_t stride = (int64_t)p.n_max * 128;
+        float4 sum = __ldcg(reinterpret_cast<const float4*>(part + (2 * b0 + which0) * stride));
+#pragma unroll 4
+        for (int b = b0 + 1; b <= b1; ++b) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 2 * (int64_t)b * stride));
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
-        y[(first + tok) * p.ldy + row] = from_f32<T>(v);
+        T* out = y + (int64_t)(t.first + tok) * p.ldy;
+        const float mine[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (p.gated) {                                               // lanes 8 i .. + 3 hold gates, + 4 .. + 7 their ups
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float up = __shfl_xor_sync(0xffffffffu, mine[c], 4);
+                const int row = t.rt * 64 + (lane >> 3) * 16 + (lane & 3) * 4 + c;
+                if (!(lane & 4) && row < p.out_rows) out[row] = gate_up<T>(mine[c], up);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int row = t.rt * 128 + lane * 4 + c;
+                if (row < p.out_rows) out[row] = from_f32<T>(mine[c]);
+            }
+        }
     }
-    if (p.splits > 1) cluster_sync_all();                            // nobody leaves while its tile may still be read
 }
 
 unsigned next_seq() {
@@ -410,61 +565,97 @@ unsigned next_seq() {
     return v;
 }
 
-template <typename T, int NT>
-int launch_small(const CUtensorMap& map, SmallParams& p, int64_t col_tiles, cudaStream_t st, const char* what) {
-    auto kernel = int4_small_kernel<T, NT>;
-    const int smem = 1024 + p.slots * p.slot_bytes + 8 * 2 * kMaxSlots;
-    if (int e = allow_smem((const void*)kernel, smem, what)) return e;
+// How a call of up to 32 tokens a tile is cut: shares of a cluster's CTAs where they are all resident at once, else
+// runs, two CTAs an SM.
+struct SmallPlan {
+    int nt, splits, ctas, slots, slot_bytes, x_at, x_sub, smem;
+    int64_t col_tiles, tiles;
+    size_t workspace;
+};
+
+SmallPlan plan_small(const Int4Call& c) {
+    SmallPlan pl = {};
+    const bool routed = c.items != nullptr;
+    const int64_t most = routed ? c.item_tokens : c.tokens < 32 ? c.tokens : 32;
+    pl.nt = (int)q4::div_up(most, 8);
+    pl.col_tiles = routed ? c.max_items : q4::div_up(c.tokens, pl.nt * 8);
+    pl.tiles = q4::row_tiles(c.rows, c.gated) * pl.col_tiles;
+    const int64_t units = q4::div_up(c.cols, q4::kUnitCols), resident = 2 * (int64_t)sm_count();
+    static const char* e1 = getenv("X_SPL"); const int mode = e1 ? atoi(e1) : 0;
+    if (mode == 0 ? pl.tiles * 2 <= resident : mode == 1) {
+        int64_t s = resident / pl.tiles;
+        if (s > 8) s = 8;
+        if (s > units / 2) s = units / 2;
+        if (s < 1) s = 1;
+        pl.splits = (int)s;
+        pl.ctas = (int)(pl.tiles * s);
+    } else {
+        const int64_t all = pl.tiles * units;
+        pl.ctas = (int)(all < resident ? all : resident);
+        pl.workspace = (size_t)pl.ctas * 2 * pl.nt * 8 * 128 * sizeof(float);
+    }
+    const int record = q4::unit_bytes(c.group, c.has_zeros);
+    pl.x_at = (int)q4::div_up(record, 1024) * 1024;
+    pl.x_sub = pl.nt * 8 * 128;
+    pl.slot_bytes = pl.x_at + 2 * pl.x_sub;
+    const int fixed = 1024 + pl.nt * 8 * kRowPad * 4 + 8 * 2 * kMaxSlots;
+    pl.slots = (112 * 1024 - fixed) / pl.slot_bytes;                 // two CTAs an SM
+    if (pl.slots > kMaxSlots) pl.slots = kMaxSlots;
+    pl.smem = fixed + pl.slots * pl.slot_bytes;
+    return pl;
+}
+
+template <typename T, int NT, bool G32>
+int launch_small(const CUtensorMap& map, const SmallParams& p, const SmallPlan& pl, cudaStream_t st, const char* what) {
+    auto kernel = int4_small_kernel<T, NT, G32>;
+    if (int e = allow_smem((const void*)kernel, pl.smem, what)) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.splits;
+    attr[1].val.clusterDim.x = pl.splits;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(p.row_tiles * p.splits), (unsigned)col_tiles);
+    cfg.gridDim = dim3((unsigned)pl.ctas);
     cfg.blockDim = dim3(kSmallThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = pl.smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = p.splits > 1 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kernel, map, (const SmallParams)p);
+    cfg.numAttrs = pl.splits > 0 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, map, p);
+    if (int e = launch_status(what)) return e;
+    if (pl.splits > 0) return P2P_OK;
+    cfg.gridDim = dim3((unsigned)pl.tiles);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, int4_small_join_kernel<T>, p, pl.ctas);
     return launch_status(what);
 }
 
-// Up to 32 tokens (an item, or a tile of the tokens).
 template <typename T>
-int run_small(const Int4Call& c, const int32_t* order, int topk, cudaStream_t st, const char* what) {
+int run_small(const Int4Call& c, const int32_t* order, int topk, void* workspace, cudaStream_t st, const char* what) {
+    const SmallPlan pl = plan_small(c);
     SmallParams p = {};
-    const bool routed = c.items != nullptr;
-    const int64_t most = routed ? c.item_tokens : c.tokens < 32 ? c.tokens : 32;
-    const int nt = (int)q4::div_up(most, 8);
-    const int64_t col_tiles = routed ? c.max_items : q4::div_up(c.tokens, nt * 8);
-    if (col_tiles > 65535) return fail(P2P_EUNSUPPORTED, "%s: %lld tiles of tokens, at most 65535", what, (long long)col_tiles);
     p.layout = reinterpret_cast<const uint8_t*>(c.layout);
     p.record = q4::unit_bytes(c.group, c.has_zeros);
     p.zeros = c.has_zeros;
     p.scales_at = q4::kCodeBytes + q4::unit_zero_bytes(c.group, c.has_zeros);
     p.units = (int)q4::div_up(c.cols, q4::kUnitCols);
     p.row_tiles = (int)q4::row_tiles(c.rows, c.gated);
+    p.col_tiles = (int)pl.col_tiles;
     p.group_shift = c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
     p.gated = c.gated;
     p.tokens = (int)c.tokens;
+    p.n_max = pl.nt * 8;
     p.out_rows = (int)(c.gated ? c.rows / 2 : c.rows);
-    p.x_at = (int)q4::div_up(p.record, 1024) * 1024;
-    p.x_sub = nt * 8 * 128;
-    p.slot_bytes = p.x_at + 2 * p.x_sub;
-    const int64_t ctas = p.row_tiles * col_tiles;
-    p.splits = 1;
-    while (p.splits < 8 && ctas * p.splits < 3 * sm_count() && p.units / (2 * p.splits) >= 2) p.splits *= 2;
-    const int share = (int)q4::div_up(p.units, p.splits);
-    p.slots = (72 * 1024 - 1024) / p.slot_bytes;
-    if (p.slots > kMaxSlots) p.slots = kMaxSlots;
-    if (p.slots > share) p.slots = share;
-    // the partial tile reuses the ring
-    const int tile_bytes = nt * 8 * kRowPad * 4;
-    while (p.slots * p.slot_bytes < tile_bytes) ++p.slots;
+    p.splits = pl.splits;
+    p.partial = reinterpret_cast<float*>(workspace);
+    p.slots = pl.slots;
+    p.slot_bytes = pl.slot_bytes;
+    p.x_at = pl.x_at;
+    p.x_sub = pl.x_sub;
     p.y = c.y;
     p.ldy = c.ldy;
     p.items = c.items;
@@ -475,14 +666,15 @@ int run_small(const Int4Call& c, const int32_t* order, int topk, cudaStream_t st
     p.pairs = c.pairs;
     p.wait_ns = kSmallWaitNs;
     p.seq = next_seq();
-    const int64_t x_rows = order ? c.pairs / topk : routed ? c.pairs : c.tokens;
+    const int64_t x_rows = order ? c.pairs / topk : c.items ? c.pairs : c.tokens;
     CUtensorMap map;
-    if (int e = encode_x_map(&map, c.x, c.dtype, x_rows, c.cols, c.ldx, order ? 1 : nt * 8)) return e;
-    switch (nt) {
-        case 1: return launch_small<T, 1>(map, p, col_tiles, st, what);
-        case 2: return launch_small<T, 2>(map, p, col_tiles, st, what);
-        case 3: return launch_small<T, 3>(map, p, col_tiles, st, what);
-        default: return launch_small<T, 4>(map, p, col_tiles, st, what);
+    if (int e = encode_x_map(&map, c.x, c.dtype, x_rows, c.cols, c.ldx, order ? 1 : pl.nt * 8)) return e;
+    const bool g32 = c.group == 32;
+    switch (pl.nt) {
+        case 1: return g32 ? launch_small<T, 1, true>(map, p, pl, st, what) : launch_small<T, 1, false>(map, p, pl, st, what);
+        case 2: return g32 ? launch_small<T, 2, true>(map, p, pl, st, what) : launch_small<T, 2, false>(map, p, pl, st, what);
+        case 3: return g32 ? launch_small<T, 3, true>(map, p, pl, st, what) : launch_small<T, 3, false>(map, p, pl, st, what);
+        default: return g32 ? launch_small<T, 4, true>(map, p, pl, st, what) : launch_small<T, 4, false>(map, p, pl, st, what);
     }
 }
 
@@ -568,8 +760,20 @@ int check_int4(const Int4Call& c, const char* what) {
 }  // namespace
 
 extern "C" size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated) {
-    if (tokens <= kSmallTokens || rows <= 0 || cols <= 0 || (gated && rows % 2)) return 0;
-    return int4_tc_workspace(tokens, rows, cols, gated);
+    if (tokens <= 0 || rows <= 0 || cols <= 0 || (gated && rows % 2)) return 0;
+    if (tokens > kSmallTokens) return int4_tc_workspace(tokens, rows, cols, gated);
+    Int4Call c = {};
+    c.tokens = tokens; c.rows = rows; c.cols = cols; c.gated = gated != 0; c.group = 128;
+    return plan_small(c).workspace;
+}
+
+extern "C" size_t p2p_int4_grouped_workspace(int64_t max_items, int64_t item_tokens, int64_t rows, int64_t cols, int gated) {
+    if (max_items <= 0 || item_tokens <= 0 || item_tokens > kSmallTokens || rows <= 0 || cols <= 0 || (gated && rows % 2)) return 0;
+    Int4Call c = {};
+    static const int32_t some = 0;
+    c.items = &some; c.max_items = max_items; c.item_tokens = item_tokens;
+    c.rows = rows; c.cols = cols; c.gated = gated != 0; c.group = 128;
+    return plan_small(c).workspace;
 }
 
 extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout,
@@ -583,12 +787,12 @@ extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t col
     c.rows = rows; c.group = group; c.gated = gated != 0; c.y = y; c.ldy = ldy;
     if (int e = check_int4(c, "p2p_int4_mm")) return e;
     cudaStream_t st = as_stream(stream);
-    if (tokens <= kSmallTokens)
-        return dtype == P2P_BF16 ? run_small<__nv_bfloat16>(c, nullptr, 1, st, "p2p_int4_mm")
-                                 : run_small<__half>(c, nullptr, 1, st, "p2p_int4_mm");
     const size_t need = p2p_int4_workspace(tokens, rows, cols, gated);
     P2P_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                 "p2p_int4_mm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (tokens <= kSmallTokens)
+        return dtype == P2P_BF16 ? run_small<__nv_bfloat16>(c, nullptr, 1, workspace, st, "p2p_int4_mm")
+                                 : run_small<__half>(c, nullptr, 1, workspace, st, "p2p_int4_mm");
     return int4_tc_run(c, workspace, st, "p2p_int4_mm");
 }
 
@@ -596,7 +800,7 @@ extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t 
                                 int has_zeros, int64_t rows, int group, int gated,
                                 const int32_t* items, const int32_t* n_items, int64_t max_items, int64_t item_tokens,
                                 const int32_t* order, int topk, const int32_t* routed, int64_t pairs, void* y,
-                                int64_t ldy, void* stream) {
+                                int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
     P2P_REQUIRE(max_items >= 0 && rows >= 0 && item_tokens >= 0 && pairs >= 0 && pairs <= 0x7fffffff,
                 "p2p_int4_grouped: bad shape");
     if (max_items == 0 || rows == 0 || item_tokens == 0 || pairs == 0) return P2P_OK;
@@ -613,9 +817,12 @@ extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t 
     c.routed = routed;
     if (int e = check_int4(c, "p2p_int4_grouped")) return e;
     cudaStream_t st = as_stream(stream);
+    const size_t need = p2p_int4_grouped_workspace(max_items, item_tokens, rows, cols, gated);
+    P2P_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+                "p2p_int4_grouped: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (item_tokens <= kSmallTokens)
-        return dtype == P2P_BF16 ? run_small<__nv_bfloat16>(c, order, topk, st, "p2p_int4_grouped")
-                                 : run_small<__half>(c, order, topk, st, "p2p_int4_grouped");
+        return dtype == P2P_BF16 ? run_small<__nv_bfloat16>(c, order, topk, workspace, st, "p2p_int4_grouped")
+                                 : run_small<__half>(c, order, topk, workspace, st, "p2p_int4_grouped");
     return int4_tc_run(c, nullptr, st, "p2p_int4_grouped");
 }
 

@@ -114,10 +114,12 @@ void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& layout, bool zer
     // few pairs: the product picks x's rows itself
     const bool pick = gather && most <= kSmallTokens;
     const at::Tensor x = aligned_rows(gather && !pick ? moe_spread(x_in, where, offsets, topk) : x_in);
+    const size_t need = p2p_int4_grouped_workspace(items.numel() / 4, most, rows, cols, gated);
+    const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte)) : at::Tensor();
     check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, aligned_stride(x), layout.data_ptr(), zeros, rows, (int)group, gated, ints(items, x, 0, "items"),
                            ints(n_items, x, 1, "n_items"), items.numel() / 4, most,
                            pick ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
-                           out.data_ptr(), row_stride(out), stream_of(x)),
+                           out.data_ptr(), row_stride(out), need ? ws.data_ptr() : nullptr, need, stream_of(x)),
           "p2p_int4_grouped");
 }
 

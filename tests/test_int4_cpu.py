@@ -42,15 +42,15 @@ def test_layout_bytes(lib):
     (lambda l: l.p2p_int4_mm(FAKE, 0, 4, 64, 64, FAKE + 4, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"16-byte"),
     (lambda l: l.p2p_int4_mm(None, 0, 4, 64, 64, FAKE, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"null"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, 0, 16, 64, 0, FAKE, FAKE, 4, 273, None, 1, None, 4,
-                                  FAKE, 16, None), -1, b"at most 272"),
+                                  FAKE, 16, None, 0, None), -1, b"at most 272"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, 0, 16, 64, 0, FAKE + 4, FAKE, 4, 8, None, 1, None, 4,
-                                  FAKE, 16, None), -1, b"16-byte"),
+                                  FAKE, 16, None, 0, None), -1, b"16-byte"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, 0, 16, 64, 0, FAKE, FAKE, 4, 8, FAKE, 0, None, 4,
-                                  FAKE, 16, None), -1, b"topk"),
+                                  FAKE, 16, None, 0, None), -1, b"topk"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 64, FAKE, 0, 16, 64, 0, FAKE, FAKE, 4, 9, FAKE, 1, None, 4,
-                                  FAKE, 16, None), -1, b"in the order's places"),
+                                  FAKE, 16, None, 0, None), -1, b"in the order's places"),
     (lambda l: l.p2p_int4_grouped(FAKE, 0, 64, 68, FAKE, 0, 16, 64, 0, FAKE, FAKE, 4, 9, None, 1, None, 4,
-                                  FAKE, 16, None), -1, b"16-byte"),
+                                  FAKE, 16, None, 0, None), -1, b"16-byte"),
     (lambda l: l.p2p_int4_mm(FAKE, 0, 9, 64, 68, FAKE, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"16-byte"),
     (lambda l: l.p2p_int4_mm(FAKE, 0, 33, 64, 64, FAKE, 0, 16, 64, 0, FAKE, 16, None, 0, None), -1, b"workspace"),
     (lambda l: l.p2p_moe_sort(FAKE, 4, 64, 1025, FAKE, FAKE, FAKE, FAKE, 2000, 32, FAKE, None), -2, b"at most 1024"),
@@ -74,7 +74,7 @@ def test_empty_work_launches_nothing(lib):
     assert lib.p2p_int4_quantize(None, 0, 0, 64, 64, 64, None, None, None, None) == 0
     assert lib.p2p_int4_mm(None, 0, 0, 64, 64, None, 0, 16, 64, 0, None, 16, None, 0, None) == 0
     assert lib.p2p_int4_grouped(None, 0, 64, 64, None, 0, 16, 64, 0, None, None, 0, 0, None, 1, None, 0, None,
-                                16, None) == 0
+                                16, None, 0, None) == 0
     assert lib.p2p_moe_spread(None, 0, 0, 2, 8, 8, None, None, None, 8, None) == 0
     assert lib.p2p_moe_sum(None, 0, 0, 2, 8, 8, None, None, 2, None, 8, None) == 0
 
