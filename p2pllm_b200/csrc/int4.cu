@@ -212,6 +212,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ int token_of(int column) { return 2 * column - (column >> 2) * 7; }
+
 // Row tile `id` of a launch: whose rows, which tokens.
 struct SmallTile {
     const uint8_t* records;
@@ -253,7 +255,7 @@ template <typename T> __device__ __forceinline__ T gate_up(float g, float u) { r
 // columns in fp32, and the group's scale multiplies that sum on its way into the fp32 accumulators: no weight is ever
 // rounded. G32: groups of 32 columns, two a column block (else one holds the block or more).
 template <typename T, int NT, bool G32>
-__global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __grid_constant__ CUtensorMap tmap_x,
+__global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                                       const __grid_constant__ SmallParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -293,6 +295,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
 
     if (warp == kComputeWarps) {
         if (elect_one()) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_x)) : "memory");
             const int n_slots = p.slots;
             const uint32_t w_bytes = (uint32_t)p.record;
             bool ok = true;
@@ -348,11 +351,14 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
         __syncwarp();
     } else {
         const int j = lane & 3, n = lane >> 2, blk = 2 * (warp & 3), half = warp >> 2;
-        // this lane's columns 4 j.. of a 16-column step, in the 128-byte swizzle: 16-byte chunk 2 r + j / 2, XOR row
+        // this lane's columns 4 j.. of a 16-column step, in the 128-byte swizzle: 16-byte chunk 2 r + j / 2, XOR token.
+        // Column n of a product is token 2 n, or 2 n - 7 for n >= 4: a half warp then reads tokens 0, 2, 4, 6 or 1, 3, 5,
+        // 7, whose chunks fill all banks once (tokens 0 to 3 share half of them).
+        const int tok = token_of(n);
         uint32_t x_off[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            x_off[r] = (uint32_t)(p.x_at + half * p.x_sub + n * 128 + (j & 1) * 8 + (((2 * r + (j >> 1)) ^ n) << 4));
+            x_off[r] = (uint32_t)(p.x_at + half * p.x_sub + tok * 128 + (j & 1) * 8 + (((2 * r + (j >> 1)) ^ tok) << 4));
         const uint32_t code_off = (uint32_t)((blk * 2 + half) * q4::kBlockBytes + lane * 16);
         // the column block's first group in its unit, this lane's pair of rows in it
         const int group0 = G32 ? 2 * half : p.group_shift == 6 ? half : 0, mine = group0 * 64 + blk * 8 + n;
@@ -448,7 +454,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                float* at = red + (c * 8 + 2 * j + (i & 1)) * kRowPad + (blk + b) * 16 + n + 8 * (i >> 1);
+                                float* at = red + (c * 8 + token_of(2 * j + (i & 1))) * kRowPad + (blk + b) * 16 + n + 8 * (i >> 1);
                                 *at = h ? acc[b][c][i] : acc[b][c][i] + *at;
                             }
                 }
@@ -580,7 +586,7 @@ SmallPlan plan_small(const Int4Call& c) {
     pl.nt = (int)q4::div_up(most, 8);
     pl.col_tiles = routed ? c.max_items : q4::div_up(c.tokens, pl.nt * 8);
     pl.tiles = q4::row_tiles(c.rows, c.gated) * pl.col_tiles;
-    const int64_t units = q4::div_up(c.cols, q4::kUnitCols), resident = 2 * (int64_t)sm_count();
+    const int64_t units = q4::div_up(c.cols, q4::kUnitCols), per_sm = pl.nt <= 2 ? 3 : 2, resident = per_sm * sm_count();
     static const char* e1 = getenv("X_SPL"); const int mode = e1 ? atoi(e1) : 0;
     if (mode == 0 ? pl.tiles * 2 <= resident : mode == 1) {
         int64_t s = resident / pl.tiles;
@@ -599,7 +605,7 @@ SmallPlan plan_small(const Int4Call& c) {
     pl.x_sub = pl.nt * 8 * 128;
     pl.slot_bytes = pl.x_at + 2 * pl.x_sub;
     const int fixed = 1024 + pl.nt * 8 * kRowPad * 4 + 8 * 2 * kMaxSlots;
-    pl.slots = (112 * 1024 - fixed) / pl.slot_bytes;                 // two CTAs an SM
+    pl.slots = (int)((226 * 1024 / per_sm - 1024 - fixed) / pl.slot_bytes);
     if (pl.slots > kMaxSlots) pl.slots = kMaxSlots;
     pl.smem = fixed + pl.slots * pl.slot_bytes;
     return pl;
@@ -744,7 +750,7 @@ extern "C" int p2p_int4_layout(const uint8_t* codes, const void* scales, const u
 namespace {
 // Calls of up to this many tokens take the kernel above, which streams weights at the memory's rate and multiplies on
 // the warps' own tensor path; above, that path's rate would bind.
-constexpr int64_t kSmallTokens = 32;
+static const char* e_st = getenv("X_ST"); static const int64_t kSmallTokens = e_st ? atoi(e_st) : 32;
 
 int check_int4(const Int4Call& c, const char* what) {
     if (c.dtype != P2P_BF16 && c.dtype != P2P_F16) return fail(P2P_EUNSUPPORTED, "%s: bf16 or f16", what);

@@ -32,12 +32,12 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kPromoteWarps = 8, kBuildWarps = 8;
-constexpr int kBuildWarp = kPromoteWarps;               // 8..15
-constexpr int kWeightWarp = kBuildWarp + kBuildWarps;   // 16
-constexpr int kXWarp = kWeightWarp + 1;                 // 17
-constexpr int kMmaWarp = kWeightWarp + 2;               // 18, 19
-constexpr int kThreads = 640;
+constexpr int kPromoteWarps = 8;
+constexpr int kBuildWarp = kPromoteWarps;               // 8..
+constexpr int kGroupWarps = 8;                          // warps that build one unit
+// Up to 64 tokens the codes' turn binds: two groups of builders take alternate units.
+constexpr int build_groups(int nh) { return nh <= 32 ? 2 : 1; }
+constexpr int threads_of(int nh) { return (kPromoteWarps + build_groups(nh) * kGroupWarps + 4) * 32; }
 constexpr int kWSlotBytes = q4::kCodeBytes + 512;       // codes and up to four groups' zero points
 constexpr int kSSlotBytes = 1024;                       // up to four groups' scales
 constexpr int kACols = 64;                              // TMEM columns of one unit's A tile
@@ -132,11 +132,13 @@ __device__ __forceinline__ int64_t run_begin(int64_t units_all, int units, int64
 
 // NH: columns of the larger half's accumulator, in registers of the warps that promote it.
 template <typename T, int NH>
-__global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
+__global__ void __launch_bounds__(threads_of(NH), 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                               const __grid_constant__ TcParams p) {
     // 640 threads start with 96 registers each; the promoting warps need an accumulator of up to 144 and take what the
     // others give back: 256 x 176 + 256 x 48 + 128 x 32 = 640 x 96.
     constexpr bool kSplitRegs = NH >= 64;
+    constexpr int kGroups = build_groups(NH), kWeightWarp = kBuildWarp + kGroups * kGroupWarps;
+    constexpr int kXWarp = kWeightWarp + 1, kMmaWarp = kWeightWarp + 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -160,9 +162,9 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     const WaitCtl wc{&g_int4_error, &g_int4_failed_seq, p.wait_ns, p.seq};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < SW; ++s) { mbar_init(wfull(s), 1); mbar_init(wempty(s), kBuildWarps); }
+        for (int s = 0; s < SW; ++s) { mbar_init(wfull(s), 1); mbar_init(wempty(s), kGroupWarps); }
         for (int s = 0; s < SX; ++s) { mbar_init(xfull(s), 1); mbar_init(xempty(s), 2); }
-        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kBuildWarps); mbar_init(aempty(s), 2); }
+        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kGroupWarps); mbar_init(aempty(s), 2); }
         for (int b = 0; b < NB; ++b)
             for (int h = 0; h < 2; ++h) { mbar_init(dfull(h, b), 1); mbar_init(dempty(h, b), 4); }
         for (int s = 0; s < kSSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), kPromoteWarps); }
@@ -293,14 +295,16 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         }
     } else if (warp >= kBuildWarp) {
         if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-        const int w = warp - kBuildWarp, blk = 2 * (w & 3) + (w >> 2);          // lanes 32 (w % 4).. are this warp's
+        const int group = (warp - kBuildWarp) / kGroupWarps, w = (warp - kBuildWarp) % kGroupWarps;
+        const int blk = 2 * (w & 3) + (w >> 2);                                 // lanes 32 (w % 4).. are this warp's
         const uint32_t lanes = (uint32_t)(16 * blk) << 16;
-        int sw = 0, sa = 0, used = 0;
+        int sw = group, sa = group, used = group;
         uint32_t phw = 0, pha = 0;
         bool ok = true;
-        for (int64_t u = u0; u < u1 && ok;) {
-            const Tile t = tile_at(p, u, u1);
-            for (int k = t.k0; k < t.k1; ++k) {
+        q4::Codes<T> codes;
+        codes.zeros(8u, 8u);
+        for (int64_t u = u0 + group; u < u1 && ok; u += kGroups) {
+            {
                 if (!(ok = wait_all(wfull(sw), phw, 9, wc))) break;
                 const uint32_t rec = w_ring + sw * kWSlotBytes, at = rec + blk * 2 * q4::kBlockBytes + lane * 16;
                 const uint4 c[2] = {lds_v4(at), lds_v4(at + q4::kBlockBytes)};
@@ -312,17 +316,19 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 }
                 if (used >= SA && !(ok = wait_all(aempty(sa), pha ^ 1u, 10, wc))) break;
                 tc_fence_after();
-                q4::Codes<T> codes;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t words[4] = {c[half].x, c[half].y, c[half].z, c[half].w};
                     uint32_t r[16];
                     // groups of 128: one zero point a unit, 64: one a half, 32: one a quarter
-                    const uint32_t z0 = p.group_shift == 5 ? zs[2 * half] : p.group_shift == 6 ? zs[half] : zs[0];
-                    codes.zeros(z0 & 15u, z0 >> 8);
+                    if (p.zero_bytes) {
+                        const uint32_t z0 = p.group_shift == 5 ? zs[2 * half] : p.group_shift == 6 ? zs[half] : zs[0];
+                        codes.zeros(z0 & 15u, z0 >> 8);
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (i == 2 && p.group_shift == 5) codes.zeros(zs[2 * half + 1] & 15u, zs[2 * half + 1] >> 8);
+                        if (i == 2 && p.zero_bytes && p.group_shift == 5)
+                            codes.zeros(zs[2 * half + 1] & 15u, zs[2 * half + 1] >> 8);
                         uint32_t a[4];
                         codes.expand(words[i], a);
                         r[4 * i] = a[0]; r[4 * i + 1] = a[2]; r[4 * i + 2] = a[1]; r[4 * i + 3] = a[3];
@@ -335,11 +341,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(afull(sa));
-                ++used;
-                advance(sw, phw, 1, SW);
-                advance(sa, pha, 1, SA);
+                used += kGroups;
+                advance(sw, phw, kGroups, SW);
+                advance(sa, pha, kGroups, SA);
             }
-            u += t.k1 - t.k0;
         }
     } else {
         if (kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
@@ -371,15 +376,18 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 if (!(ok = wait_all(dfull(h, sb), phb, 11, wc))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + d_col(h, sb);
-                uint32_t v[2][16];
-                if (nh > 0) ld16_async(d, v[0]);
+                // 16 columns at a time, the next ones on their way meanwhile where there are more than two
+                constexpr int kBufs = NH > 32 ? 2 : 1;
+                uint32_t v[kBufs][16];
+                if (kBufs == 2 && nh > 0) ld16_async(d, v[0]);
 #pragma unroll
                 for (int c = 0; c < NH / 16; ++c) {
                     if (c * 16 < nh) {
-                        ld16_wait(v[c & 1]);
-                        if ((c + 1) * 16 < nh) ld16_async(d + (c + 1) * 16, v[(c + 1) & 1]);
+                        if (kBufs == 1) ld16_async(d + c * 16, v[0]);
+                        ld16_wait(v[c % kBufs]);
+                        if (kBufs == 2 && (c + 1) * 16 < nh) ld16_async(d + (c + 1) * 16, v[(c + 1) % kBufs]);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], s2, v[c & 1][2 * i], v[c & 1][2 * i + 1]);
+                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], s2, v[c % kBufs][2 * i], v[c % kBufs][2 * i + 1]);
                     }
                 }
                 tc_fence_before();
@@ -524,7 +532,7 @@ template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcPara
                 return fail(P2P_ECUDA, "%s: %s", what, cudaGetErrorString(cudaGetLastError()));
             regs = a.numRegs;
         }
-        if (regs * kThreads < 256 * 176 + 256 * 48 + 128 * 32)
+        if (regs * threads_of(NH) < 256 * 176 + 256 * 48 + 128 * 32)
             return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread, 96 needed", what, regs.load());
     }
     cudaLaunchConfig_t cfg = {};
@@ -532,7 +540,7 @@ template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcPara
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads_of(NH));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
