@@ -12,10 +12,12 @@
 //   warp 17 (x)         TMA of each unit's x tile [tokens x 128] (two 64-column boxes, 128-byte swizzle)
 //   warps 8-15 (build)  warp w turns the codes of one 16-row block into bf16 / f16 integers and stores them into the
 //                       unit's A tile in tensor memory (two tcgen05.st.16x256b.x4: the layout is that store's order)
-//   warps 18, 19 (MMA)  one thread each issues tcgen05.mma kind::f16, A from TMEM, M = 128, for one half of the tokens:
-//                       a group's columns into a zeroed accumulator, then a commit
-//   warps 0-3, 4-7      read the two halves' accumulators out, group after group, acc += scale * sum (packed fp32
-//                       pairs), and write the finished row tile: y itself, silu(gate) * up of it, or, where the tile
+//   two warps (MMA)     one thread each issues tcgen05.mma kind::f16, A from TMEM, M = 128: a group's columns times a
+//                       piece of the tokens (quarters, halves, or all of few) into a zeroed accumulator, then a commit.
+//                       The warps take the even and the odd pieces, or of a single piece alternate units: a look at a
+//                       barrier costs an issuing thread 130 cycles even when it has nothing to wait for
+//   warps 0-3, 4-7      read the even and the odd pieces' accumulators out, group after group, acc += scale * sum
+//                       (packed fp32 pairs), while other pieces multiply, and write the finished row tile: y itself, silu(gate) * up of it, or, where the tile
 //                       is shared with the neighbouring run, an fp32 partial that int4_join_kernel adds in run order
 //
 // Every wait is bounded (2 s): a launch that gives up records where, issues nothing more, drains what it issued and
@@ -36,13 +38,13 @@ constexpr int kPromoteWarps = 8;
 constexpr int kBuildWarp = kPromoteWarps;               // 8..
 constexpr int kGroupWarps = 8;                          // warps that build one unit
 // Up to 64 tokens the codes' turn binds: two groups of builders take alternate units.
-constexpr int build_groups(int nh) { return nh <= 32 ? 2 : 1; }
-constexpr int threads_of(int nh) { return (kPromoteWarps + build_groups(nh) * kGroupWarps + 4) * 32; }
+constexpr int build_groups(int acc) { return acc <= 32 ? 2 : 1; }
+constexpr int threads_of(int acc) { return (kPromoteWarps + build_groups(acc) * kGroupWarps + 4) * 32; }
 constexpr int kWSlotBytes = q4::kCodeBytes + 512;       // codes and up to four groups' zero points
 constexpr int kSSlotBytes = 1024;                       // up to four groups' scales
 constexpr int kACols = 64;                              // TMEM columns of one unit's A tile
 constexpr int kTmemCols = 512;
-constexpr int kMaxW = 12, kMaxX = 8, kMaxA = 6, kMaxBuf = 2;
+constexpr int kMaxW = 12, kMaxX = 8, kMaxA = 6, kMaxBuf = 4, kMaxPieces = 4;
 constexpr int kSSlots = 16;                             // scales wait for the rings before them: more than W + A slots hold
 constexpr int kSmemLimit = 227 * 1024 - 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -90,6 +92,25 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t s, uint32_t lo, uin
 }
 __device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(v >> (32 * i))); }
 
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// Up to three barriers at once: their looks overlap.
+__device__ __forceinline__ bool wait_three(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2,
+                                           bool third, int site, const WaitCtl& wc) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i) {
+        const bool r0 = mbar_test(b0, p0), r1 = mbar_test(b1, p1), r2 = mbar_test(third ? b2 : b0, third ? p2 : p0);
+        if (r0 && r1 && r2) return true;
+    }
+    return wait_one(b0, p0, site, wc) && wait_one(b1, p1, site + 1, wc) && (!third || wait_one(b2, p2, site + 2, wc));
+}
+
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
     return __all_sync(0xffffffffu, wait_one(bar, parity, site, wc));
 }
@@ -122,22 +143,31 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t u, int64_t u1
     }
     return t;
 }
-// Tokens of the first half (a multiple of 16) and of both.
-__device__ __forceinline__ int n_total(int n) { return (n + 15) & ~15; }
-__device__ __forceinline__ int n_first(int n) { return (n_total(n) / 2 + 15) & ~15; }
+// Pieces of the tokens, each a multiple of 16: all of them up to 32, halves up to 128, quarters above. (An accumulator
+// that is read out cannot take products: with four pieces three multiply meanwhile.)
+__host__ __device__ constexpr int n_total(int n) { return (n + 15) & ~15; }
+__host__ __device__ constexpr int pieces_of(int n_max) { return n_max <= 32 ? 1 : n_max <= 128 ? 2 : 4; }
+template <int PIECES> __device__ __forceinline__ int piece_size(int n, int i) { return (n_total(n) / 16 - i + PIECES - 1) / PIECES * 16; }
+template <int PIECES> __device__ __forceinline__ int piece_begin(int n, int i) {
+    int at = 0;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) at += k < i ? piece_size<PIECES>(n, k) : 0;
+    return at;
+}
 
 __device__ __forceinline__ int64_t run_begin(int64_t units_all, int units, int64_t b, int ctas, bool split) {
     return split ? units_all * b / ctas : units_all / units * b / ctas * units;
 }
 
-// NH: columns of the larger half's accumulator, in registers of the warps that promote it.
-template <typename T, int NH>
-__global__ void __launch_bounds__(threads_of(NH), 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
+// PIECES of the tokens; W0, W1: the most columns of a promoting warp's first and second piece, whose sums it holds in
+// registers (W1 = 0: it has one).
+template <typename T, int PIECES, int W0, int W1>
+__global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                               const __grid_constant__ TcParams p) {
     // 640 threads start with 96 registers each; the promoting warps need an accumulator of up to 144 and take what the
     // others give back: 256 x 176 + 256 x 48 + 128 x 32 = 640 x 96.
-    constexpr bool kSplitRegs = NH >= 64;
-    constexpr int kGroups = build_groups(NH), kWeightWarp = kBuildWarp + kGroups * kGroupWarps;
+    constexpr bool kSplitRegs = W0 + W1 >= 64;
+    constexpr int kGroups = build_groups(W0 + W1), kWeightWarp = kBuildWarp + kGroups * kGroupWarps;
     constexpr int kXWarp = kWeightWarp + 1, kMmaWarp = kWeightWarp + 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
@@ -152,22 +182,23 @@ __global__ void __launch_bounds__(threads_of(NH), 1) int4_tc_kernel(const __grid
     auto xempty = [&](int s) { return bars + 8u * (2 * kMaxW + kMaxX + s); };
     auto afull = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + s); };
     auto aempty = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + kMaxA + s); };
-    auto dfull = [&](int h, int b) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * b + h); };
-    auto dempty = [&](int h, int b) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * kMaxBuf + 2 * b + h); };
-    auto sfull = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + s); };
-    auto sempty = [&](int s) { return bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + kSSlots + s); };
-    const uint32_t done = bars + 8u * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + 2 * kSSlots);
+    constexpr int kDBar = 2 * kMaxW + 2 * kMaxX + 2 * kMaxA, kSBar = kDBar + 2 * kMaxBuf * kMaxPieces;
+    auto dfull = [&](int piece, int b) { return bars + 8u * (kDBar + kMaxPieces * b + piece); };
+    auto dempty = [&](int piece, int b) { return bars + 8u * (kDBar + kMaxPieces * (kMaxBuf + b) + piece); };
+    auto sfull = [&](int s) { return bars + 8u * (kSBar + s); };
+    auto sempty = [&](int s) { return bars + 8u * (kSBar + kSSlots + s); };
+    const uint32_t done = bars + 8u * (kSBar + 2 * kSSlots);
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const WaitCtl wc{&g_int4_error, &g_int4_failed_seq, p.wait_ns, p.seq};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < SW; ++s) { mbar_init(wfull(s), 1); mbar_init(wempty(s), kGroupWarps); }
-        for (int s = 0; s < SX; ++s) { mbar_init(xfull(s), 1); mbar_init(xempty(s), 2); }
-        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kGroupWarps); mbar_init(aempty(s), 2); }
+        for (int s = 0; s < SX; ++s) { mbar_init(xfull(s), 1); mbar_init(xempty(s), PIECES == 1 ? 1 : 2); }
+        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kGroupWarps); mbar_init(aempty(s), PIECES == 1 ? 1 : 2); }
         for (int b = 0; b < NB; ++b)
-            for (int h = 0; h < 2; ++h) { mbar_init(dfull(h, b), 1); mbar_init(dempty(h, b), 4); }
-        for (int s = 0; s < kSSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), kPromoteWarps); }
+            for (int i = 0; i < kMaxPieces; ++i) { mbar_init(dfull(i, b), 1); mbar_init(dempty(i, b), 4); }
+        for (int s = 0; s < kSSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), PIECES == 1 ? 4 : kPromoteWarps); }
         mbar_init(done, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -191,8 +222,8 @@ __global__ void __launch_bounds__(threads_of(NH), 1) int4_tc_kernel(const __grid
     const int64_t u0 = run_begin(units_all, p.units, blockIdx.x, p.ctas, split);
     const int64_t u1 = run_begin(units_all, p.units, blockIdx.x + 1, p.ctas, split);
     const int subs = 128 >> p.group_shift;               // groups a unit
-    // TMEM column of buffer b of half h: the same for every tile, so that one half may run ahead into the next tile
-    auto d_col = [&](int h, int b) { return (uint32_t)(b * p.n_max + h * n_first(p.n_max)); };
+    // TMEM column of buffer b of a piece: the same for every tile, so that one piece may run ahead into the next tile
+    auto d_col = [&](int piece, int b) { return (uint32_t)(b * p.n_max + piece_begin<PIECES>(p.n_max, piece)); };
 
     if (warp >= kWeightWarp) {
         if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
@@ -252,39 +283,73 @@ __global__ void __launch_bounds__(threads_of(NH), 1) int4_tc_kernel(const __grid
         } else {
             const int h = warp - kMmaWarp;
             if (elect_one()) {
+                // a single piece's units alternate between the two warps, which then skip every other slot and buffer
+                constexpr int kStride = PIECES == 1 ? 2 : 1;
                 int sa = 0, sx = 0, sb = 0, jobs = 0;
                 uint32_t pha = 0, phx = 0, phb = 0;
                 bool ok = true;
-                const int steps = 8 / subs;              // K = 16 products a group
+                const uint64_t x_desc = sw128_desc(x_ring);
+                const uint32_t d0 = tmem + d_col(PIECES == 1 ? 0 : h, 0), d1 = tmem + d_col(h + 2, 0);
+                // one unit: SUBS groups of 8 / SUBS products of K = 16 for each of this warp's pieces
+                auto unit = [&](auto subs_, uint32_t id0, uint32_t id1, uint32_t row0, uint32_t row1) {
+                    constexpr int SUBS = decltype(subs_)::value, STEPS = 8 / SUBS;
+                    const uint32_t a = tmem + (uint32_t)(p.a_col0 + sa * kACols);
+                    const uint64_t b0 = x_desc + (uint64_t)((uint32_t)(sx * x_bytes) >> 4);
+                    const uint64_t b1 = b0 + (uint64_t)(sub_bytes >> 4);
+                    const int first = PIECES == 1 ? 0 : h;
+#pragma unroll
+                    for (int s = 0; s < SUBS; ++s) {
+                        if (s == 0) {
+                            if (!(ok = wait_three(afull(sa), pha, xfull(sx), phx, dempty(first, sb), phb ^ 1u, jobs >= NB, 5, wc))) return;
+                        } else {
+                            if (jobs >= NB && !(ok = wait_one(dempty(first, sb), phb ^ 1u, 7, wc))) return;
+                        }
+                        tc_fence_after();
+                        auto piece = [&](uint32_t d, uint32_t row, uint32_t id) {
+                            if (id == 0) return;
+#pragma unroll
+                            for (int k = 0; k < STEPS; ++k) {
+                                const int kk = s * STEPS + k;
+                                umma_f16_ts(d, a + 8u * kk, (kk < 4 ? b0 : b1) + row + 2 * (kk & 3), id, k ? 1u : 0u);
+                            }
+                        };
+                        piece(d0 + sb * p.n_max, row0, id0);
+                        umma_commit(dfull(first, sb));
+                        if constexpr (PIECES == 4) {
+                            if (jobs >= NB && !(ok = wait_one(dempty(h + 2, sb), phb ^ 1u, 7, wc))) return;
+                            tc_fence_after();
+                            piece(d1 + sb * p.n_max, row1, id1);
+                            umma_commit(dfull(h + 2, sb));
+                        }
+                        ++jobs;
+                        advance(sb, phb, 1, NB);
+                    }
+                };
+                auto skip = [&] {                        // the other warp's unit
+                    advance(sa, pha, 1, SA);
+                    advance(sx, phx, 1, SX);
+                    for (int s = 0; s < subs; ++s) advance(sb, phb, 1, NB);
+                    jobs += subs;
+                };
+                if (PIECES == 1 && h) skip();
                 for (int64_t u = u0; u < u1 && ok;) {
                     const Tile t = tile_at(p, u, u1);
-                    const int n0 = n_first(t.n), n = h ? n_total(t.n) - n0 : n0;
-                    const uint32_t id = idesc_f16<T>(n ? n : 16);
-                    for (int k = t.k0; k < t.k1 && ok; ++k) {
-                        if (!(ok = wait_one(afull(sa), pha, 5, wc))) break;
-                        if (!(ok = wait_one(xfull(sx), phx, 6, wc))) break;
-                        tc_fence_after();
-                        const uint32_t a = tmem + (uint32_t)(p.a_col0 + sa * kACols);
-                        const uint64_t b0 = sw128_desc(x_ring + sx * x_bytes) + (uint64_t)((h * n0 * 128) >> 4);
-                        const uint64_t b1 = b0 + (uint64_t)(sub_bytes >> 4);
-                        for (int s = 0; s < subs; ++s) {
-                            if (jobs >= NB && !(ok = wait_one(dempty(h, sb), phb ^ 1u, 7, wc))) break;
-                            tc_fence_after();
-                            if (n) {
-                                const uint32_t d = tmem + d_col(h, sb);
-                                for (int i = 0; i < steps; ++i) {
-                                    const int kk = s * steps + i;
-                                    umma_f16_ts(d, a + 8u * kk, (kk < 4 ? b0 : b1) + 2 * (kk & 3), id, i ? 1u : 0u);
-                                }
-                            }
-                            umma_commit(dfull(h, sb));
-                            ++jobs;
-                            advance(sb, phb, 1, NB);
-                        }
+                    const int n0 = piece_size<PIECES>(t.n, PIECES == 1 ? 0 : h), n1 = PIECES == 4 ? piece_size<PIECES>(t.n, h + 2) : 0;
+                    const uint32_t id0 = n0 > 0 ? idesc_f16<T>(n0) : 0u, id1 = n1 > 0 ? idesc_f16<T>(n1) : 0u;
+                    const uint32_t row0 = (uint32_t)(piece_begin<PIECES>(t.n, PIECES == 1 ? 0 : h) * 128) >> 4;
+                    const uint32_t row1 = (uint32_t)(piece_begin<PIECES>(t.n, h + 2) * 128) >> 4;
+                    int k = t.k0;
+                    if (PIECES == 1) k += (int)((u - u0 + h) & 1);
+                    for (; k < t.k1; k += kStride) {
+                        if (subs == 1) unit(std::integral_constant<int, 1>(), id0, id1, row0, row1);
+                        else if (subs == 2) unit(std::integral_constant<int, 2>(), id0, id1, row0, row1);
+                        else unit(std::integral_constant<int, 4>(), id0, id1, row0, row1);
+                        if (!ok) break;
                         umma_commit(aempty(sa));
                         umma_commit(xempty(sx));
                         advance(sa, pha, 1, SA);
                         advance(sx, phx, 1, SX);
+                        if (PIECES == 1) skip();
                     }
                     u += t.k1 - t.k0;
                 }
@@ -351,83 +416,90 @@ __global__ void __launch_bounds__(threads_of(NH), 1) int4_tc_kernel(const __grid
         const int h = warp >> 2, q = warp & 3, row_in = 32 * q + lane;
         T* y = reinterpret_cast<T*>(p.y);
         const uint32_t scale_at = (uint32_t)(((row_in >> 4) * 8 + (row_in & 7)) * 2 + ((row_in >> 3) & 1)) * 2u;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+        const uint32_t d_at[2] = {lanes + d_col(h, 0), lanes + d_col(h + 2, 0)};
         int sb = 0, ss = 0;
         uint32_t phb = 0, phs = 0;
         bool ok = true;
-        for (int64_t u = u0; u < u1 && ok;) {
+        for (int64_t u = u0; u < u1 && ok && h < PIECES;) {
             const Tile t = tile_at(p, u, u1);
-            const int n0 = n_first(t.n), nh = h ? n_total(t.n) - n0 : n0;
-            uint64_t acc[NH / 2];
+            const int size[2] = {piece_size<PIECES>(t.n, h), W1 ? piece_size<PIECES>(t.n, h + 2) : 0};
+            uint64_t acc[(W0 + W1) / 2];
 #pragma unroll
-            for (int i = 0; i < NH / 2; ++i) acc[i] = 0;
+            for (int i = 0; i < (W0 + W1) / 2; ++i) acc[i] = 0;
             for (int k = t.k0; k < t.k1 && ok; ++k) {
                 if (!(ok = wait_all(sfull(ss), phs, 13, wc))) break;
 #pragma unroll 1
                 for (int sub = 0; sub < subs; ++sub) {
-                const uint16_t sb16 = (uint16_t)lds_u16(s_ring + ss * kSSlotBytes + sub * 256 + scale_at);
-                if (sub == subs - 1) {                   // the unit's scales are read
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sempty(ss));
-                    advance(ss, phs, 1, kSSlots);
-                }
-                const float s = to_f32(*reinterpret_cast<const T*>(&sb16));
-                uint64_t s2;
-                asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(s)));
-                if (!(ok = wait_all(dfull(h, sb), phb, 11, wc))) break;
-                tc_fence_after();
-                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + d_col(h, sb);
-                // 16 columns at a time, the next ones on their way meanwhile where there are more than two
-                constexpr int kBufs = NH > 32 ? 2 : 1;
-                uint32_t v[kBufs][16];
-                if (kBufs == 2 && nh > 0) ld16_async(d, v[0]);
+                    const uint16_t bits = (uint16_t)lds_u16(s_ring + ss * kSSlotBytes + sub * 256 + scale_at);
+                    uint64_t s2;
+                    asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(to_f32(*reinterpret_cast<const T*>(&bits)))));
+                    auto promote = [&](auto which) {
+                        constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0;
+                        const int piece = h + 2 * I;
+                        if (!ok || !(ok = wait_all(dfull(piece, sb), phb, 11, wc))) return;
+                        tc_fence_after();
+                        const uint32_t d = d_at[I] + sb * p.n_max;
 #pragma unroll
-                for (int c = 0; c < NH / 16; ++c) {
-                    if (c * 16 < nh) {
-                        if (kBufs == 1) ld16_async(d + c * 16, v[0]);
-                        ld16_wait(v[c % kBufs]);
-                        if (kBufs == 2 && (c + 1) * 16 < nh) ld16_async(d + (c + 1) * 16, v[(c + 1) % kBufs]);
+                        for (int c = 0; c < kWidth / 16; ++c) {
+                            if (c * 16 < size[I]) {
+                                uint32_t v[16];
+                                ld16_async(d + c * 16, v);
+                                ld16_wait(v);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], s2, v[c % kBufs][2 * i], v[c % kBufs][2 * i + 1]);
-                    }
+                                for (int e = 0; e < 8; ++e) fma2(acc[I * W0 / 2 + c * 8 + e], s2, v[2 * e], v[2 * e + 1]);
+                            }
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(dempty(piece, sb));
+                    };
+                    promote(std::integral_constant<int, 0>());
+                    if constexpr (W1 > 0) promote(std::integral_constant<int, 1>());
+                    if (!ok) break;
+                    advance(sb, phb, 1, NB);
                 }
-                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(dempty(h, sb));
-                advance(sb, phb, 1, NB);
-                }
+                if (lane == 0) mbar_arrive(sempty(ss));
+                advance(ss, phs, 1, kSSlots);
             }
             if (!ok) break;
-            const int left = min(nh, t.n - h * n0);      // this half's tokens
-            if (t.k1 - t.k0 < p.units) {                 // shared with the neighbouring run
-                float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 +
-                              (int64_t)h * n0 * 128 + row_in;
+            auto store = [&](auto which) {
+                constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0, kAt = I * W0 / 2;
+                const int col0 = piece_begin<PIECES>(t.n, h + 2 * I);
+                const int left = min(size[I], t.n - col0);                               // this piece's tokens
+                if (t.k1 - t.k0 < p.units) {             // shared with the neighbouring run
+                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 +
+                                  (int64_t)col0 * 128 + row_in;
 #pragma unroll
-                for (int c = 0; c < NH; ++c)
-                    if (c < left) part[c * 128] = half_of(acc[c / 2], c & 1);
-            } else if (p.gated) {
-                // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each pair of
-                // lanes exchanges one of two columns and finishes the other.
-                const int64_t row = (int64_t)t.rt * 64 + 16 * q + (lane & 15);
+                    for (int c = 0; c < kWidth; ++c)
+                        if (c < left) part[c * 128] = half_of(acc[kAt + c / 2], c & 1);
+                } else if (p.gated) {
+                    // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each pair
+                    // of lanes exchanges one of two columns and finishes the other.
+                    const int row = t.rt * 64 + 16 * q + (lane & 15);
+                    T* out = y + (int64_t)(t.first + col0 + (lane >> 4)) * p.ldy + row;
 #pragma unroll
-                for (int c = 0; c < NH; c += 2) {
-                    if (c >= left) continue;
-                    const float mine = half_of(acc[c / 2], lane >> 4), send = half_of(acc[c / 2], (lane >> 4) ^ 1);
-                    const float other = __shfl_xor_sync(0xffffffffu, send, 16);
-                    const float gate = lane < 16 ? mine : other, up = lane < 16 ? other : mine;
-                    const int col = c + (lane >> 4);
-                    if (col < left && row < p.out_rows)
-                        y[(int64_t)(t.first + h * n0 + col) * p.ldy + row] =
-                            from_f32<T>(gate / (1.f + expf(-gate)) * up);
+                    for (int c = 0; c < kWidth; c += 2) {
+                        if (c >= left) continue;
+                        const float even = half_of(acc[kAt + c / 2], 0), odd = half_of(acc[kAt + c / 2], 1);
+                        const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? odd : even, 16);
+                        const float gate = lane < 16 ? even : other, up = lane < 16 ? other : odd;
+                        if (c + (lane >> 4) < left && row < p.out_rows)
+                            out[c * p.ldy] = from_f32<T>(gate / (1.f + expf(-gate)) * up);
+                    }
+                } else {
+                    const int row = t.rt * 128 + row_in;
+                    if (row < p.out_rows) {
+                        T* out = y + (int64_t)(t.first + col0) * p.ldy + row;
+#pragma unroll
+                        for (int c = 0; c < kWidth; ++c)
+                            if (c < left) out[c * p.ldy] = from_f32<T>(half_of(acc[kAt + c / 2], c & 1));
+                    }
                 }
-            } else {
-                const int64_t row = (int64_t)t.rt * 128 + row_in;
-                if (row < p.out_rows) {
-                    T* out = y + (int64_t)(t.first + h * n0) * p.ldy + row;
-#pragma unroll
-                    for (int c = 0; c < NH; ++c)
-                        if (c < left) out[c * p.ldy] = from_f32<T>(half_of(acc[c / 2], c & 1));
-                }
-            }
+            };
+            store(std::integral_constant<int, 0>());
+            if constexpr (W1 > 0) store(std::integral_constant<int, 1>());
             u += t.k1 - t.k0;
         }
         if (p.routed) {                                  // what lies behind the last pair
@@ -493,25 +565,23 @@ unsigned next_seq() {
 
 // What a launch of at most `most` tokens a tile takes: accumulator columns, rings.
 struct TcPlan {
-    int nh, n_max, x_rows, box_rows, bufs, a_col0, a_slots, x_slots, w_slots, smem;
+    int n_max, x_rows, box_rows, bufs, a_col0, a_slots, x_slots, w_slots, smem;
 };
-
-int bucket(int n_half) { return n_half <= 16 ? 16 : n_half <= 32 ? 32 : n_half <= 64 ? 64 : n_half <= 96 ? 96 : 144; }
 
 TcPlan plan_tc(int most, bool routed) {
     TcPlan pl;
-    const int total = (most + 15) / 16 * 16, half = (total / 2 + 15) / 16 * 16;
-    pl.nh = bucket(half);
+    const int total = n_total(most);
     pl.n_max = total;
     pl.x_rows = total;
     // a routed item's x rows end anywhere: boxes of 16 rows follow it; a dense tile is one box, or two above 256 rows
     pl.box_rows = routed ? 16 : total <= 256 ? total : total / 2;
-    pl.bufs = 2 * total + 2 * kACols <= kTmemCols ? 2 : 1;
+    pl.bufs = kMaxBuf;                                   // accumulators in turn, as far as two A tiles leave room
+    while (pl.bufs > 1 && pl.bufs * total + (pl.bufs > 2 ? 4 : 2) * kACols > kTmemCols) --pl.bufs;
     pl.a_col0 = (pl.bufs * total + 31) / 32 * 32;
     pl.a_slots = (kTmemCols - pl.a_col0) / kACols;
     if (pl.a_slots > kMaxA) pl.a_slots = kMaxA;
     const int x_bytes = 2 * pl.x_rows * 128;
-    const int fixed = 1024 + kSSlots * kSSlotBytes + 8 * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 4 * kMaxBuf + 2 * kSSlots + 1);
+    const int fixed = 1024 + kSSlots * kSSlotBytes + 8 * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * kMaxBuf * kMaxPieces + 2 * kSSlots + 1);
     // eight units of weights in flight at least, then x, then as much again as is left for weights
     pl.x_slots = (kSmemLimit - fixed - 8 * kWSlotBytes) / x_bytes;
     if (pl.x_slots > kMaxX) pl.x_slots = kMaxX;
@@ -521,10 +591,11 @@ TcPlan plan_tc(int most, bool routed) {
     return pl;
 }
 
-template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
-    auto kernel = int4_tc_kernel<T, NH>;
+template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
+    auto kernel = int4_tc_kernel<T, PIECES, W0, W1>;
+    constexpr int kThreads = threads_of(W0 + W1);
     if (int e = allow_smem((const void*)kernel, smem, what)) return e;
-    if (NH >= 64) {                                      // the register split needs what it was written for
+    if (W0 + W1 >= 64) {                                      // the register split needs what it was written for
         static std::atomic<int> regs{0};
         if (regs == 0) {
             cudaFuncAttributes a;
@@ -532,7 +603,7 @@ template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcPara
                 return fail(P2P_ECUDA, "%s: %s", what, cudaGetErrorString(cudaGetLastError()));
             regs = a.numRegs;
         }
-        if (regs * threads_of(NH) < 256 * 176 + 256 * 48 + 128 * 32)
+        if (regs * kThreads < 256 * 176 + 256 * 48 + 128 * 32)
             return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread, 96 needed", what, regs.load());
     }
     cudaLaunchConfig_t cfg = {};
@@ -540,7 +611,7 @@ template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcPara
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(threads_of(NH));
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
@@ -555,14 +626,12 @@ template <typename T, int NH> int launch_tc(const CUtensorMap& map, const TcPara
     return launch_status(what);
 }
 
-template <typename T> int launch_nh(int nh, const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
-    switch (nh) {
-        case 16: return launch_tc<T, 16>(map, p, smem, st, what);
-        case 32: return launch_tc<T, 32>(map, p, smem, st, what);
-        case 64: return launch_tc<T, 64>(map, p, smem, st, what);
-        case 96: return launch_tc<T, 96>(map, p, smem, st, what);
-        default: return launch_tc<T, 144>(map, p, smem, st, what);
-    }
+template <typename T> int launch_width(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
+    if (p.n_max <= 32) return launch_tc<T, 1, 32, 0>(map, p, smem, st, what);
+    if (p.n_max <= 64) return launch_tc<T, 2, 32, 0>(map, p, smem, st, what);
+    if (p.n_max <= 128) return launch_tc<T, 2, 64, 0>(map, p, smem, st, what);
+    if (p.n_max <= 192) return launch_tc<T, 4, 48, 48>(map, p, smem, st, what);
+    return launch_tc<T, 4, 80, 64>(map, p, smem, st, what);
 }
 
 // Token tiles of a dense call: as even as they divide, at most 272 tokens each.
@@ -632,8 +701,8 @@ int int4_tc_run(const Int4Call& c, void* workspace, cudaStream_t st, const char*
     p.seq = next_seq();
     CUtensorMap map;
     if (int e = encode_x_map(&map, c.x, c.dtype, routed ? c.pairs : c.tokens, c.cols, c.ldx, pl.box_rows)) return e;
-    return c.dtype == P2P_BF16 ? launch_nh<__nv_bfloat16>(pl.nh, map, p, pl.smem, st, what)
-                               : launch_nh<__half>(pl.nh, map, p, pl.smem, st, what);
+    return c.dtype == P2P_BF16 ? launch_width<__nv_bfloat16>(map, p, pl.smem, st, what)
+                               : launch_width<__half>(map, p, pl.smem, st, what);
 }
 
 int int4_tc_error(int* site, int reset, cudaStream_t st) {
