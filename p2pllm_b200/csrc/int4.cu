@@ -163,7 +163,8 @@ struct SmallParams {
     int tokens, n_max, out_rows;        // n_max: tokens of a tile, at most
     int splits;                         // > 0: CTAs of a cluster, each with its share of one row tile; 0: runs
     float* partial;                     // runs: [ctas][2][n_max][128], the row tiles a run shares with its neighbours
-    int slots, slot_bytes, x_at, x_sub; // ring: record, then two x boxes of x_sub bytes at x_at
+    int slots, half_bytes, x_at, x_sub; // ring: slots of two units (a tile's last may hold one), half_bytes each: record,
+                                        // then two x boxes of x_sub bytes at x_at
     void* y;
     int64_t ldy;
     const int32_t* items;               // routed: {expert, first place, places, 0}
@@ -176,31 +177,19 @@ struct SmallParams {
     unsigned seq;
 };
 
-// c += a b, or with Zero c = a b.
-template <bool Zero, typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-    const float z = 0.f;
-    if constexpr (bf && Zero)
+// d = a b + c: c is four registers of their own, so that a zero one costs nothing.
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint2 b, const float (&c)[4]) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                     "{%10, %10, %10, %10};"
-                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(z));
-    else if constexpr (bf)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                     "{%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
-    else if constexpr (Zero)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                     "{%10, %10, %10, %10};"
-                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(z));
+            "{%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                     "{%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+            "{%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 // A value at byte `at` of shared memory: plain loads, which the compiler may move about between two barriers.
 template <typename V> __device__ __forceinline__ V lds(const uint8_t* smem, uint32_t at) {
@@ -259,7 +248,7 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
                                                                       const __grid_constant__ SmallParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    float* red = reinterpret_cast<float*>(smem_raw + (base - raw) + p.slots * p.slot_bytes);   // [8 NT][kRowPad]
+    float* red = reinterpret_cast<float*>(smem_raw + (base - raw) + p.slots * 2 * p.half_bytes);   // [8 NT][kRowPad]
     const uint32_t bars = smem_u32(red) + NT * 8 * kRowPad * 4;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (kMaxSlots + s); };
@@ -299,34 +288,44 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
             const int n_slots = p.slots;
             const uint32_t w_bytes = (uint32_t)p.record;
             bool ok = true;
-            auto load_w = [&](int slot, const SmallTile& t, int k) {
+            // Units k and, if there is one, k + 1 of a tile into slot `slot`.
+            auto load_w = [&](int slot, const SmallTile& t, int k, int n) {
                 const uint32_t x_rows = p.order ? (uint32_t)t.n : (uint32_t)(NT * 8);
-                mbar_expect_tx(full(slot), w_bytes + 2u * 128u * x_rows);
-                bulk_load(base + slot * p.slot_bytes, t.records + (int64_t)k * p.record, w_bytes, full(slot));
+                mbar_expect_tx(full(slot), n * (w_bytes + 2u * 128u * x_rows));
+                for (int i = 0; i < n; ++i)
+                    bulk_load(base + (2 * slot + i) * p.half_bytes, t.records + (int64_t)(k + i) * p.record, w_bytes, full(slot));
             };
-            auto load_x = [&](int slot, const SmallTile& t, int k) {
-                const uint32_t at = base + slot * p.slot_bytes + p.x_at;
-                if (p.order) {                                       // a row at a time, from wherever its token lies
-                    for (int i = 0; i < t.n; ++i) {
-                        const int row = __ldcg(p.order + t.first + i) / p.topk;
-                        tma_load_2d(at + i * 128, &tmap_x, k * 128, row, full(slot));
-                        tma_load_2d(at + p.x_sub + i * 128, &tmap_x, k * 128 + 64, row, full(slot));
+            auto load_x = [&](int slot, const SmallTile& t, int k, int n) {
+                for (int h = 0; h < n; ++h) {
+                    const uint32_t at = base + (2 * slot + h) * p.half_bytes + p.x_at;
+                    if (p.order) {                                   // a row at a time, from wherever its token lies
+                        for (int i = 0; i < t.n; ++i) {
+                            const int row = __ldcg(p.order + t.first + i) / p.topk;
+                            tma_load_2d(at + i * 128, &tmap_x, (k + h) * 128, row, full(slot));
+                            tma_load_2d(at + p.x_sub + i * 128, &tmap_x, (k + h) * 128 + 64, row, full(slot));
+                        }
+                    } else {
+                        tma_load_2d(at, &tmap_x, (k + h) * 128, t.first, full(slot));
+                        tma_load_2d(at + p.x_sub, &tmap_x, (k + h) * 128 + 64, t.first, full(slot));
                     }
-                } else {
-                    tma_load_2d(at, &tmap_x, k * 128, t.first, full(slot));
-                    tma_load_2d(at + p.x_sub, &tmap_x, k * 128 + 64, t.first, full(slot));
                 }
             };
             int slot = 0, used = 0;
             uint32_t ph = 0;
+            int64_t u = u0;
             if (!p.items) {
                 // the ring's first fill: weights, then, once the previous kernel has ended, x
                 for (int pass = 0; pass < 2; ++pass) {
                     int i = 0;
-                    for (int64_t u = u0; u < u1 && i < n_slots;) {
+                    for (u = u0; u < u1 && i < n_slots;) {
                         const SmallTile t = small_tile(p, u / p.units);
-                        for (int k = (int)(u % p.units); k < p.units && u < u1 && i < n_slots; ++k, ++u, ++i)
-                            if (pass == 0) load_w(i, t, k); else load_x(i, t, k);
+                        const int kz = (int)min((int64_t)p.units, u % p.units + (u1 - u));
+                        for (int k = (int)(u % p.units); k < kz && i < n_slots; ++i) {
+                            const int n = min(2, kz - k);
+                            if (pass == 0) load_w(i, t, k, n); else load_x(i, t, k, n);
+                            k += n;
+                            u += n;
+                        }
                     }
                     used = i;
                     if (pass == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -334,12 +333,16 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
                 slot = used == n_slots ? 0 : used;
                 ph = used == n_slots ? 1u : 0u;
             }
-            for (int64_t u = u0 + used; u < u1 && ok;) {
+            while (u < u1 && ok) {
                 const SmallTile t = small_tile(p, u / p.units);
-                for (int k = (int)(u % p.units); k < p.units && u < u1; ++k, ++u) {
+                const int kz = (int)min((int64_t)p.units, u % p.units + (u1 - u));
+                for (int k = (int)(u % p.units); k < kz;) {
                     if (used >= n_slots && !(ok = wait_one(empty(slot), ph ^ 1u, 1, wc))) break;
-                    load_w(slot, t, k);
-                    load_x(slot, t, k);
+                    const int n = min(2, kz - k);
+                    load_w(slot, t, k, n);
+                    load_x(slot, t, k, n);
+                    k += n;
+                    u += n;
                     ++used;
                     advance(slot, ph, 1, n_slots);
                 }
@@ -370,6 +373,9 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
         q4::Codes<T> codes[2];
         codes[0].zeros(8u, 8u);
         codes[1].zeros(8u, 8u);
+        float zero[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero[i] = __uint_as_float(q4::opaque(0u));
         for (int64_t u = u0; u < u1;) {
             const SmallTile t = small_tile(p, u / p.units);
             const int ka = (int)(u % p.units), kz = (int)min((int64_t)p.units, ka + (u1 - u));
@@ -380,10 +386,13 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
                 for (int c = 0; c < NT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[b][c][i] = 0.f;
-            for (int k = ka; k < kz; ++k) {
+            for (int k = ka; k < kz; k += 2) {
                 // a warp that gave up multiplies nothing more, but keeps meeting the others at every row tile's end
                 if (!ok || !(ok = __all_sync(0xffffffffu, wait_one(full(slot), ph, 3, wc)))) break;
                 const uint8_t* at = ring + rec;
+                const int n_units = min(2, kz - k);
+#pragma unroll 1
+                for (int unit = 0; unit < n_units; ++unit, at += p.half_bytes) {
                 uint32_t w[2][4];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -427,16 +436,16 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
                         codes[b].expand(w[b][r], a);
 #pragma unroll
                         for (int c = 0; c < NT; ++c) {
-                            if (r == 0 || (G32 && r == 2)) mma16816<true, T>(part[b][c], a, xf[c]);
-                            else mma16816<false, T>(part[b][c], a, xf[c]);
+                            mma16816<T>(part[b][c], a, xf[c], r == 0 || (G32 && r == 2) ? zero : part[b][c]);
                         }
                     }
                 }
                 end(0, G32 ? 1 : 0);
                 end(1, G32 ? 1 : 0);
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty(slot));
-                rec += (uint32_t)p.slot_bytes;
+                rec += 2u * (uint32_t)p.half_bytes;
                 if (++slot == p.slots) {
                     slot = 0;
                     ph ^= 1u;
@@ -574,7 +583,7 @@ unsigned next_seq() {
 // How a call of up to 32 tokens a tile is cut: shares of a cluster's CTAs where they are all resident at once, else
 // runs, two CTAs an SM.
 struct SmallPlan {
-    int nt, splits, ctas, slots, slot_bytes, x_at, x_sub, smem;
+    int nt, splits, ctas, slots, half_bytes, x_at, x_sub, smem;
     int64_t col_tiles, tiles;
     size_t workspace;
 };
@@ -603,11 +612,11 @@ SmallPlan plan_small(const Int4Call& c) {
     const int record = q4::unit_bytes(c.group, c.has_zeros);
     pl.x_at = (int)q4::div_up(record, 1024) * 1024;
     pl.x_sub = pl.nt * 8 * 128;
-    pl.slot_bytes = pl.x_at + 2 * pl.x_sub;
+    pl.half_bytes = pl.x_at + 2 * pl.x_sub;
     const int fixed = 1024 + pl.nt * 8 * kRowPad * 4 + 8 * 2 * kMaxSlots;
-    pl.slots = (int)((226 * 1024 / per_sm - 1024 - fixed) / pl.slot_bytes);
+    pl.slots = (int)((226 * 1024 / per_sm - 1024 - fixed) / (2 * pl.half_bytes));
     if (pl.slots > kMaxSlots) pl.slots = kMaxSlots;
-    pl.smem = fixed + pl.slots * pl.slot_bytes;
+    pl.smem = fixed + pl.slots * 2 * pl.half_bytes;
     return pl;
 }
 
@@ -659,7 +668,7 @@ int run_small(const Int4Call& c, const int32_t* order, int topk, void* workspace
     p.splits = pl.splits;
     p.partial = reinterpret_cast<float*>(workspace);
     p.slots = pl.slots;
-    p.slot_bytes = pl.slot_bytes;
+    p.half_bytes = pl.half_bytes;
     p.x_at = pl.x_at;
     p.x_sub = pl.x_sub;
     p.y = c.y;
