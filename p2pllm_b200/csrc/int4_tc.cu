@@ -36,10 +36,19 @@ using namespace sm100;
 
 constexpr int kPromoteWarps = 8;
 constexpr int kBuildWarp = kPromoteWarps;               // 8..
-constexpr int kGroupWarps = 8;                          // warps that build one unit
-// Up to 64 tokens the codes' turn binds: two groups of builders take alternate units.
+// Warps that build one unit, and groups of them taking alternate units: up to 64 tokens the codes' turn binds; above 128
+// the promoting warps' accumulators leave registers for four builders only.
+constexpr int group_warps(int acc) { return acc >= 96 ? 4 : 8; }
 constexpr int build_groups(int acc) { return acc <= 32 ? 2 : 1; }
-constexpr int threads_of(int acc) { return (kPromoteWarps + build_groups(acc) * kGroupWarps + 4) * 32; }
+constexpr int threads_of(int acc) { return (kPromoteWarps + build_groups(acc) * group_warps(acc) + 4) * 32; }
+// Registers a thread of promoting, building and other warps: what the launch gives (a whole register file over the
+// threads, in eights), dealt anew. 0: as launched.
+constexpr int promote_regs(int acc) { return acc >= 96 ? 200 : acc >= 64 ? 128 : 0; }
+constexpr int build_regs(int acc) { return acc >= 96 ? 64 : 72; }
+constexpr int other_regs(int acc) { return acc >= 96 ? 40 : 48; }
+constexpr int dealt_regs(int acc) {
+    return kPromoteWarps * 32 * promote_regs(acc) + build_groups(acc) * group_warps(acc) * 32 * build_regs(acc) + 128 * other_regs(acc);
+}
 constexpr int kWSlotBytes = q4::kCodeBytes + 512;       // codes and up to four groups' zero points
 constexpr int kSSlotBytes = 1024;                       // up to four groups' scales
 constexpr int kACols = 64;                              // TMEM columns of one unit's A tile
@@ -123,21 +132,21 @@ struct Tile {
     int k0, k1;                         // steps [k0, k1) of p.units
 };
 
-__device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t u, int64_t u1) {
+__device__ __forceinline__ Tile tile_at(const TcParams& p, int u, int u1) {
     Tile t;
-    const int64_t id = u / p.units;
-    t.k0 = (int)(u - id * p.units);
-    t.k1 = (int)min((int64_t)p.units, t.k0 + (u1 - u));
+    const int id = u / p.units;
+    t.k0 = u - id * p.units;
+    t.k1 = min(p.units, t.k0 + (u1 - u));
     if (p.items) {
-        const int item = (int)(id / p.row_tiles);
-        t.rt = (int)(id - (int64_t)item * p.row_tiles);
+        const int item = id / p.row_tiles;
+        t.rt = id - item * p.row_tiles;
         const int4 it = __ldcg(reinterpret_cast<const int4*>(p.items) + item);
         t.records = p.layout + ((int64_t)it.x * p.row_tiles + t.rt) * p.units * p.record;
         t.first = it.y;
         t.n = min(it.z, p.n_max);
     } else {
-        t.rt = (int)(id / p.token_tiles);
-        t.first = (int)(id - (int64_t)t.rt * p.token_tiles) * p.tile_tokens;
+        t.rt = id / p.token_tiles;
+        t.first = (id - t.rt * p.token_tiles) * p.tile_tokens;
         t.n = min(p.tile_tokens, p.tokens - t.first);
         t.records = p.layout + (int64_t)t.rt * p.units * p.record;
     }
@@ -155,19 +164,35 @@ template <int PIECES> __device__ __forceinline__ int piece_begin(int n, int i) {
     return at;
 }
 
-__device__ __forceinline__ int64_t run_begin(int64_t units_all, int units, int64_t b, int ctas, bool split) {
-    return split ? units_all * b / ctas : units_all / units * b / ctas * units;
-}
+template <typename T> struct alignas(8) Quad { T v[4]; };
+
+// The runs: `whole` things (units, or row tiles of that many units each) dealt to the CTAs, the first `rest` of which take
+// one more. Below 2^31 units in all.
+struct Runs {
+    uint32_t whole, rest, each;
+    __device__ __forceinline__ Runs(const TcParams& p, uint32_t tiles) {
+        each = p.partial ? 1u : (uint32_t)p.units;
+        const uint32_t things = p.partial ? tiles * (uint32_t)p.units : tiles;
+        whole = things / (uint32_t)p.ctas;
+        rest = things - whole * (uint32_t)p.ctas;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t b) const { return (b * whole + min(b, rest)) * each; }
+    // The run that holds unit u, of a launch that deals units.
+    __device__ __forceinline__ uint32_t of(uint32_t u) const {
+        const uint32_t longer = rest * (whole + 1);
+        return u < longer ? u / (whole + 1) : rest + (u - longer) / whole;
+    }
+};
 
 // PIECES of the tokens; W0, W1: the most columns of a promoting warp's first and second piece, whose sums it holds in
 // registers (W1 = 0: it has one).
 template <typename T, int PIECES, int W0, int W1>
 __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                               const __grid_constant__ TcParams p) {
-    // 640 threads start with 96 registers each; the promoting warps need an accumulator of up to 144 and take what the
-    // others give back: 256 x 176 + 256 x 48 + 128 x 32 = 640 x 96.
-    constexpr bool kSplitRegs = W0 + W1 >= 64;
-    constexpr int kGroups = build_groups(W0 + W1), kWeightWarp = kBuildWarp + kGroups * kGroupWarps;
+    // The promoting warps need an accumulator of up to 144 registers and take what the others give back.
+    constexpr int kAcc = W0 + W1, kGroups = build_groups(kAcc), kGroupWarps = group_warps(kAcc);
+    constexpr bool kSplitRegs = promote_regs(kAcc) > 0;
+    constexpr int kWeightWarp = kBuildWarp + kGroups * kGroupWarps;
     constexpr int kXWarp = kWeightWarp + 1, kMmaWarp = kWeightWarp + 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
@@ -216,24 +241,21 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
     // The items are the previous kernel's; dense weights wait for nobody, and everything else for that kernel's end.
     if (p.items || (warp != kWeightWarp && (warp < kBuildWarp || warp >= kWeightWarp)))
         asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t tiles = p.items ? (int64_t)*p.n_items * p.row_tiles : (int64_t)p.row_tiles * p.token_tiles;
-    const int64_t units_all = tiles * p.units;
-    const bool split = p.partial != nullptr;
-    const int64_t u0 = run_begin(units_all, p.units, blockIdx.x, p.ctas, split);
-    const int64_t u1 = run_begin(units_all, p.units, blockIdx.x + 1, p.ctas, split);
+    const Runs runs(p, (uint32_t)(p.items ? *p.n_items * p.row_tiles : p.row_tiles * p.token_tiles));
+    const int u0 = (int)runs.begin(blockIdx.x), u1 = (int)runs.begin(blockIdx.x + 1);
     const int subs = 128 >> p.group_shift;               // groups a unit
     // TMEM column of buffer b of a piece: the same for every tile, so that one piece may run ahead into the next tile
     auto d_col = [&](int piece, int b) { return (uint32_t)(b * p.n_max + piece_begin<PIECES>(p.n_max, piece)); };
 
     if (warp >= kWeightWarp) {
-        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(kAcc)));
         if (warp == kWeightWarp) {
             if (elect_one()) {
                 int slot = 0, ss = 0, used = 0;
                 uint32_t ph = 0, phs = 0;
                 bool ok = true;
                 const uint32_t w_bytes = (uint32_t)(q4::kCodeBytes + p.zero_bytes);
-                for (int64_t u = u0; u < u1 && ok;) {
+                for (int u = u0; u < u1 && ok;) {
                     const Tile t = tile_at(p, u, u1);
                     const uint8_t* src = t.records + (int64_t)t.k0 * p.record;
                     for (int k = t.k0; k < t.k1; ++k, src += p.record) {
@@ -261,7 +283,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                 int slot = 0, used = 0;
                 uint32_t ph = 0;
                 bool ok = true;
-                for (int64_t u = u0; u < u1 && ok;) {
+                for (int u = u0; u < u1 && ok;) {
                     const Tile t = tile_at(p, u, u1);
                     const int boxes = (n_total(t.n) + p.box_rows - 1) / p.box_rows;
                     for (int k = t.k0; k < t.k1; ++k) {
@@ -332,7 +354,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                     jobs += subs;
                 };
                 if (PIECES == 1 && h) skip();
-                for (int64_t u = u0; u < u1 && ok;) {
+                for (int u = u0; u < u1 && ok;) {
                     const Tile t = tile_at(p, u, u1);
                     const int n0 = piece_size<PIECES>(t.n, PIECES == 1 ? 0 : h), n1 = PIECES == 4 ? piece_size<PIECES>(t.n, h + 2) : 0;
                     const uint32_t id0 = n0 > 0 ? idesc_f16<T>(n0) : 0u, id1 = n1 > 0 ? idesc_f16<T>(n1) : 0u;
@@ -359,46 +381,43 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
             __syncwarp();
         }
     } else if (warp >= kBuildWarp) {
-        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(build_regs(kAcc)));
         const int group = (warp - kBuildWarp) / kGroupWarps, w = (warp - kBuildWarp) % kGroupWarps;
-        const int blk = 2 * (w & 3) + (w >> 2);                                 // lanes 32 (w % 4).. are this warp's
-        const uint32_t lanes = (uint32_t)(16 * blk) << 16;
+        constexpr int kBlocks = 8 / kGroupWarps;                                // row blocks a warp builds
+        const int blk0 = 2 * (w & 3) + (kBlocks == 1 ? w >> 2 : 0);             // lanes 32 (w % 4).. are this warp's
         int sw = group, sa = group, used = group;
         uint32_t phw = 0, pha = 0;
         bool ok = true;
         q4::Codes<T> codes;
         codes.zeros(8u, 8u);
-        for (int64_t u = u0 + group; u < u1 && ok; u += kGroups) {
+        for (int u = u0 + group; u < u1 && ok; u += kGroups) {
             {
                 if (!(ok = wait_all(wfull(sw), phw, 9, wc))) break;
-                const uint32_t rec = w_ring + sw * kWSlotBytes, at = rec + blk * 2 * q4::kBlockBytes + lane * 16;
-                const uint4 c[2] = {lds_v4(at), lds_v4(at + q4::kBlockBytes)};
-                uint32_t zs[4] = {0x0808u, 0x0808u, 0x0808u, 0x0808u};
-                if (p.zero_bytes) {
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        if (s < subs) zs[s] = lds_u16(rec + q4::kCodeBytes + ((s * 8 + blk) * 8 + (lane >> 2)) * 2);
-                }
+                const uint32_t rec = w_ring + sw * kWSlotBytes;
                 if (used >= SA && !(ok = wait_all(aempty(sa), pha ^ 1u, 10, wc))) break;
                 tc_fence_after();
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t words[4] = {c[half].x, c[half].y, c[half].z, c[half].w};
+                for (int i = 0; i < 2 * kBlocks; ++i) {
+                    const int blk = blk0 + i / 2, half = i & 1;
+                    const uint4 c = lds_v4(rec + (blk * 2 + half) * q4::kBlockBytes + lane * 16);
+                    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+                    // this column block's groups: one holds it, or (32 columns) two do
+                    auto zeros = [&](int g) {
+                        if (p.zero_bytes) {
+                            const uint32_t z = lds_u16(rec + q4::kCodeBytes + ((g * 8 + blk) * 8 + (lane >> 2)) * 2);
+                            codes.zeros(z & 15u, z >> 8);
+                        }
+                    };
+                    zeros(p.group_shift == 5 ? 2 * half : p.group_shift == 6 ? half : 0);
                     uint32_t r[16];
-                    // groups of 128: one zero point a unit, 64: one a half, 32: one a quarter
-                    if (p.zero_bytes) {
-                        const uint32_t z0 = p.group_shift == 5 ? zs[2 * half] : p.group_shift == 6 ? zs[half] : zs[0];
-                        codes.zeros(z0 & 15u, z0 >> 8);
-                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (i == 2 && p.zero_bytes && p.group_shift == 5)
-                            codes.zeros(zs[2 * half + 1] & 15u, zs[2 * half + 1] >> 8);
+                    for (int k = 0; k < 4; ++k) {
+                        if (k == 2 && p.group_shift == 5) zeros(2 * half + 1);
                         uint32_t a[4];
-                        codes.expand(words[i], a);
-                        r[4 * i] = a[0]; r[4 * i + 1] = a[2]; r[4 * i + 2] = a[1]; r[4 * i + 3] = a[3];
+                        codes.expand(words[k], a);
+                        r[4 * k] = a[0]; r[4 * k + 1] = a[2]; r[4 * k + 2] = a[1]; r[4 * k + 3] = a[3];
                     }
-                    tmem_st_16x256b_x4(tmem + lanes + (uint32_t)(p.a_col0 + sa * kACols + half * 32), r);
+                    tmem_st_16x256b_x4(tmem + ((uint32_t)(16 * blk) << 16) + (uint32_t)(p.a_col0 + sa * kACols + half * 32), r);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(wempty(sw));
@@ -412,7 +431,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
             }
         }
     } else {
-        if (kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        if constexpr (kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(promote_regs(kAcc)));
         const int h = warp >> 2, q = warp & 3, row_in = 32 * q + lane;
         T* y = reinterpret_cast<T*>(p.y);
         const uint32_t scale_at = (uint32_t)(((row_in >> 4) * 8 + (row_in & 7)) * 2 + ((row_in >> 3) & 1)) * 2u;
@@ -421,7 +440,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
         int sb = 0, ss = 0;
         uint32_t phb = 0, phs = 0;
         bool ok = true;
-        for (int64_t u = u0; u < u1 && ok && h < PIECES;) {
+        for (int u = u0; u < u1 && ok && h < PIECES;) {
             const Tile t = tile_at(p, u, u1);
             const int size[2] = {piece_size<PIECES>(t.n, h), W1 ? piece_size<PIECES>(t.n, h + 2) : 0};
             uint64_t acc[(W0 + W1) / 2];
@@ -515,43 +534,50 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
     }
 }
 
-// Row tiles that several runs share: their fp32 partials added in run order. A block takes one row tile and 8 tokens,
-// a thread one row.
-constexpr int kJoinTokens = 8;
-template <typename T> __global__ void __launch_bounds__(128) int4_join_kernel(const __grid_constant__ TcParams p) {
+// Row tiles that several runs share: their fp32 partials added in run order. A block takes a row tile and 32 tokens, a
+// warp a token at a time, a thread four rows.
+constexpr int kJoinTokens = 32;
+template <typename T> __global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ TcParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t tile = blockIdx.x, units_all = (int64_t)p.row_tiles * p.token_tiles * p.units;
-    const int64_t a = tile * p.units, z = a + p.units;
-    const auto begin = [&](int64_t b) { return run_begin(units_all, p.units, b, p.ctas, true); };
-    // the run that holds unit u: the last b whose begin is at most u
-    const auto run_of = [&](int64_t u) { return ((u + 1) * p.ctas + units_all - 1) / units_all - 1; };
-    const int64_t b0 = run_of(a), b1 = run_of(z - 1);
+    const Runs runs(p, (uint32_t)(p.row_tiles * p.token_tiles));
+    const uint32_t a = blockIdx.x * (uint32_t)p.units, b0 = runs.of(a), b1 = runs.of(a + p.units - 1);
     if (b0 == b1) return;                                // one run wrote y itself
-    const Tile t = tile_at(p, a, z);
-    const int row_in = threadIdx.x, lane = threadIdx.x & 31, q = threadIdx.x >> 5;
-    const int c0 = blockIdx.y * kJoinTokens;
-    float acc[kJoinTokens];
-#pragma unroll
-    for (int c = 0; c < kJoinTokens; ++c) acc[c] = 0.f;
-    for (int64_t b = b0; b <= b1; ++b) {
-        const float* part = p.partial + (b * 2 + (begin(b) >= a ? 0 : 1)) * p.n_max * 128 + row_in;
-#pragma unroll
-        for (int c = 0; c < kJoinTokens; ++c)
-            if (c0 + c < t.n) acc[c] += __ldcg(part + (int64_t)(c0 + c) * 128);
-    }
+    const Tile t = tile_at(p, (int)a, (int)a + p.units);
+    const int lane = threadIdx.x & 31, last = min(t.n, (int)(blockIdx.y + 1) * kJoinTokens);
+    // the tile is run b0's last row tile, unless b0 begins with it, and every other run's first
+    const float* part = p.partial + ((int64_t)b0 * 2 + (runs.begin(b0) >= a ? 0 : 1)) * p.n_max * 128 + lane * 4;
+    const float* next = p.partial + (int64_t)(b0 + 1) * 2 * p.n_max * 128 + lane * 4;
     T* y = reinterpret_cast<T*>(p.y);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll 2
+    for (int tok = blockIdx.y * kJoinTokens + (threadIdx.x >> 5); tok < last; tok += 8) {
+        float4 sum = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)tok * 128));
+#pragma unroll 4
+        for (uint32_t b = b0 + 1; b <= b1; ++b) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(next + ((int64_t)(b - b0 - 1) * 2 * p.n_max + tok) * 128));
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        T* out = y + (int64_t)(t.first + tok) * p.ldy;
+        const float mine[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (p.gated) {                                   // lanes 8 i .. + 3 hold gates, + 4 .. + 7 their ups
 #pragma unroll
-    for (int c = 0; c < kJoinTokens; ++c) {
-        if (c0 + c >= t.n) break;
-        T* out = y + (int64_t)(t.first + c0 + c) * p.ldy;
-        if (p.gated) {
-            const float up = __shfl_xor_sync(0xffffffffu, acc[c], 16);
-            const int64_t row = (int64_t)t.rt * 64 + 16 * q + (lane & 15);
-            if (lane < 16 && row < p.out_rows) out[row] = from_f32<T>(acc[c] / (1.f + expf(-acc[c])) * up);
+            for (int c = 0; c < 4; ++c) {
+                const float up = __shfl_xor_sync(0xffffffffu, mine[c], 4);
+                const int row = t.rt * 64 + (lane >> 3) * 16 + (lane & 3) * 4 + c;
+                if (!(lane & 4) && row < p.out_rows) out[row] = from_f32<T>(mine[c] / (1.f + expf(-mine[c])) * up);
+            }
         } else {
-            const int64_t row = (int64_t)t.rt * 128 + row_in;
-            if (row < p.out_rows) out[row] = from_f32<T>(acc[c]);
+            const int row = t.rt * 128 + lane * 4;
+            Quad<T> q;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q.v[c] = from_f32<T>(mine[c]);
+            if (row + 3 < p.out_rows && (reinterpret_cast<uintptr_t>(out + row) & 7u) == 0) {
+                *reinterpret_cast<Quad<T>*>(out + row) = q;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (row + c < p.out_rows) out[row + c] = q.v[c];
+            }
         }
     }
 }
@@ -595,7 +621,7 @@ template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMa
     auto kernel = int4_tc_kernel<T, PIECES, W0, W1>;
     constexpr int kThreads = threads_of(W0 + W1);
     if (int e = allow_smem((const void*)kernel, smem, what)) return e;
-    if (W0 + W1 >= 64) {                                      // the register split needs what it was written for
+    if (promote_regs(W0 + W1) > 0) {                     // the register split needs what it was written for
         static std::atomic<int> regs{0};
         if (regs == 0) {
             cudaFuncAttributes a;
@@ -603,8 +629,8 @@ template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMa
                 return fail(P2P_ECUDA, "%s: %s", what, cudaGetErrorString(cudaGetLastError()));
             regs = a.numRegs;
         }
-        if (regs * kThreads < 256 * 176 + 256 * 48 + 128 * 32)
-            return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread, 96 needed", what, regs.load());
+        if (regs * kThreads < dealt_regs(W0 + W1))
+            return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread for %d in all", what, regs.load(), dealt_regs(W0 + W1));
     }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -620,7 +646,7 @@ template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMa
     if (int e = launch_status(what)) return e;
     if (!p.partial) return P2P_OK;
     cfg.gridDim = dim3((unsigned)(p.row_tiles * p.token_tiles), (unsigned)((p.tile_tokens + kJoinTokens - 1) / kJoinTokens));
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cudaLaunchKernelEx(&cfg, int4_join_kernel<T>, p);
     return launch_status(what);
@@ -690,6 +716,9 @@ int int4_tc_run(const Int4Call& c, void* workspace, cudaStream_t st, const char*
         p.ctas = dense_ctas((int64_t)p.row_tiles * p.token_tiles, p.units, &split);
     }
     p.partial = split ? reinterpret_cast<float*>(workspace) : nullptr;
+    const int64_t tiles = (int64_t)p.row_tiles * (routed ? c.max_items : p.token_tiles);
+    if (tiles * p.units > 0x7fffffff || tiles > 0x7fffffff / 2)
+        return fail(P2P_EUNSUPPORTED, "%s: %lld units of 128 x 128 weights, below 2^31", what, (long long)(tiles * p.units));
     p.x_rows = pl.x_rows;
     p.box_rows = pl.box_rows;
     p.w_slots = pl.w_slots;
