@@ -208,10 +208,10 @@ struct SmallTile {
     const uint8_t* records;
     int rt, first, n;
 };
-__device__ __forceinline__ SmallTile small_tile(const SmallParams& p, int64_t id) {
+__device__ __forceinline__ SmallTile small_tile(const SmallParams& p, int id) {
     SmallTile t;
-    const int col = (int)(id / p.row_tiles);             // an item, or a tile of the tokens
-    t.rt = (int)(id - (int64_t)col * p.row_tiles);
+    const int col = id / p.row_tiles;                    // an item, or a tile of the tokens
+    t.rt = id - col * p.row_tiles;
     int64_t expert = 0;
     if (p.items) {
         const int4 it = __ldcg(reinterpret_cast<const int4*>(p.items) + col);
@@ -225,13 +225,9 @@ __device__ __forceinline__ SmallTile small_tile(const SmallParams& p, int64_t id
     t.records = p.layout + (expert * p.row_tiles + t.rt) * p.units * p.record;
     return t;
 }
-__device__ __forceinline__ int64_t small_tiles(const SmallParams& p) {
-    return (int64_t)(p.items ? *p.n_items : p.col_tiles) * p.row_tiles;
-}
-// Runs of a launch: no more than it has units (routed launches learn that here), so that none is empty; and where run b
-// begins.
-__device__ __forceinline__ int small_runs(int64_t units_all, int ctas) { return (int)min((int64_t)ctas, units_all); }
-__device__ __forceinline__ int64_t small_begin(int64_t units_all, int64_t b, int runs) { return units_all * b / runs; }
+__device__ __forceinline__ int small_tiles(const SmallParams& p) { return (p.items ? *p.n_items : p.col_tiles) * p.row_tiles; }
+// Runs of a launch: no more than it has units (routed launches learn that here), so that none is empty.
+__device__ __forceinline__ uint32_t small_runs(uint32_t units_all, uint32_t ctas) { return max(1u, min(ctas, units_all)); }
 
 // y of a finished pair of sums (gated) or sum.
 template <typename T> __device__ __forceinline__ T gate_up(float g, float u) { return from_f32<T>(g / (1.f + expf(-g)) * u); }
@@ -267,19 +263,23 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
     // The items are the previous kernel's. Dense weights wait for nobody; x (its input) and y (whose old values it may
     // still read) for that kernel's end.
     if (p.items || warp < kComputeWarps) asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t tiles = small_tiles(p), units_all = tiles * p.units;
+    const int tiles = small_tiles(p), units_all = tiles * p.units;
     const bool clustered = p.splits > 0;
-    int64_t u0, u1;
-    int rank = 0;
+    int u0 = 0, u1 = 0, rank = 0;
     if (clustered) {
-        const int64_t tile = blockIdx.x / p.splits;
-        rank = blockIdx.x - (int)tile * p.splits;
-        u0 = tile < tiles ? tile * p.units + (int64_t)p.units * rank / p.splits : 0;
-        u1 = tile < tiles ? tile * p.units + (int64_t)p.units * (rank + 1) / p.splits : 0;
+        const int tile = blockIdx.x / p.splits;
+        rank = blockIdx.x - tile * p.splits;
+        if (tile < tiles) {
+            u0 = tile * p.units + p.units * rank / p.splits;
+            u1 = tile * p.units + p.units * (rank + 1) / p.splits;
+        }
     } else {
-        const int runs = small_runs(units_all, gridDim.x);
-        u0 = blockIdx.x < runs ? small_begin(units_all, blockIdx.x, runs) : 0;
-        u1 = blockIdx.x < runs ? small_begin(units_all, blockIdx.x + 1, runs) : 0;
+        const uint32_t n = small_runs(units_all, gridDim.x);
+        const q4::Runs runs(units_all, n, 1u);
+        if (blockIdx.x < n) {
+            u0 = (int)runs.begin(blockIdx.x);
+            u1 = (int)runs.begin(blockIdx.x + 1);
+        }
     }
 
     if (warp == kComputeWarps) {
@@ -312,15 +312,15 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
             };
             int slot = 0, used = 0;
             uint32_t ph = 0;
-            int64_t u = u0;
+            int u = u0;
             if (!p.items) {
                 // the ring's first fill: weights, then, once the previous kernel has ended, x
                 for (int pass = 0; pass < 2; ++pass) {
                     int i = 0;
                     for (u = u0; u < u1 && i < n_slots;) {
                         const SmallTile t = small_tile(p, u / p.units);
-                        const int kz = (int)min((int64_t)p.units, u % p.units + (u1 - u));
-                        for (int k = (int)(u % p.units); k < kz && i < n_slots; ++i) {
+                        const int kz = min(p.units, u % p.units + (u1 - u));
+                        for (int k = u % p.units; k < kz && i < n_slots; ++i) {
                             const int n = min(2, kz - k);
                             if (pass == 0) load_w(i, t, k, n); else load_x(i, t, k, n);
                             k += n;
@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
             }
             while (u < u1 && ok) {
                 const SmallTile t = small_tile(p, u / p.units);
-                const int kz = (int)min((int64_t)p.units, u % p.units + (u1 - u));
-                for (int k = (int)(u % p.units); k < kz;) {
+                const int kz = min(p.units, u % p.units + (u1 - u));
+                for (int k = u % p.units; k < kz;) {
                     if (used >= n_slots && !(ok = wait_one(empty(slot), ph ^ 1u, 1, wc))) break;
                     const int n = min(2, kz - k);
                     load_w(slot, t, k, n);
@@ -376,9 +376,9 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
         float zero[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) zero[i] = __uint_as_float(q4::opaque(0u));
-        for (int64_t u = u0; u < u1;) {
+        for (int u = u0; u < u1;) {
             const SmallTile t = small_tile(p, u / p.units);
-            const int ka = (int)(u % p.units), kz = (int)min((int64_t)p.units, ka + (u1 - u));
+            const int ka = u % p.units, kz = min(p.units, ka + (u1 - u));
             float acc[2][NT][4];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -533,25 +533,26 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
 // a time, a thread four rows.
 template <typename T> __global__ void __launch_bounds__(256) int4_small_join_kernel(const __grid_constant__ SmallParams p, int ctas) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t tile = blockIdx.x, tiles = small_tiles(p), units_all = tiles * p.units;
+    if (p.items) asm volatile("griddepcontrol.wait;" ::: "memory");  // the items may be the kernel's before the last
+    const int tile = blockIdx.x, tiles = small_tiles(p);
     if (tile >= tiles) return;
-    const int64_t a = tile * p.units, z = a + p.units;
-    // the run that holds unit u: the last b whose begin is at most u
-    const int runs = small_runs(units_all, ctas);
-    const auto run_of = [&](int64_t u) { return (int)(((u + 1) * runs + units_all - 1) / units_all - 1); };
-    const int b0 = run_of(a), b1 = run_of(z - 1);
+    const uint32_t units_all = (uint32_t)(tiles * p.units), a = (uint32_t)(tile * p.units);
+    const q4::Runs runs(units_all, small_runs(units_all, ctas), 1u);
+    const uint32_t b0 = runs.of(a), b1 = runs.of(a + p.units - 1);
     if (b0 == b1) return;                                            // one run wrote y itself
     const SmallTile t = small_tile(p, tile);
-    const int which0 = small_begin(units_all, b0, runs) >= a ? 0 : 1, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
+    const int64_t size = (int64_t)p.n_max * 128;
+    // the tile is run b0's last row tile, unless b0 begins with it, and every other run's first
+    const float* part = p.partial + ((int64_t)b0 * 2 + (runs.begin(b0) >= a ? 0 : 1)) * size + lane * 4;
+    const float* next = p.partial + (int64_t)(b0 + 1) * 2 * size + lane * 4;
     T* y = reinterpret_cast<T*>(p.y);
+    if (!p.items) asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int tok = threadIdx.x >> 5; tok < t.n; tok += 8) {
-        const float* part = p.partial + (int64_t)tok * 128 + lane * 4;
-        const int64_t stride = (int64_t)p.n_max * 128;
-        float4 sum = __ldcg(reinterpret_cast<const float4*>(part + (2 * b0 + which0) * stride));
+        float4 sum = __ldcg(reinterpret_cast<const float4*>(part + tok * 128));
 #pragma unroll 4
-        for (int b = b0 + 1; b <= b1; ++b) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 2 * (int64_t)b * stride));
+        for (uint32_t b = b0 + 1; b <= b1; ++b) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(next + (int64_t)(b - b0 - 1) * 2 * size + tok * 128));
             sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
         T* out = y + (int64_t)(t.first + tok) * p.ldy;
@@ -564,10 +565,16 @@ template <typename T> __global__ void __launch_bounds__(256) int4_small_join_ker
                 if (!(lane & 4) && row < p.out_rows) out[row] = gate_up<T>(mine[c], up);
             }
         } else {
+            const int row = t.rt * 128 + lane * 4;
+            q4::Quad<T> q;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int row = t.rt * 128 + lane * 4 + c;
-                if (row < p.out_rows) out[row] = from_f32<T>(mine[c]);
+            for (int c = 0; c < 4; ++c) q.v[c] = from_f32<T>(mine[c]);
+            if (row + 3 < p.out_rows && (reinterpret_cast<uintptr_t>(out + row) & 7u) == 0) {
+                *reinterpret_cast<q4::Quad<T>*>(out + row) = q;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (row + c < p.out_rows) out[row + c] = q.v[c];
             }
         }
     }
@@ -652,6 +659,9 @@ int launch_small(const CUtensorMap& map, const SmallParams& p, const SmallPlan& 
 template <typename T>
 int run_small(const Int4Call& c, const int32_t* order, int topk, void* workspace, cudaStream_t st, const char* what) {
     const SmallPlan pl = plan_small(c);
+    const int64_t all = pl.tiles * q4::div_up(c.cols, q4::kUnitCols);
+    if (all > 0x7fffffff)
+        return fail(P2P_EUNSUPPORTED, "%s: %lld units of 128 x 128 weights, below 2^31", what, (long long)all);
     SmallParams p = {};
     p.layout = reinterpret_cast<const uint8_t*>(c.layout);
     p.record = q4::unit_bytes(c.group, c.has_zeros);

@@ -107,6 +107,25 @@ template <> struct Codes<__half> {
     }
 };
 
+template <typename T> struct alignas(8) Quad { T v[4]; };
+
+// `things` (units, or row tiles of `each` units) dealt to n runs, the first `rest` of which take one more. Below 2^31
+// units in all, and arithmetic in 32 bits: a 64-bit division takes the time of a unit.
+struct Runs {
+    uint32_t whole, rest, each;
+    __device__ __forceinline__ Runs(uint32_t things, uint32_t n, uint32_t each_) {
+        each = each_;
+        whole = things / n;
+        rest = things - whole * n;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t b) const { return (b * whole + min(b, rest)) * each; }
+    // The run that holds unit u, of units dealt one by one, at least one a run.
+    __device__ __forceinline__ uint32_t of(uint32_t u) const {
+        const uint32_t longer = rest * (whole + 1);
+        return u < longer ? u / (whole + 1) : rest + (u - longer) / whole;
+    }
+};
+
 }  // namespace q4
 namespace sm100 {
 

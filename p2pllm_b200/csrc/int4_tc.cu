@@ -164,26 +164,6 @@ template <int PIECES> __device__ __forceinline__ int piece_begin(int n, int i) {
     return at;
 }
 
-template <typename T> struct alignas(8) Quad { T v[4]; };
-
-// The runs: `whole` things (units, or row tiles of that many units each) dealt to the CTAs, the first `rest` of which take
-// one more. Below 2^31 units in all.
-struct Runs {
-    uint32_t whole, rest, each;
-    __device__ __forceinline__ Runs(const TcParams& p, uint32_t tiles) {
-        each = p.partial ? 1u : (uint32_t)p.units;
-        const uint32_t things = p.partial ? tiles * (uint32_t)p.units : tiles;
-        whole = things / (uint32_t)p.ctas;
-        rest = things - whole * (uint32_t)p.ctas;
-    }
-    __device__ __forceinline__ uint32_t begin(uint32_t b) const { return (b * whole + min(b, rest)) * each; }
-    // The run that holds unit u, of a launch that deals units.
-    __device__ __forceinline__ uint32_t of(uint32_t u) const {
-        const uint32_t longer = rest * (whole + 1);
-        return u < longer ? u / (whole + 1) : rest + (u - longer) / whole;
-    }
-};
-
 // PIECES of the tokens; W0, W1: the most columns of a promoting warp's first and second piece, whose sums it holds in
 // registers (W1 = 0: it has one).
 template <typename T, int PIECES, int W0, int W1>
@@ -241,7 +221,8 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
     // The items are the previous kernel's; dense weights wait for nobody, and everything else for that kernel's end.
     if (p.items || (warp != kWeightWarp && (warp < kBuildWarp || warp >= kWeightWarp)))
         asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Runs runs(p, (uint32_t)(p.items ? *p.n_items * p.row_tiles : p.row_tiles * p.token_tiles));
+    const uint32_t tiles = (uint32_t)(p.items ? *p.n_items * p.row_tiles : p.row_tiles * p.token_tiles);
+    const q4::Runs runs(p.partial ? tiles * (uint32_t)p.units : tiles, (uint32_t)p.ctas, p.partial ? 1u : (uint32_t)p.units);
     const int u0 = (int)runs.begin(blockIdx.x), u1 = (int)runs.begin(blockIdx.x + 1);
     const int subs = 128 >> p.group_shift;               // groups a unit
     // TMEM column of buffer b of a piece: the same for every tile, so that one piece may run ahead into the next tile
@@ -539,7 +520,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
 constexpr int kJoinTokens = 32;
 template <typename T> __global__ void __launch_bounds__(256) int4_join_kernel(const __grid_constant__ TcParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const Runs runs(p, (uint32_t)(p.row_tiles * p.token_tiles));
+    const q4::Runs runs((uint32_t)(p.row_tiles * p.token_tiles * p.units), (uint32_t)p.ctas, 1u);
     const uint32_t a = blockIdx.x * (uint32_t)p.units, b0 = runs.of(a), b1 = runs.of(a + p.units - 1);
     if (b0 == b1) return;                                // one run wrote y itself
     const Tile t = tile_at(p, (int)a, (int)a + p.units);
@@ -568,11 +549,11 @@ template <typename T> __global__ void __launch_bounds__(256) int4_join_kernel(co
             }
         } else {
             const int row = t.rt * 128 + lane * 4;
-            Quad<T> q;
+            q4::Quad<T> q;
 #pragma unroll
             for (int c = 0; c < 4; ++c) q.v[c] = from_f32<T>(mine[c]);
             if (row + 3 < p.out_rows && (reinterpret_cast<uintptr_t>(out + row) & 7u) == 0) {
-                *reinterpret_cast<Quad<T>*>(out + row) = q;
+                *reinterpret_cast<q4::Quad<T>*>(out + row) = q;
             } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
