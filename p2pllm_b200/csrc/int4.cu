@@ -240,7 +240,7 @@ template <typename T> __device__ __forceinline__ T gate_up(float g, float u) { r
 // columns in fp32, and the group's scale multiplies that sum on its way into the fp32 accumulators: no weight is ever
 // rounded. G32: groups of 32 columns, two a column block (else one holds the block or more).
 template <typename T, int NT, bool G32>
-__global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_kernel(const __grid_constant__ CUtensorMap tmap_x,
+__global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                                       const __grid_constant__ SmallParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -386,72 +386,80 @@ __global__ void __launch_bounds__(kSmallThreads, NT <= 2 ? 3 : 2) int4_small_ker
                 for (int c = 0; c < NT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[b][c][i] = 0.f;
-            for (int k = ka; k < kz; k += 2) {
-                // a warp that gave up multiplies nothing more, but keeps meeting the others at every row tile's end
-                if (!ok || !(ok = __all_sync(0xffffffffu, wait_one(full(slot), ph, 3, wc)))) break;
-                const uint8_t* at = ring + rec;
-                const int n_units = min(2, kz - k);
+            // LIVE: 8-token columns of this tile that hold a token (an item may be a few of the tile's)
+            auto multiply = [&](auto live) {
+                constexpr int LIVE = decltype(live)::value;
+                for (int k = ka; k < kz; k += 2) {
+                    // a warp that gave up multiplies nothing more, but keeps meeting the others at every row tile's end
+                    if (!ok || !(ok = __all_sync(0xffffffffu, wait_one(full(slot), ph, 3, wc)))) break;
+                    const uint8_t* at = ring + rec;
+                    const int n_units = min(2, kz - k);
 #pragma unroll 1
-                for (int unit = 0; unit < n_units; ++unit, at += p.half_bytes) {
-                uint32_t w[2][4];
+                    for (int unit = 0; unit < n_units; ++unit, at += p.half_bytes) {
+                        uint32_t w[2][4];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint4 c = lds<uint4>(at, code_off + b * 2 * q4::kBlockBytes);
-                    w[b][0] = c.x; w[b][1] = c.y; w[b][2] = c.z; w[b][3] = c.w;
-                }
-                // the two row blocks' products alternate: each waits for its own last one only
-                float part[2][NT][4];
-                auto begin = [&](int b, int g) {
-                    if (p.zeros) {
-                        const uint32_t z = lds<uint16_t>(at, zero_off + b * 16 + g * 128);
-                        codes[b].zeros(z & 15u, z >> 8);
-                    }
-                };
-                auto end = [&](int b, int g) {
-                    const float2 s = unpack2<T>(lds<uint32_t>(at, scale_off + b * 32 + g * 256));
-#pragma unroll
-                    for (int c = 0; c < NT; ++c) {
-                        acc[b][c][0] = fmaf(s.x, part[b][c][0], acc[b][c][0]);
-                        acc[b][c][1] = fmaf(s.x, part[b][c][1], acc[b][c][1]);
-                        acc[b][c][2] = fmaf(s.y, part[b][c][2], acc[b][c][2]);
-                        acc[b][c][3] = fmaf(s.y, part[b][c][3], acc[b][c][3]);
-                    }
-                };
-                begin(0, 0);
-                begin(1, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (G32 && r == 2) {
-                        end(0, 0);
-                        end(1, 0);
-                        begin(0, 1);
-                        begin(1, 1);
-                    }
-                    uint2 xf[NT];
-#pragma unroll
-                    for (int c = 0; c < NT; ++c) xf[c] = lds<uint2>(at, x_off[r] + c * 1024);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t a[4];
-                        codes[b].expand(w[b][r], a);
-#pragma unroll
-                        for (int c = 0; c < NT; ++c) {
-                            mma16816<T>(part[b][c], a, xf[c], r == 0 || (G32 && r == 2) ? zero : part[b][c]);
+                        for (int b = 0; b < 2; ++b) {
+                            const uint4 c = lds<uint4>(at, code_off + b * 2 * q4::kBlockBytes);
+                            w[b][0] = c.x; w[b][1] = c.y; w[b][2] = c.z; w[b][3] = c.w;
                         }
+                        // the two row blocks' products alternate: each waits for its own last one only
+                        float part[2][LIVE][4];
+                        auto begin = [&](int b, int g) {
+                            if (p.zeros) {
+                                const uint32_t z = lds<uint16_t>(at, zero_off + b * 16 + g * 128);
+                                codes[b].zeros(z & 15u, z >> 8);
+                            }
+                        };
+                        auto end = [&](int b, int g) {
+                            const float2 s = unpack2<T>(lds<uint32_t>(at, scale_off + b * 32 + g * 256));
+#pragma unroll
+                            for (int c = 0; c < LIVE; ++c) {
+                                acc[b][c][0] = fmaf(s.x, part[b][c][0], acc[b][c][0]);
+                                acc[b][c][1] = fmaf(s.x, part[b][c][1], acc[b][c][1]);
+                                acc[b][c][2] = fmaf(s.y, part[b][c][2], acc[b][c][2]);
+                                acc[b][c][3] = fmaf(s.y, part[b][c][3], acc[b][c][3]);
+                            }
+                        };
+                        begin(0, 0);
+                        begin(1, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (G32 && r == 2) {
+                                end(0, 0);
+                                end(1, 0);
+                                begin(0, 1);
+                                begin(1, 1);
+                            }
+                            uint2 xf[LIVE];
+#pragma unroll
+                            for (int c = 0; c < LIVE; ++c) xf[c] = lds<uint2>(at, x_off[r] + c * 1024);
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                uint32_t a[4];
+                                codes[b].expand(w[b][r], a);
+#pragma unroll
+                                for (int c = 0; c < LIVE; ++c) {
+                                    mma16816<T>(part[b][c], a, xf[c], r == 0 || (G32 && r == 2) ? zero : part[b][c]);
+                                }
+                            }
+                        }
+                        end(0, G32 ? 1 : 0);
+                        end(1, G32 ? 1 : 0);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty(slot));
+                    rec += 2u * (uint32_t)p.half_bytes;
+                    if (++slot == p.slots) {
+                        slot = 0;
+                        ph ^= 1u;
+                        rec = 0;
                     }
                 }
-                end(0, G32 ? 1 : 0);
-                end(1, G32 ? 1 : 0);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty(slot));
-                rec += 2u * (uint32_t)p.half_bytes;
-                if (++slot == p.slots) {
-                    slot = 0;
-                    ph ^= 1u;
-                    rec = 0;
-                }
-            }
+            };
+            if (NT > 3 && t.n > 24) multiply(std::integral_constant<int, NT>());
+            else if (NT > 2 && t.n > 16) multiply(std::integral_constant<int, NT < 3 ? NT : 3>());
+            else if (NT > 1 && t.n > 8) multiply(std::integral_constant<int, NT < 2 ? NT : 2>());
+            else multiply(std::integral_constant<int, 1>());
             // The row tile's sums [token][row]: the second column block's first, the first one's added to them.
 #pragma unroll
             for (int h = 1; h >= 0; --h) {
@@ -588,7 +596,8 @@ unsigned next_seq() {
 }
 
 // How a call of up to 32 tokens a tile is cut: shares of a cluster's CTAs where they are all resident at once, else
-// runs, two CTAs an SM.
+// runs. Two CTAs an SM: three leave 72 registers, and measured slower (28672 x 4096 at 16 tokens the same, 24 to 33 us at
+// 24; 128 experts on 17 tokens 78 to 100 us).
 struct SmallPlan {
     int nt, splits, ctas, slots, half_bytes, x_at, x_sub, smem;
     int64_t col_tiles, tiles;
@@ -602,15 +611,13 @@ SmallPlan plan_small(const Int4Call& c) {
     pl.nt = (int)q4::div_up(most, 8);
     pl.col_tiles = routed ? c.max_items : q4::div_up(c.tokens, pl.nt * 8);
     pl.tiles = q4::row_tiles(c.rows, c.gated) * pl.col_tiles;
-    const int64_t units = q4::div_up(c.cols, q4::kUnitCols), per_sm = pl.nt <= 2 ? 3 : 2, resident = per_sm * sm_count();
-    static const char* e1 = getenv("X_SPL"); const int mode = e1 ? atoi(e1) : 0;
-    if (mode == 0 ? pl.tiles * 2 <= resident : mode == 1) {
-        int64_t s = resident / pl.tiles;
-        if (s > 8) s = 8;
-        if (s > units / 2) s = units / 2;
-        if (s < 1) s = 1;
-        pl.splits = (int)s;
-        pl.ctas = (int)(pl.tiles * s);
+    const int64_t units = q4::div_up(c.cols, q4::kUnitCols), per_sm = 2, resident = per_sm * sm_count();
+    if (pl.tiles * 2 <= resident) {
+        // a power of two: clusters of three leave SMs empty
+        int s = 2;
+        while (s < 8 && pl.tiles * s * 2 <= resident && units / (2 * s) >= 2) s *= 2;
+        pl.splits = units >= 2 * s ? s : 1;
+        pl.ctas = (int)(pl.tiles * pl.splits);
     } else {
         const int64_t all = pl.tiles * units;
         pl.ctas = (int)(all < resident ? all : resident);

@@ -14,12 +14,12 @@ using torch::autograd::variable_list;
 
 constexpr int64_t kSmallTokens = 8;                   // items of up to here pick x's rows by the order
 
-// Places of one item, what one pass over an expert's weights takes: few where experts have few pairs on average, so
-// that a tile is not mostly empty; otherwise as many as keep the weights' codes from being turned twice.
+// Places of one item, what one pass over an expert's weights takes: about twice what experts have on average, so that
+// few take two passes and no tile is mostly empty; at most what leaves the accumulators room.
 int64_t item_tokens(int64_t pairs, int64_t experts) {
-    if (pairs <= kSmallTokens) return kSmallTokens;
-    const int64_t mean = pairs / experts;
-    return mean <= 8 ? 32 : mean <= 64 ? 128 : 256;
+    const double mean = (double)pairs / experts;
+    if (pairs <= kSmallTokens || mean <= 4) return kSmallTokens;
+    return mean <= 10 ? 16 : mean <= 24 ? 32 : mean <= 96 ? 128 : 256;
 }
 
 // t [rows, cols] with unit column stride and rows that do not overlap (an expanded gradient's do).

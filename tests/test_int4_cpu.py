@@ -86,7 +86,7 @@ def test_operators_propagate_shapes_on_meta_tensors(lib):
     assert ops.int4_mm(meta(17, 64), w, False, 40, 64, 64, False).shape == (17, 40)
     assert ops.int4_mm(meta(17, 64), w, False, 40, 64, 64, True).shape == (17, 20)
     order, where, offsets, items, n = ops.moe_sort(meta(17, 8, dtype=torch.int64), 128)
-    assert order.shape == where.shape == (136,) and offsets.shape == (129,) and items.shape == (4 * 133,) and n.shape == (1,)
+    assert order.shape == where.shape == (136,) and offsets.shape == (129,) and items.shape == (4 * 136,) and n.shape == (1,)
     assert ops.int4_grouped(meta(17, 64), w, False, 128, 40, 64, 64, True, order, where, offsets, items, n, 8, True).shape == (136, 20)
     x = meta(17, 96).requires_grad_(True)
     xs = ops.moe_spread(x, where, offsets, 8)
