@@ -295,14 +295,24 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
                 for (int i = 0; i < n; ++i)
                     bulk_load(base + (2 * slot + i) * p.half_bytes, t.records + (int64_t)(k + i) * p.record, w_bytes, full(slot));
             };
+            int rows[8];                                             // x's rows of a tile that picks them, at most 8
+            auto pick = [&](const SmallTile& t) {
+                if (!p.order) return;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rows[i] = i < t.n ? __ldcg(p.order + t.first + i) : 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rows[i] /= p.topk;
+            };
             auto load_x = [&](int slot, const SmallTile& t, int k, int n) {
                 for (int h = 0; h < n; ++h) {
                     const uint32_t at = base + (2 * slot + h) * p.half_bytes + p.x_at;
                     if (p.order) {                                   // a row at a time, from wherever its token lies
-                        for (int i = 0; i < t.n; ++i) {
-                            const int row = __ldcg(p.order + t.first + i) / p.topk;
-                            tma_load_2d(at + i * 128, &tmap_x, (k + h) * 128, row, full(slot));
-                            tma_load_2d(at + p.x_sub + i * 128, &tmap_x, (k + h) * 128 + 64, row, full(slot));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if (i < t.n) {
+                                tma_load_2d(at + i * 128, &tmap_x, (k + h) * 128, rows[i], full(slot));
+                                tma_load_2d(at + p.x_sub + i * 128, &tmap_x, (k + h) * 128 + 64, rows[i], full(slot));
+                            }
                         }
                     } else {
                         tma_load_2d(at, &tmap_x, (k + h) * 128, t.first, full(slot));
@@ -336,6 +346,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
             while (u < u1 && ok) {
                 const SmallTile t = small_tile(p, u / p.units);
                 const int kz = min(p.units, u % p.units + (u1 - u));
+                pick(t);
                 for (int k = u % p.units; k < kz;) {
                     if (used >= n_slots && !(ok = wait_one(empty(slot), ph ^ 1u, 1, wc))) break;
                     const int n = min(2, kz - k);

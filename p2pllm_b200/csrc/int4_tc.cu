@@ -43,8 +43,8 @@ constexpr int build_groups(int acc) { return acc <= 32 ? 2 : 1; }
 constexpr int threads_of(int acc) { return (kPromoteWarps + build_groups(acc) * group_warps(acc) + 4) * 32; }
 // Registers a thread of promoting, building and other warps: what the launch gives (a whole register file over the
 // threads, in eights), dealt anew. 0: as launched.
-constexpr int promote_regs(int acc) { return acc >= 96 ? 200 : acc >= 64 ? 128 : 0; }
-constexpr int build_regs(int acc) { return acc >= 96 ? 64 : 72; }
+constexpr int promote_regs(int acc) { return acc >= 96 ? 200 : acc >= 64 ? 136 : 0; }
+constexpr int build_regs(int acc) { return acc >= 96 ? 64 : 64; }
 constexpr int other_regs(int acc) { return acc >= 96 ? 40 : 48; }
 constexpr int dealt_regs(int acc) {
     return kPromoteWarps * 32 * promote_regs(acc) + build_groups(acc) * group_warps(acc) * 32 * build_regs(acc) + 128 * other_regs(acc);
@@ -152,10 +152,10 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int u, int u1) {
     }
     return t;
 }
-// Pieces of the tokens, each a multiple of 16: all of them up to 32, halves up to 128, quarters above. (An accumulator
+// Pieces of the tokens, each a multiple of 16: all of them up to 32, halves up to 160, quarters above. (An accumulator
 // that is read out cannot take products: with four pieces three multiply meanwhile.)
 __host__ __device__ constexpr int n_total(int n) { return (n + 15) & ~15; }
-__host__ __device__ constexpr int pieces_of(int n_max) { return n_max <= 32 ? 1 : n_max <= 128 ? 2 : 4; }
+__host__ __device__ constexpr int pieces_of(int n_max) { return n_max <= 32 ? 1 : n_max <= 160 ? 2 : 4; }
 template <int PIECES> __device__ __forceinline__ int piece_size(int n, int i) { return (n_total(n) / 16 - i + PIECES - 1) / PIECES * 16; }
 template <int PIECES> __device__ __forceinline__ int piece_begin(int n, int i) {
     int at = 0;
@@ -637,6 +637,7 @@ template <typename T> int launch_width(const CUtensorMap& map, const TcParams& p
     if (p.n_max <= 32) return launch_tc<T, 1, 32, 0>(map, p, smem, st, what);
     if (p.n_max <= 64) return launch_tc<T, 2, 32, 0>(map, p, smem, st, what);
     if (p.n_max <= 128) return launch_tc<T, 2, 64, 0>(map, p, smem, st, what);
+    if (p.n_max <= 160) return launch_tc<T, 2, 80, 0>(map, p, smem, st, what);
     if (p.n_max <= 192) return launch_tc<T, 4, 48, 48>(map, p, smem, st, what);
     return launch_tc<T, 4, 80, 64>(map, p, smem, st, what);
 }

@@ -14,12 +14,12 @@ using torch::autograd::variable_list;
 
 constexpr int64_t kSmallTokens = 8;                   // items of up to here pick x's rows by the order
 
-// Places of one item, what one pass over an expert's weights takes: about twice what experts have on average, so that
+// Places of one item, what one pass over an expert's weights takes: somewhat more than experts have on average, so that
 // few take two passes and no tile is mostly empty; at most what leaves the accumulators room.
 int64_t item_tokens(int64_t pairs, int64_t experts) {
     const double mean = (double)pairs / experts;
     if (pairs <= kSmallTokens || mean <= 4) return kSmallTokens;
-    return mean <= 10 ? 16 : mean <= 24 ? 32 : mean <= 96 ? 128 : 256;
+    return mean <= 10 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 100 ? 128 : mean <= 130 ? 160 : 256;
 }
 
 // t [rows, cols] with unit column stride and rows that do not overlap (an expanded gradient's do).

@@ -44,7 +44,10 @@ def _check_order(order, ids, experts):
     items = order.items.view(-1, 4)[:int(order.n_items)].tolist()
     at, plain = offsets.tolist(), []
     most, mean = ids.numel(), ids.numel() / experts                 # what one pass over an expert's weights takes
-    most = 8 if most <= 8 or mean <= 4 else 16 if mean <= 10 else 32 if mean <= 24 else 128 if mean <= 96 else 256
+    if most > 8:
+        most = next(n for n, up_to in ((8, 4), (16, 10), (32, 24), (64, 48), (128, 100), (160, 130), (256, 1e9)) if mean <= up_to)
+    else:
+        most = 8
     for e in range(experts):
         plain += [[e, a, min(most, at[e + 1] - a), 0] for a in range(at[e], at[e + 1], most)]
     assert items == plain
