@@ -95,6 +95,16 @@ __device__ __forceinline__ void ld16_wait(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t taddr, const uint64_t* v) {
+    asm volatile(
+        "{\n\t.reg .b32 r<16>;\n\t"
+        "mov.b64 {r0, r1}, %1;\n\tmov.b64 {r2, r3}, %2;\n\tmov.b64 {r4, r5}, %3;\n\tmov.b64 {r6, r7}, %4;\n\t"
+        "mov.b64 {r8, r9}, %5;\n\tmov.b64 {r10, r11}, %6;\n\tmov.b64 {r12, r13}, %7;\n\tmov.b64 {r14, r15}, %8;\n\t"
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, "
+        "r15};\n\t}" ::"r"(taddr),
+        "l"(v[0]), "l"(v[1]), "l"(v[2]), "l"(v[3]), "l"(v[4]), "l"(v[5]), "l"(v[6]), "l"(v[7])
+        : "memory");
+}
 // Two fp32 products and sums at once: acc.{lo,hi} += s.{lo,hi} * {lo, hi}.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t s, uint32_t lo, uint32_t hi) {
     asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%2, %3};\n\tfma.rn.f32x2 %0, %1, v, %0;\n\t}" : "+l"(acc) : "l"(s), "r"(lo), "r"(hi));
@@ -172,6 +182,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
     // The promoting warps need an accumulator of up to 144 registers and take what the others give back.
     constexpr int kAcc = W0 + W1, kGroups = build_groups(kAcc), kGroupWarps = group_warps(kAcc);
     constexpr bool kSplitRegs = promote_regs(kAcc) > 0;
+    constexpr bool kStaged = kAcc > 32;                  // sums leave through tensor memory
     constexpr int kWeightWarp = kBuildWarp + kGroups * kGroupWarps;
     constexpr int kXWarp = kWeightWarp + 1, kMmaWarp = kWeightWarp + 2;
     extern __shared__ uint8_t smem_raw[];
@@ -427,79 +438,143 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
             uint64_t acc[(W0 + W1) / 2];
 #pragma unroll
             for (int i = 0; i < (W0 + W1) / 2; ++i) acc[i] = 0;
-            for (int k = t.k0; k < t.k1 && ok; ++k) {
-                if (!(ok = wait_all(sfull(ss), phs, 13, wc))) break;
-#pragma unroll 1
-                for (int sub = 0; sub < subs; ++sub) {
-                    const uint16_t bits = (uint16_t)lds_u16(s_ring + ss * kSSlotBytes + sub * 256 + scale_at);
-                    uint64_t s2;
-                    asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(to_f32(*reinterpret_cast<const T*>(&bits)))));
-                    auto promote = [&](auto which) {
-                        constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0;
-                        const int piece = h + 2 * I;
-                        if (!ok || !(ok = wait_all(dfull(piece, sb), phb, 11, wc))) return;
-                        tc_fence_after();
-                        const uint32_t d = d_at[I] + sb * p.n_max;
+            // one group of the run's next unit; the tile's last sums are kept for the way out
+            int sub = 0;
+            auto step = [&](auto kept) {
+                if (sub == 0 && !(ok = wait_all(sfull(ss), phs, 13, wc))) return;
+                const uint16_t bits = (uint16_t)lds_u16(s_ring + ss * kSSlotBytes + sub * 256 + scale_at);
+                uint64_t s2;
+                asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(to_f32(*reinterpret_cast<const T*>(&bits)))));
+                auto promote = [&](auto which) {
+                    constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0;
+                    const int piece = h + 2 * I;
+                    if (!ok || !(ok = wait_all(dfull(piece, sb), phb, 11, wc))) return;
+                    tc_fence_after();
+                    const uint32_t d = d_at[I] + sb * p.n_max;
 #pragma unroll
-                        for (int c = 0; c < kWidth / 16; ++c) {
-                            if (c * 16 < size[I]) {
-                                uint32_t v[16];
-                                ld16_async(d + c * 16, v);
-                                ld16_wait(v);
+                    for (int c = 0; c < kWidth / 16; ++c) {
+                        if (c * 16 < size[I]) {
+                            uint32_t v[16];
+                            ld16_async(d + c * 16, v);
+                            ld16_wait(v);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) fma2(acc[I * W0 / 2 + c * 8 + e], s2, v[2 * e], v[2 * e + 1]);
-                            }
+                            for (int e = 0; e < 8; ++e) fma2(acc[I * W0 / 2 + c * 8 + e], s2, v[2 * e], v[2 * e + 1]);
                         }
+                    }
+                    if constexpr (!decltype(kept)::value) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(dempty(piece, sb));
-                    };
-                    promote(std::integral_constant<int, 0>());
-                    if constexpr (W1 > 0) promote(std::integral_constant<int, 1>());
-                    if (!ok) break;
-                    advance(sb, phb, 1, NB);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sempty(ss));
-                advance(ss, phs, 1, kSSlots);
-            }
-            if (!ok) break;
-            auto store = [&](auto which) {
-                constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0, kAt = I * W0 / 2;
-                const int col0 = piece_begin<PIECES>(t.n, h + 2 * I);
-                const int left = min(size[I], t.n - col0);                               // this piece's tokens
-                if (t.k1 - t.k0 < p.units) {             // shared with the neighbouring run
-                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 +
-                                  (int64_t)col0 * 128 + row_in;
-#pragma unroll
-                    for (int c = 0; c < kWidth; ++c)
-                        if (c < left) part[c * 128] = half_of(acc[kAt + c / 2], c & 1);
-                } else if (p.gated) {
-                    // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each pair
-                    // of lanes exchanges one of two columns and finishes the other.
-                    const int row = t.rt * 64 + 16 * q + (lane & 15);
-                    T* out = y + (int64_t)(t.first + col0 + (lane >> 4)) * p.ldy + row;
-#pragma unroll
-                    for (int c = 0; c < kWidth; c += 2) {
-                        if (c >= left) continue;
-                        const float even = half_of(acc[kAt + c / 2], 0), odd = half_of(acc[kAt + c / 2], 1);
-                        const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? odd : even, 16);
-                        const float gate = lane < 16 ? even : other, up = lane < 16 ? other : odd;
-                        if (c + (lane >> 4) < left && row < p.out_rows)
-                            out[c * p.ldy] = from_f32<T>(gate / (1.f + expf(-gate)) * up);
                     }
-                } else {
-                    const int row = t.rt * 128 + row_in;
-                    if (row < p.out_rows) {
-                        T* out = y + (int64_t)(t.first + col0) * p.ldy + row;
-#pragma unroll
-                        for (int c = 0; c < kWidth; ++c)
-                            if (c < left) out[c * p.ldy] = from_f32<T>(half_of(acc[kAt + c / 2], c & 1));
-                    }
+                };
+                promote(std::integral_constant<int, 0>());
+                if constexpr (W1 > 0) promote(std::integral_constant<int, 1>());
+                if constexpr (!decltype(kept)::value) advance(sb, phb, 1, NB);
+                if (++sub == subs) {
+                    sub = 0;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sempty(ss));
+                    advance(ss, phs, 1, kSSlots);
                 }
             };
-            store(std::integral_constant<int, 0>());
-            if constexpr (W1 > 0) store(std::integral_constant<int, 1>());
+#pragma unroll 1
+            for (int jobs = (t.k1 - t.k0) * subs - 1; jobs > 0 && ok; --jobs) step(std::false_type());
+            if (ok) step(std::integral_constant<bool, kStaged>());
+            if (!ok) break;
+            if constexpr (!kStaged) {
+                auto store = [&](auto which) {
+                    constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0, kAt = I * W0 / 2;
+                    const int col0 = piece_begin<PIECES>(t.n, h + 2 * I);
+                    const int left = min(size[I], t.n - col0);                               // this piece's tokens
+                    if (t.k1 - t.k0 < p.units) {             // shared with the neighbouring run
+                        float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 +
+                                      (int64_t)col0 * 128 + row_in;
+#pragma unroll
+                        for (int c = 0; c < kWidth; ++c)
+                            if (c < left) part[c * 128] = half_of(acc[kAt + c / 2], c & 1);
+                    } else if (p.gated) {
+                        // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each pair
+                        // of lanes exchanges one of two columns and finishes the other.
+                        const int row = t.rt * 64 + 16 * q + (lane & 15);
+                        T* out = y + (int64_t)(t.first + col0 + (lane >> 4)) * p.ldy + row;
+#pragma unroll
+                        for (int c = 0; c < kWidth; c += 2) {
+                            if (c >= left) continue;
+                            const float even = half_of(acc[kAt + c / 2], 0), odd = half_of(acc[kAt + c / 2], 1);
+                            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? odd : even, 16);
+                            const float gate = lane < 16 ? even : other, up = lane < 16 ? other : odd;
+                            if (c + (lane >> 4) < left && row < p.out_rows)
+                                out[c * p.ldy] = from_f32<T>(gate / (1.f + expf(-gate)) * up);
+                        }
+                    } else {
+                        const int row = t.rt * 128 + row_in;
+                        if (row < p.out_rows) {
+                            T* out = y + (int64_t)(t.first + col0) * p.ldy + row;
+#pragma unroll
+                            for (int c = 0; c < kWidth; ++c)
+                                if (c < left) out[c * p.ldy] = from_f32<T>(half_of(acc[kAt + c / 2], c & 1));
+                        }
+                    }
+                };
+                store(std::integral_constant<int, 0>());
+            } else {
+                // The way out, through the accumulator just read: a loop over 16 columns at a time. (Straight from the
+                // registers every column would be code of its own, fetched anew each time: 21,000 cycles a row tile of 272
+                // tokens.)
+                auto stage = [&](auto which) {
+                    constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0;
+#pragma unroll
+                    for (int c = 0; c < kWidth / 16; ++c)
+                        if (c * 16 < size[I]) st16(d_at[I] + sb * p.n_max + c * 16, acc + I * W0 / 2 + c * 8);
+                };
+                stage(std::integral_constant<int, 0>());
+                if constexpr (W1 > 0) stage(std::integral_constant<int, 1>());
+                tmem_wait_st();
+                const bool whole = t.k1 - t.k0 == p.units;
+#pragma unroll 1
+                for (int i = 0; i < (W1 > 0 ? 2 : 1); ++i) {
+                    const int piece = h + 2 * i, col0 = piece_begin<PIECES>(t.n, piece), n = i ? size[1] : size[0];
+                    const int left = min(n, t.n - col0);     // this piece's tokens
+                    const uint32_t d = (i ? d_at[1] : d_at[0]) + sb * p.n_max;
+                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 + (int64_t)col0 * 128 + row_in;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < n; c0 += 16) {
+                        uint32_t v[16];
+                        ld16_async(d + c0, v);
+                        ld16_wait(v);
+                        if (!whole) {                        // shared with the neighbouring run
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                if (c0 + c < left) part[(c0 + c) * 128] = __uint_as_float(v[c]);
+                        } else if (p.gated) {
+                            // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each
+                            // pair of lanes exchanges one of two columns and finishes the other.
+                            const int row = t.rt * 64 + 16 * q + (lane & 15);
+                            T* out = y + (int64_t)(t.first + col0 + c0 + (lane >> 4)) * p.ldy + row;
+#pragma unroll
+                            for (int c = 0; c < 16; c += 2) {
+                                const uint32_t other = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[c + 1] : v[c], 16);
+                                const float gate = __uint_as_float(lane < 16 ? v[c] : other);
+                                const float up = __uint_as_float(lane < 16 ? other : v[c + 1]);
+                                if (c0 + c + (lane >> 4) < left && row < p.out_rows)
+                                    out[c * p.ldy] = from_f32<T>(gate / (1.f + expf(-gate)) * up);
+                            }
+                        } else {
+                            const int row = t.rt * 128 + row_in;
+                            T* out = y + (int64_t)(t.first + col0 + c0) * p.ldy + row;
+                            if (row < p.out_rows) {
+#pragma unroll
+                                for (int c = 0; c < 16; ++c)
+                                    if (c0 + c < left) out[c * p.ldy] = from_f32<T>(__uint_as_float(v[c]));
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(dempty(piece, sb));
+                }
+                advance(sb, phb, 1, NB);
+            }
             u += t.k1 - t.k0;
         }
         if (p.routed) {                                  // what lies behind the last pair
