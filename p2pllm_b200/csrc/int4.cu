@@ -10,7 +10,6 @@
 //   p2p_int4_grouped    the same for the rows of one expert after the other, rows gathered by token or in place, with
 //                       silu(gate) * up applied on the way out of a gated module
 #include <atomic>
-#include <stdlib.h>
 
 #include "int4.cuh"
 #include "int4_run.cuh"
@@ -787,7 +786,7 @@ extern "C" int p2p_int4_layout(const uint8_t* codes, const void* scales, const u
 namespace {
 // Calls of up to this many tokens take the kernel above, which streams weights at the memory's rate and multiplies on
 // the warps' own tensor path; above, that path's rate would bind.
-static const char* e_st = getenv("X_ST"); static const int64_t kSmallTokens = e_st ? atoi(e_st) : 32;
+constexpr int64_t kSmallTokens = 32;
 
 int check_int4(const Int4Call& c, const char* what) {
     if (c.dtype != P2P_BF16 && c.dtype != P2P_F16) return fail(P2P_EUNSUPPORTED, "%s: bf16 or f16", what);

@@ -479,20 +479,33 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
             };
 #pragma unroll 1
             for (int jobs = (t.k1 - t.k0) * subs - 1; jobs > 0 && ok; --jobs) step(std::false_type());
-            if (ok) step(std::integral_constant<bool, kStaged>());
+            const bool whole = t.k1 - t.k0 == p.units;
+            if (ok) {
+                if (kStaged && whole) step(std::integral_constant<bool, kStaged>());
+                else step(std::false_type());
+            }
             if (!ok) break;
-            if constexpr (!kStaged) {
+            if (!whole) {                                // shared with the neighbouring run: all of the piece's columns
+                float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 + row_in;
+                auto leave = [&](auto which) {
+                    constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0;
+                    float* at = part + piece_begin<PIECES>(t.n, h + 2 * I) * 128;
+#pragma unroll
+                    for (int c0 = 0; c0 < kWidth; c0 += 16) {
+                        if (c0 < size[I]) {
+#pragma unroll
+                            for (int c = c0; c < c0 + 16; ++c) at[c * 128] = half_of(acc[I * W0 / 2 + c / 2], c & 1);
+                        }
+                    }
+                };
+                leave(std::integral_constant<int, 0>());
+                if constexpr (W1 > 0) leave(std::integral_constant<int, 1>());
+            } else if constexpr (!kStaged) {
                 auto store = [&](auto which) {
                     constexpr int I = decltype(which)::value, kWidth = I ? W1 : W0, kAt = I * W0 / 2;
                     const int col0 = piece_begin<PIECES>(t.n, h + 2 * I);
                     const int left = min(size[I], t.n - col0);                               // this piece's tokens
-                    if (t.k1 - t.k0 < p.units) {             // shared with the neighbouring run
-                        float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 +
-                                      (int64_t)col0 * 128 + row_in;
-#pragma unroll
-                        for (int c = 0; c < kWidth; ++c)
-                            if (c < left) part[c * 128] = half_of(acc[kAt + c / 2], c & 1);
-                    } else if (p.gated) {
+                    if (p.gated) {
                         // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each pair
                         // of lanes exchanges one of two columns and finishes the other.
                         const int row = t.rt * 64 + 16 * q + (lane & 15);
@@ -530,23 +543,17 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                 stage(std::integral_constant<int, 0>());
                 if constexpr (W1 > 0) stage(std::integral_constant<int, 1>());
                 tmem_wait_st();
-                const bool whole = t.k1 - t.k0 == p.units;
 #pragma unroll 1
                 for (int i = 0; i < (W1 > 0 ? 2 : 1); ++i) {
                     const int piece = h + 2 * i, col0 = piece_begin<PIECES>(t.n, piece), n = i ? size[1] : size[0];
                     const int left = min(n, t.n - col0);     // this piece's tokens
                     const uint32_t d = (i ? d_at[1] : d_at[0]) + sb * p.n_max;
-                    float* part = p.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * p.n_max * 128 + (int64_t)col0 * 128 + row_in;
 #pragma unroll 1
                     for (int c0 = 0; c0 < n; c0 += 16) {
                         uint32_t v[16];
                         ld16_async(d + c0, v);
                         ld16_wait(v);
-                        if (!whole) {                        // shared with the neighbouring run
-#pragma unroll
-                            for (int c = 0; c < 16; ++c)
-                                if (c0 + c < left) part[(c0 + c) * 128] = __uint_as_float(v[c]);
-                        } else if (p.gated) {
+                        if (p.gated) {
                             // even row blocks are gates, odd ones the same units' ups: lanes i and i + 16 of a warp. Each
                             // pair of lanes exchanges one of two columns and finishes the other.
                             const int row = t.rt * 64 + 16 * q + (lane & 15);
