@@ -15,6 +15,7 @@ namespace {
 constexpr int kSortThreads = 1024;
 constexpr int kSortExperts = 1024;
 constexpr int kClusterCtas = 8;
+constexpr int kKept = 8;
 constexpr int64_t kOneCtaPairs = 8192;
 
 struct SortParams {
@@ -27,7 +28,8 @@ struct SortParams {
 
 // A stable counting sort by one CTA, or by a cluster of 8 above 8192 pairs (each then counts and places an eighth).
 // Every warp owns a run of consecutive pairs: it counts them into a histogram of its own, 32 at a step (lanes with the
-// same expert find each other by match.any, so no atomics and no order to lose), the histograms turn into first places
+// same expert find each other by one ballot a bit of the expert -- match.any takes a turn for every expert among them --
+// so no atomics and no order to lose), the histograms turn into first places
 // by sums over warps, CTAs (through distributed shared memory) and experts, and the warp walks its run again and places
 // the pairs.
 template <typename I>
@@ -36,6 +38,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.experts;
     int* hist = sm;                                  // [warps][E]
     int* mine = hist + warps * E;                    // [E]: this CTA's pairs of each expert, which the others read
+    int* base = mine + E;                            // [E]: the place of this CTA's first pair of each expert
     __shared__ int s_sum[2][32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int cta = blockIdx.x, ctas = gridDim.x;    // the grid is one cluster
@@ -48,36 +51,69 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
     const unsigned below = (1u << lane) - 1u;
     int* h = hist + warp * E;
     auto expert_at = [&](int i) -> int {             // -1: routed nowhere
-        const int64_t e = i < end ? (int64_t)ids[i] : -1;
+        const int64_t e = i < end ? (int64_t)__ldcg(ids + i) : -1;
         return e >= 0 && e < E ? (int)e : -1;
     };
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int e = expert_at(i0 + lane);
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && (peers & below) == 0) h[e] += __popc(peers);
+    // Up to kKept steps of 32 pairs are kept in registers between the two walks, and loaded all at once.
+    int kept[kKept];
+    unsigned peers[kKept];
+#pragma unroll
+    for (int s = 0; s < kKept; ++s) kept[s] = expert_at(begin + s * 32 + lane);
+    const int bits = 32 - __clz(E);                  // of 0..E, E standing for nowhere
+    auto same_expert = [&](int e) -> unsigned {
+        const unsigned key = e >= 0 ? (unsigned)e : (unsigned)E;
+        unsigned same = 0xffffffffu;
+        for (int b = 0; b < bits; ++b) {
+            const bool one = (key >> b) & 1u;
+            const unsigned ones = __ballot_sync(0xffffffffu, one);
+            same &= one ? ones : ~ones;
+        }
+        return same;
+    };
+    auto count = [&](int e, unsigned same) {
+        if (e >= 0 && (same & below) == 0) h[e] += __popc(same);
         __syncwarp();
+    };
+#pragma unroll
+    for (int s = 0; s < kKept; ++s) {
+        if (begin + s * 32 < end) {
+            peers[s] = same_expert(kept[s]);
+            count(kept[s], peers[s]);
+        }
+    }
+    for (int i0 = begin + kKept * 32; i0 < end; i0 += 32) {
+        const int e = expert_at(i0 + lane);
+        count(e, same_expert(e));
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += blockDim.x) {              // first places within this CTA
+    if (threadIdx.x < E) {                                           // first places within this CTA; E <= blockDim
         int run = 0;
-        for (int w = 0; w < warps; ++w) {
-            const int c = hist[w * E + e];
-            hist[w * E + e] = run;
-            run += c;
+        for (int w0 = 0; w0 < warps; w0 += 8) {
+            int c[8];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) c[w] = w0 + w < warps ? hist[(w0 + w) * E + threadIdx.x] : 0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                if (w0 + w < warps) hist[(w0 + w) * E + threadIdx.x] = run;
+                run += c[w];
+            }
         }
-        mine[e] = run;
+        mine[threadIdx.x] = run;
     }
     if (ctas > 1) sm100::cluster_sync_all(); else __syncthreads();
-    // totals over the CTAs, and exclusive sums over the experts: of the pairs and of the items. E <= blockDim.
+    // totals over the CTAs, and exclusive sums over the experts: of the pairs and of the items
     int all = 0, before = 0;
     if (threadIdx.x < E) {
         if (ctas > 1) {
             const uint32_t at = sm100::smem_u32(mine + threadIdx.x);
-            for (int c = 0; c < ctas; ++c) {
-                int v;
-                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(sm100::cluster_addr(at, c)) : "memory");
-                if (c < cta) before += v;
-                all += v;
+            int v[kClusterCtas];
+#pragma unroll
+            for (int c = 0; c < kClusterCtas; ++c)
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[c]) : "r"(sm100::cluster_addr(at, c)) : "memory");
+#pragma unroll
+            for (int c = 0; c < kClusterCtas; ++c) {
+                if (c < cta) before += v[c];
+                all += v[c];
             }
         } else {
             all = mine[threadIdx.x];
@@ -100,7 +136,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
     }
     const int start = pair_base + pairs - all, first_item = item_base + items - n_it;
     if (threadIdx.x < E) {
-        for (int w = 0; w < warps; ++w) hist[w * E + threadIdx.x] += start + before;
+        base[threadIdx.x] = start + before;
         if (cta == 0) {
             p.offsets[threadIdx.x] = start;
             for (int k = 0; k < n_it && first_item + k < p.max_items; ++k)
@@ -113,18 +149,23 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
         *p.n_items = min(item_total, p.max_items);
     }
     __syncthreads();
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane, e = expert_at(i);
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
+    auto place = [&](int i, int e, unsigned same) {
         const int at = e >= 0 ? h[e] : 0;
         __syncwarp();
-        if (e >= 0 && (peers & below) == 0) h[e] = at + __popc(peers);
+        if (e >= 0 && (same & below) == 0) h[e] = at + __popc(same);
         __syncwarp();
         if (i < end) {
-            const int place = at + __popc(peers & below);
-            p.where[i] = e >= 0 ? place : -1;
-            if (e >= 0) p.order[place] = i;
+            const int to = e >= 0 ? base[e] + at + __popc(same & below) : -1;
+            p.where[i] = to;
+            if (e >= 0) p.order[to] = i;
         }
+    };
+#pragma unroll
+    for (int s = 0; s < kKept; ++s)
+        if (begin + s * 32 < end) place(begin + s * 32 + lane, kept[s], peers[s]);
+    for (int i0 = begin + kKept * 32; i0 < end; i0 += 32) {
+        const int e = expert_at(i0 + lane);
+        place(i0 + lane, e, same_expert(e));
     }
     for (int i = pair_total + cta * blockDim.x + threadIdx.x; i < p.n; i += ctas * blockDim.x) p.order[i] = -1;
     if (ctas > 1) sm100::cluster_sync_all();         // nobody leaves while its counts may still be read
@@ -174,60 +215,82 @@ template <typename T, int N> __device__ __forceinline__ void zero_behind(const R
         store_vec<T, N>(p.out, (last + i / p.vecs) * p.ldo + i % p.vecs * N, zero);
 }
 
-constexpr int kBatch = 8;                            // slots whose rows a thread holds at a time
+constexpr int kBatch = 4;                            // slots whose rows a thread holds at a time: eight cost half the blocks
+                                                     // an SM (8192 x 8 rows of 4 KB: gradient 128 us to 98)
 constexpr int kRowThreads = 256;
+
+// The places (-1: nowhere) and weights of slots j0.. of token t, which every lane of its warp gets: one load a warp.
+template <int N> struct Slots { int at[N]; float w[N]; };
+template <int N> __device__ __forceinline__ Slots<N> load_slots(const RowParams& p, int64_t t, int j0, bool live) {
+    const int lane = threadIdx.x & 31;
+    const bool in = live && lane < N && j0 + lane < p.k;
+    const int64_t i = t * p.k + j0 + lane;
+    const int at = in ? __ldcg(p.where + i) : -1;
+    const float w = in && p.w ? load_weight(p.w, p.w_dtype, i) : 1.f;
+    Slots<N> s;
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+        s.at[b] = __shfl_sync(0xffffffffu, at, b);
+        s.w[b] = __shfl_sync(0xffffffffu, w, b);
+    }
+    return s;
+}
 
 template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) spread_kernel(const RowParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (t < p.tokens) {
+    for (int j0 = 0; j0 < p.k; j0 += kBatch) {
+        const Slots<kBatch> s = load_slots<kBatch>(p, t, j0, t < p.tokens);
+        if (t >= p.tokens) break;
         for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < p.vecs; v += gridDim.y * blockDim.x) {
             const Vec<T, N> val = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
-#pragma unroll 4
-            for (int j = 0; j < p.k; ++j) {
-                const int at = __ldcg(p.where + t * p.k + j);
-                if (at >= 0) store_vec<T, N>(p.out, at * p.ldo + (int64_t)v * N, val);
-            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (s.at[b] >= 0) store_vec<T, N>(p.out, s.at[b] * p.ldo + (int64_t)v * N, val);
         }
     }
     zero_behind<T, N>(p);
 }
 
-template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_kernel(const RowParams p) {
+// A thread's loads of a batch go out together: a slot routed nowhere reads the batch's row 0 and drops it.
+template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) sum_kernel(const RowParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (t >= p.tokens) return;
-    for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < p.vecs; v += gridDim.y * blockDim.x) {
+    const int lane = threadIdx.x & 31;
+    Slots<kBatch> s = load_slots<kBatch>(p, t, 0, true);
+    // whole warps go round, so that all lanes of one are there when it loads its slots
+    for (int v0 = blockIdx.y * blockDim.x + threadIdx.x - lane; v0 < p.vecs; v0 += gridDim.y * blockDim.x) {
+        const bool on = v0 + lane < p.vecs;
+        const int64_t col = (int64_t)(on ? v0 + lane : 0) * N;
         float acc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.f;
         for (int j0 = 0; j0 < p.k; j0 += kBatch) {
+            if (p.k > kBatch) s = load_slots<kBatch>(p, t, j0, true);
             Vec<T, N> rows[kBatch];
-            int at[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (j0 + b < p.k) rows[b] = load_vec<T, N>(p.y, max(s.at[b], 0) * p.ldy + col);
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                at[b] = j0 + b < p.k ? __ldcg(p.where + t * p.k + j0 + b) : -1;
-                if (at[b] >= 0) rows[b] = load_vec<T, N>(p.y, at[b] * p.ldy + (int64_t)v * N);
-            }
+                if (s.at[b] < 0) continue;
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                if (at[b] < 0) continue;
-                const float w = p.w ? load_weight(p.w, p.w_dtype, t * p.k + j0 + b) : 1.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] = fmaf(w, to_f32(rows[b].v[i]), acc[i]);
+                for (int i = 0; i < N; ++i) acc[i] = fmaf(s.w[b], to_f32(rows[b].v[i]), acc[i]);
             }
         }
+        if (!on) continue;
         Vec<T, N> o;
 #pragma unroll
         for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[i]);
-        store_vec<T, N>(p.out, t * p.ldo + (int64_t)v * N, o);
+        store_vec<T, N>(p.out, t * p.ldo + col, o);
     }
 }
 
 // blockDim.x is whole warps: a token's dots are summed by shuffles, then over its warps in warp order.
-template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_back_kernel(const RowParams p) {
+template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) sum_back_kernel(const RowParams p) {
     __shared__ float s_dot[kRowThreads / 32][kBatch];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -235,32 +298,27 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) sum_
     const int lane = threadIdx.x & 31, row_warps = blockDim.x >> 5, row_warp = threadIdx.x >> 5;
     const bool live = t < p.tokens;
     for (int j0 = 0; j0 < p.k; j0 += kBatch) {
-        float dot[kBatch], w[kBatch];
-        int at[kBatch];
+        const Slots<kBatch> s = load_slots<kBatch>(p, t, j0, live);
+        float dot[kBatch];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const bool in = live && j0 + b < p.k;
-            dot[b] = 0.f;
-            at[b] = in ? __ldcg(p.where + t * p.k + j0 + b) : -1;
-            w[b] = at[b] >= 0 ? load_weight(p.w, p.w_dtype, t * p.k + j0 + b) : 0.f;
-        }
+        for (int b = 0; b < kBatch; ++b) dot[b] = 0.f;
         for (int v = threadIdx.x; live && v < p.vecs; v += blockDim.x) {
             const Vec<T, N> g = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
             Vec<T, N> rows[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b)
-                if (at[b] >= 0) rows[b] = load_vec<T, N>(p.y, at[b] * p.ldy + (int64_t)v * N);
+                if (j0 + b < p.k) rows[b] = load_vec<T, N>(p.y, max(s.at[b], 0) * p.ldy + (int64_t)v * N);
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                if (at[b] < 0) continue;
+                if (s.at[b] < 0) continue;
                 Vec<T, N> o;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float gi = to_f32(g.v[i]);
                     dot[b] = fmaf(gi, to_f32(rows[b].v[i]), dot[b]);
-                    o.v[i] = from_f32<T>(w[b] * gi);
+                    o.v[i] = from_f32<T>(s.w[b] * gi);
                 }
-                store_vec<T, N>(p.out, at[b] * p.ldo + (int64_t)v * N, o);
+                store_vec<T, N>(p.out, s.at[b] * p.ldo + (int64_t)v * N, o);
             }
         }
 #pragma unroll
@@ -355,7 +413,7 @@ extern "C" int p2p_moe_sort(const void* ids, int ids_bytes, int64_t n_pairs, int
     const int64_t want = (n_pairs / ctas / 8 + 31) / 32 * 32;
     if (threads < want) threads = want < kSortThreads ? (int)want : kSortThreads;
     // one histogram a warp: fewer warps where the experts are many
-    const size_t smem = ((size_t)(threads / 32) + 1) * experts * sizeof(int);
+    const size_t smem = ((size_t)(threads / 32) + 2) * experts * sizeof(int);
     const void* fn = ids_bytes == 4 ? (const void*)sort_kernel<int32_t> : (const void*)sort_kernel<int64_t>;
     if (int e = allow_smem(fn, (int)smem, "p2p_moe_sort")) return e;
     cudaLaunchConfig_t cfg = {};
