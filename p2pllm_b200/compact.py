@@ -105,6 +105,7 @@ class Tiles:
     def __init__(self, blocks: list, layout: str | None = None):
         if not blocks:
             raise P2PError("a module needs at least one row block")
+        self.int4 = None
         if any(b[0] == "int4" for b in blocks):
             self._init_int4(blocks, layout)
             return
@@ -156,8 +157,8 @@ class Tiles:
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [T, cols] @ W.T: [T, rows]. Any T (the reference launches at most 64 tokens at a time)."""
-        if self.layout == "int4":
-            return self.int4.mm(x, out=out)
+        if self.int4 is not None:
+            return self.int4.mm(x, out)
         if x.dtype != self.dtype:
             raise P2PError(f"x is {x.dtype}, the weights {self.dtype}")
         if self.layout == "mask":

@@ -112,6 +112,7 @@ class Layout:
         nbytes = _lib.load().p2p_int4_layout_bytes(self.experts, self.rows, cols, group, self.has_zeros, gated)
         if nbytes < 0:
             raise P2PError(f"a gated module has as many gate rows as up rows, not {self.rows} in all")
+        self._op = _lib.ops().int4_mm
         self.data = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         codes, scales, zeros = codes.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
         with torch.cuda.device(self.device):
@@ -132,9 +133,13 @@ class Layout:
 
     def mm(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [T, cols] W^T: [T, rows], gated [T, rows / 2] (p2p_int4_mm through the torch operator)."""
+        if out is None and x.dtype is self.dtype:
+            try:                                               # the operator makes the same checks, at less cost
+                return self._op(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated)
+            except RuntimeError:
+                self.check_x(x)
+                raise
         self.check_x(x)
-        if out is None:
-            return _lib.ops().int4_mm(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated)
         from .kernels import _out
         out = _out(out, (x.shape[0], self.rows // 2 if self.gated else self.rows), x)
         _lib.ops().int4_mm_into(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated, out)

@@ -114,7 +114,7 @@ def route(ids: torch.Tensor, experts: int) -> dict:
     return {"order": order[:pairs], "where": where[:n], "counts": counts, "items": items[:n_items], "most": most}
 
 
-@dataclass(frozen=True)
+@dataclass
 class TokenOrder:
     """A pass's routed (token, slot) pairs sorted by expert, those of one expert in their own order; all on the GPU.
     Of the T K places the first offsets[-1] hold a pair."""
@@ -156,14 +156,22 @@ def _check_rows(t: torch.Tensor, order: TokenOrder, rows: int) -> None:
 def to_experts(x: torch.Tensor, order: TokenOrder) -> torch.Tensor:
     """[T K, H]: x's rows in the order's places, zero behind the last pair. bfloat16, float16 or float32. The gradient
     of x is the sum over its slots, in slot order and fp32."""
-    _check_rows(x, order, order.tokens)
-    return _lib.ops().moe_spread(x, order.where, order.offsets, order.topk)
+    try:                                            # the operator makes the same checks, at less cost
+        return _lib.ops().moe_spread(x, order.where, order.offsets, order.topk)
+    except RuntimeError:
+        _check_rows(x, order, order.tokens)
+        raise
 
 
 def from_experts(y: torch.Tensor, order: TokenOrder, weights: torch.Tensor | None = None) -> torch.Tensor:
     """[T, H]: per token the sum over its slots, in slot order and fp32, of weights[t, j] times the slot's row of
     y [T K, H] (no weights: 1); slots routed nowhere add nothing. Gradients for y (zero behind the last pair) and for
     weights [T, K] (bfloat16, float16 or float32)."""
+    if weights is None or weights.dim() == 2:
+        try:                                        # the operator makes the same checks, at less cost
+            return _lib.ops().moe_sum(y, order.where, order.offsets, weights, order.topk)
+        except RuntimeError:
+            pass
     _check_rows(y, order, order.tokens * order.topk)
     if weights is not None:
         require_cuda(weights)
@@ -188,24 +196,31 @@ class Int4Experts:
         if self.int4.experts > 1024:
             raise P2PError(f"{self.int4.experts} experts: 1 to 1024")
         self.gated, self.experts = gated, self.int4.experts
+        self._op = _lib.ops().int4_grouped
         self.rows, self.cols, self.dtype, self.device = (self.int4.rows, self.int4.cols, self.int4.dtype,
                                                          self.int4.device)
 
     def __call__(self, x: torch.Tensor, order: TokenOrder, gather: bool = False,
                  out: torch.Tensor | None = None) -> torch.Tensor:
         q = self.int4
-        q.check_x(x)
-        pairs = order.tokens * order.topk
-        _check_rows(x, order, order.tokens if gather else pairs)
+        if out is None and x.dtype is q.dtype:
+            try:                                    # the operator makes the same checks, at less cost
+                return self._op(x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order,
+                                order.where, order.offsets, order.items, order.n_items, order.topk, gather)
+            except RuntimeError:
+                self._check(x, order, gather)
+                raise
+        self._check(x, order, gather)
+        out = kernels._out(out, (order.tokens * order.topk, q.rows // 2 if q.gated else q.rows), x)
+        _lib.ops().int4_grouped_into(x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order,
+                                     order.where, order.offsets, order.items, order.n_items, order.topk, gather, out)
+        return out
+
+    def _check(self, x: torch.Tensor, order: TokenOrder, gather: bool) -> None:
+        self.int4.check_x(x)
+        _check_rows(x, order, order.tokens if gather else order.tokens * order.topk)
         if order.experts != self.experts:
             raise P2PError(f"an order of {order.experts} experts, weights of {self.experts}")
-        args = (x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order, order.where,
-                order.offsets, order.items, order.n_items, order.topk, gather)
-        if out is None:
-            return _lib.ops().int4_grouped(*args)
-        out = kernels._out(out, (pairs, q.rows // 2 if q.gated else q.rows), x)
-        _lib.ops().int4_grouped_into(*args, out)
-        return out
 
     def nbytes(self) -> int:
         return self.int4.nbytes()

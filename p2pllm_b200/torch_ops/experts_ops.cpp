@@ -148,6 +148,14 @@ int64_t max_items(int64_t pairs, int64_t experts) {
     return std::min(pairs, (pairs + most - 1) / most + experts);
 }
 
+// all[begin .. begin + n) as a tensor of its own on the same storage, without a trip through the dispatcher.
+at::Tensor part(const at::Tensor& all, int64_t begin, int64_t n) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(all.storage_offset() + begin);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& ids_in, int64_t experts) {
     TORCH_CHECK(ids_in.is_cuda(), "p2p_b200: CUDA tensors only (the replica path has no CPU fallback)");
     TORCH_CHECK(ids_in.scalar_type() == at::kInt || ids_in.scalar_type() == at::kLong, "p2p_b200: ids are int32 or int64");
@@ -157,9 +165,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(
     const int64_t n = ids.numel(), most = std::max<int64_t>(max_items(n, experts), 1);
     // one allocation: items (16-byte aligned), order, where, offsets, n_items
     at::Tensor all = at::empty({4 * most + 2 * n + experts + 2}, ids.options().dtype(at::kInt));
-    at::Tensor items = all.narrow(0, 0, 4 * most), order = all.narrow(0, 4 * most, n),
-               where = all.narrow(0, 4 * most + n, n), offsets = all.narrow(0, 4 * most + 2 * n, experts + 1),
-               n_items = all.narrow(0, 4 * most + 2 * n + experts + 1, 1);
+    at::Tensor items = part(all, 0, 4 * most), order = part(all, 4 * most, n), where = part(all, 4 * most + n, n),
+               offsets = part(all, 4 * most + 2 * n, experts + 1),
+               n_items = part(all, 4 * most + 2 * n + experts + 1, 1);
     check(p2p_moe_sort(ids.data_ptr(), (int)ids.element_size(), n, (int)experts, order.data_ptr<int32_t>(),
                        where.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), items.data_ptr<int32_t>(), most,
                        (int)item_tokens(n, experts), n_items.data_ptr<int32_t>(), stream_of(ids)),
@@ -190,8 +198,9 @@ void check_sum(const at::Tensor& y, const at::Tensor& where, const std::optional
     check_matrix(y, "y");
     TORCH_CHECK(topk >= 1 && where.numel() % topk == 0 && y.size(0) == where.numel(), "p2p_b200: y has ", y.size(0),
                 " rows, the order is of ", where.numel(), " pairs, ", topk, " a token");
-    TORCH_CHECK(!weights || (weights->device() == y.device() && weights->numel() == where.numel()),
-                "p2p_b200: weights are not ", where.numel(), " on ", y.device());
+    TORCH_CHECK(!weights || (weights->device() == y.device() && weights->dim() == 2 && weights->size(1) == topk &&
+                             weights->numel() == where.numel()),
+                "p2p_b200: weights are not [", where.numel() / topk, ", ", topk, "] on ", y.device());
 }
 
 at::Tensor moe_sum(const at::Tensor& y_in, const at::Tensor& where, const at::Tensor&,
