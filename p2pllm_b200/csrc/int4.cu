@@ -551,7 +551,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
 // a time, a thread four rows.
 template <typename T> __global__ void __launch_bounds__(256) int4_small_join_kernel(const __grid_constant__ SmallParams p, int ctas) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (p.items) asm volatile("griddepcontrol.wait;" ::: "memory");  // the items may be the kernel's before the last
+    // Every block waits, those without work too: this kernel's end stands for the end of the one before.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tile = blockIdx.x, tiles = small_tiles(p);
     if (tile >= tiles) return;
     const uint32_t units_all = (uint32_t)(tiles * p.units), a = (uint32_t)(tile * p.units);
@@ -565,7 +566,6 @@ template <typename T> __global__ void __launch_bounds__(256) int4_small_join_ker
     const float* part = p.partial + ((int64_t)b0 * 2 + (runs.begin(b0) >= a ? 0 : 1)) * size + lane * 4;
     const float* next = p.partial + (int64_t)(b0 + 1) * 2 * size + lane * 4;
     T* y = reinterpret_cast<T*>(p.y);
-    if (!p.items) asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int tok = threadIdx.x >> 5; tok < t.n; tok += 8) {
         float4 sum = __ldcg(reinterpret_cast<const float4*>(part + tok * 128));
 #pragma unroll 4

@@ -604,6 +604,8 @@ template <typename T> __global__ void __launch_bounds__(256) int4_join_kernel(co
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const q4::Runs runs((uint32_t)(p.row_tiles * p.token_tiles * p.units), (uint32_t)p.ctas, 1u);
     const uint32_t a = blockIdx.x * (uint32_t)p.units, b0 = runs.of(a), b1 = runs.of(a + p.units - 1);
+    // Every block waits, those without work too: this kernel's end stands for the end of the one before.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (b0 == b1) return;                                // one run wrote y itself
     const Tile t = tile_at(p, (int)a, (int)a + p.units);
     const int lane = threadIdx.x & 31, last = min(t.n, (int)(blockIdx.y + 1) * kJoinTokens);
@@ -611,7 +613,6 @@ template <typename T> __global__ void __launch_bounds__(256) int4_join_kernel(co
     const float* part = p.partial + ((int64_t)b0 * 2 + (runs.begin(b0) >= a ? 0 : 1)) * p.n_max * 128 + lane * 4;
     const float* next = p.partial + (int64_t)(b0 + 1) * 2 * p.n_max * 128 + lane * 4;
     T* y = reinterpret_cast<T*>(p.y);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll 2
     for (int tok = blockIdx.y * kJoinTokens + (threadIdx.x >> 5); tok < last; tok += 8) {
         float4 sum = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)tok * 128));

@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, kernels
 from ._lib import P2PError, call, dtype_code, ptr, require_cuda, stream_of
 
 __all__ = ["GROUPS", "quantize", "expand", "Layout"]
@@ -135,14 +135,16 @@ class Layout:
         """x [T, cols] W^T: [T, rows], gated [T, rows / 2] (p2p_int4_mm through the torch operator)."""
         if out is None and x.dtype is self.dtype:
             try:                                               # the operator makes the same checks, at less cost
-                return self._op(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated)
+                out = self._op(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated)
             except RuntimeError:
                 self.check_x(x)
                 raise
-        self.check_x(x)
-        from .kernels import _out
-        out = _out(out, (x.shape[0], self.rows // 2 if self.gated else self.rows), x)
-        _lib.ops().int4_mm_into(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated, out)
+        else:
+            self.check_x(x)
+            out = kernels._out(out, (x.shape[0], self.rows // 2 if self.gated else self.rows), x)
+            _lib.ops().int4_mm_into(x, self.data, self.has_zeros, self.rows, self.cols, self.group, self.gated, out)
+        if kernels.CHECK_WAITS:
+            kernels.int4_status(x.device)
         return out
 
     def nbytes(self) -> int:

@@ -404,6 +404,14 @@ def spmm_tc_status(device=None, reset: bool = True) -> None:
         raise
 
 
+def int4_status(device=None, reset: bool = True) -> None:
+    """Raises if a 4-bit product gave up waiting on its pipeline since the last reset; that launch's output is undefined.
+    Syncs. (Its workspaces belong to one call each, so none needs zeroing.)"""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        call("p2p_int4_status", int(reset), torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _ptr_array(ts) -> ctypes.Array:
     arr = (ctypes.c_void_p * len(ts))()
     for i, t in enumerate(ts):

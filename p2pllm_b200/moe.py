@@ -205,15 +205,19 @@ class Int4Experts:
         q = self.int4
         if out is None and x.dtype is q.dtype:
             try:                                    # the operator makes the same checks, at less cost
-                return self._op(x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order,
-                                order.where, order.offsets, order.items, order.n_items, order.topk, gather)
+                out = self._op(x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order,
+                               order.where, order.offsets, order.items, order.n_items, order.topk, gather)
             except RuntimeError:
                 self._check(x, order, gather)
                 raise
-        self._check(x, order, gather)
-        out = kernels._out(out, (order.tokens * order.topk, q.rows // 2 if q.gated else q.rows), x)
-        _lib.ops().int4_grouped_into(x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated, order.order,
-                                     order.where, order.offsets, order.items, order.n_items, order.topk, gather, out)
+        else:
+            self._check(x, order, gather)
+            out = kernels._out(out, (order.tokens * order.topk, q.rows // 2 if q.gated else q.rows), x)
+            _lib.ops().int4_grouped_into(x, q.data, q.has_zeros, q.experts, q.rows, q.cols, q.group, q.gated,
+                                         order.order, order.where, order.offsets, order.items, order.n_items,
+                                         order.topk, gather, out)
+        if kernels.CHECK_WAITS:
+            kernels.int4_status(x.device)
         return out
 
     def _check(self, x: torch.Tensor, order: TokenOrder, gather: bool) -> None:

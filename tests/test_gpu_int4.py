@@ -166,6 +166,31 @@ def test_results_do_not_depend_on_the_launch():
     assert all(torch.equal(y, want) for y in ys + here)
 
 
+@pytest.mark.parametrize("tokens", [1, 8, 17, 40, 150])
+@pytest.mark.parametrize("sizes", [(128, 640, 128, 96), (640, 100, 2048, 130), (64, 4096, 4096, 64)])
+def test_modules_in_a_chain_read_what_the_one_before_wrote(tokens, sizes):
+    """Each launch may begin before the one before has ended, joins of row tiles that no two runs share among them: the
+    results are those of launches that wait."""
+    g = _gen(tokens + sizes[1])
+    chain = [compact.Tiles([_block((), r, c, 64, False, torch.bfloat16, g)]) for c, r in zip(sizes, sizes[1:])]
+    x = torch.randn(tokens, sizes[0], generator=g, device="cuda").bfloat16()
+    norm = lambda y: (y.float() / y.float().abs().amax().clamp(min=1)).bfloat16()
+
+    def run(wait):
+        y = x
+        for tiles in chain:
+            y = tiles(y)
+            y = tiles(y[:, :tiles.cols]) if y.shape[1] >= tiles.cols else y      # straight after each other
+            if wait:
+                torch.cuda.synchronize()
+            y = norm(y)
+        return y
+    want = run(True)
+    assert all(torch.equal(run(False), want) for _ in range(10))
+    from p2pllm_b200 import kernels
+    kernels.int4_status()
+
+
 def test_two_captured_graphs_replay_side_by_side():
     g = _gen(4)
     tiles = compact.Tiles([_block((), 4096, 4096, 128, False, torch.bfloat16, g)])
