@@ -203,9 +203,18 @@ class GatedTiles:
     """A gated MLP's gate and up projections as one tensor-core module whose GEMM also applies the gate: calling it on
     x [T, cols] returns dtype(silu(g) * u) [T, R], g and u being the projections' outputs rounded to the model dtype
     -- what SGLang's SiluAndMul makes of the gate_up projection's output, without writing it (p2p/compact.py:205-224
-    multiplies the two projections; the activation is the model's own). Blocks: the gate rows, then the up rows."""
+    multiplies the two projections; the activation is the model's own). Blocks: the gate rows, then the up rows. Of
+    4-bit blocks, which take any number of rows and columns, g and u are the unrounded fp32 sums."""
 
     def __init__(self, blocks: list):
+        self.int4 = None
+        if any(b[0] == "int4" for b in blocks):
+            if any(b[0] != "int4" or b[1].dim() != 2 for b in blocks):
+                raise P2PError("4-bit blocks make up a whole module, in the layout \"int4\", of 2-D blocks")
+            self.int4 = int4.Layout(blocks, gated=True)
+            self.layout, self.rows, self.layout_rows = "int4", self.int4.rows // 2, self.int4.rows
+            self.cols, self.dtype, self.device = self.int4.cols, self.int4.dtype, self.int4.device
+            return
         values, idx = gate_up_rows(blocks)
         self.cols = _cols(to_compact(blocks[0]))
         self.dtype, self.device = values.dtype, values.device
@@ -215,11 +224,15 @@ class GatedTiles:
         self.words, self.seg, self.seg_cap = kernels.tiles_build([(0, values, idx)], self.cols)
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        if self.int4 is not None:
+            return self.int4.mm(x, out)
         if x.dtype != self.dtype:
             raise P2PError(f"x is {x.dtype}, the weights {self.dtype}")
         return kernels.spmm_tc_gated(x, self.words, self.seg, self.layout_rows, self.cols, self.seg_cap, out=out)
 
     def nbytes(self) -> int:
+        if self.int4 is not None:
+            return self.int4.nbytes()
         return self.words.numel() * 4 + self.seg.numel() * 8
 
 

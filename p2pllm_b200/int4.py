@@ -87,7 +87,11 @@ def expand(block: tuple, experts=None) -> torch.Tensor:
 class Layout:
     """Row blocks of one module (or, with a leading expert dimension, of one routed-expert tensor) in the layout of
     csrc/int4.cuh, built once at load. gated: the first half of the rows is the gate, the second half the up
-    projection, and the products return silu(gate) * up."""
+    projection, and the products return silu(gate) * up.
+
+    The products add a group's codes times x in fp32 and scale that sum, so the sum itself (up to 15 times the group's
+    absolute x) has to stay below fp32's largest value. They may read the weights before the stream's previous kernel
+    has ended: who rewrites `data` on the GPU waits for that (as building it does) before the next product."""
 
     def __init__(self, blocks: list, gated: bool = False):
         if not blocks:

@@ -1,9 +1,12 @@
 """Products with 4-bit weights (compact.Tiles on "int4" blocks, moe.Int4Experts, the 4-bit moe.GroupedMoE, 4-bit
 replica files) against plain 64-bit arithmetic on the codes.
 
-Bound of one output: half a step of its type, plus the fp32 sums'. A product's sum is a chain of at most 3 additions a
-16-column step inside a group of 64, one addition a group of a warp's column blocks and one a warp: below 64 + cols / 256
-additions, each off by at most 2^-23 of the terms' absolute sum."""
+Bound of one output: half a step of its type, plus the fp32 sums', in units of 2^-23 of the terms' absolute sum. Inside a
+group: at most 8 steps of 16 columns, 3 additions a step, each off by one unit at most (tensor cores may cut off): 24.
+Then a chain of one fused multiply-add a group, each rounded to nearest, half a unit: at most cols / 32 of them, cols / 64
+units; and of one addition a run of units that a row tile is cut into, at most cols / 128 of them and a few of the column
+halves: cols / 256 + 4 units. 24 + 4 is below the 64 kept here: 64 + cols / 64 + cols / 256. (64 + cols / 256 before left out
+the chain over groups, which a kernel that adds every group of a row tile one after another has.)"""
 from typing import NamedTuple
 
 import numpy as np
@@ -38,7 +41,7 @@ def _dense64(block):
 
 
 def _sum_bound(x, w):
-    return (64 + w.shape[-1] / 256) * 2.0 ** -23 * (x.abs() @ w.abs().mT)
+    return (64 + w.shape[-1] / 64 + w.shape[-1] / 256) * 2.0 ** -23 * (x.abs() @ w.abs().mT)
 
 
 def _half_step(want, dtype):
@@ -96,6 +99,25 @@ def test_blocks_of_a_module_are_its_rows_in_order():
     tiles = compact.Tiles(blocks)
     assert (tiles.layout, tiles.rows, tiles.cols) == ("int4", 93, 200) and tiles.nbytes() > 0
     _check_product(tiles(x), x, torch.cat([_dense64(b) for b in blocks]), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("tokens,half,cols", [(1, 1, 1), (1, 40, 130), (7, 64, 257), (9, 100, 1000), (17, 640, 96),
+                                              (32, 33, 2048), (33, 100, 640), (100, 129, 321), (200, 70, 1030),
+                                              (272, 4096, 256), (300, 33, 130)])
+def test_gate_and_up_in_one_module(tokens, half, cols, group, zeros, dtype):
+    g = _gen(tokens * 10007 + half)
+    blocks = [_block((), half, cols, group, z, DT[dtype], g) for z in (zeros, False)]
+    x = (torch.randn(tokens, cols, generator=g, device="cuda") / cols ** 0.5).to(DT[dtype])
+    tiles = compact.GatedTiles(blocks)
+    assert (tiles.layout, tiles.rows, tiles.cols) == ("int4", half, cols) and tiles.nbytes() > 0
+    w = torch.cat([_dense64(b) for b in blocks])
+    y = tiles(x)
+    assert y.shape == (tokens, half) and y.dtype == DT[dtype]
+    _check_gated(y, x, w, DT[dtype])
+    out = torch.full((tokens, half + 3), 7.0, dtype=DT[dtype], device="cuda")
+    assert torch.equal(tiles(x, out=out[:, 1:-2]), y) and bool((out[:, 0] == 7).all()) and bool((out[:, -2:] == 7).all())
 
 
 @pytest.mark.parametrize("cols,pad,offset", [(128, 8, 0), (128, 3, 0), (128, 8, 1), (127, 1, 0), (96, 0, 4), (100, 4, 2)])
@@ -429,7 +451,9 @@ def test_calls_that_do_not_fit_are_refused():
     with pytest.raises(P2PError, match="same columns"):
         compact.Tiles([block, _block((), 4, 64, 64, True, torch.bfloat16, g)])
     with pytest.raises(P2PError, match="whole module"):
-        compact.GatedTiles([block])
+        compact.GatedTiles([block, ("dense", torch.zeros(32, 128, dtype=torch.bfloat16, device="cuda"))])
+    with pytest.raises(P2PError, match="gate rows"):
+        compact.GatedTiles([_block((), 33, 128, 64, True, torch.bfloat16, g)])
     kind, codes, scales, zeros, cols, group = block
     for bad, needle in (((kind, codes[:, 1:], scales, zeros, cols, group), "do not hold"),
                         ((kind, codes, scales[:, 1:], zeros, cols, group), "wanted"),
