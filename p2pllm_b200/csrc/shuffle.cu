@@ -5,6 +5,9 @@
 //   p2p_moe_sum      out[t] = sum_j w[t, j] y[where[t K + j]], fp32 in slot order (w = 1: the gradient of the spread)
 //   p2p_moe_sum_back dy[where[t K + j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], y[where[t K + j]]>
 //
+// The row kernels are bound by the memory: 8192 tokens x 8 rows of 4 KB: spread 302 MB in 49 us (6.1 TB/s), sum the same in
+// 55 us (5.5 TB/s), its gradient 604 MB in 94 us (6.4 TB/s). The sort of those 65536 pairs is bound by latency: 17 us.
+//
 // Rows of an order are `pairs` long whatever the routing: behind the last routed pair order is -1 and rows are zero.
 // p2p/compact.py:241-256 leaves all of this to SGLang's fused MoE.
 #include "sm100.cuh"
@@ -173,7 +176,43 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
 
 // --- rows there and back: vectors of N elements of T, 16 bytes where every row allows it, else one element -------------
 
-template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+// 16-bit values stay in pairs: kept one by one they took the sum's kernel past its registers.
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec {
+    using Word = std::conditional_t<N == 1, T, uint32_t>;
+    static constexpr int kPer = sizeof(Word) / sizeof(T);
+    Word v[N / kPer];
+    __device__ __forceinline__ void to(float (&f)[N]) const {
+        if constexpr (kPer == 2) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const float2 u = unpack2<T>(v[i]);
+                f[2 * i] = u.x;
+                f[2 * i + 1] = u.y;
+            }
+        } else if constexpr (N == 1) {
+            f[0] = to_f32(v[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = __uint_as_float(v[i]);
+        }
+    }
+    __device__ __forceinline__ void from(const float (&f)[N]) {
+        if constexpr (kPer == 2) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const T pair[2] = {from_f32<T>(f[2 * i]), from_f32<T>(f[2 * i + 1])};
+                uint16_t bits[2];
+                memcpy(bits, pair, 4);
+                v[i] = (uint32_t)bits[0] | (uint32_t)bits[1] << 16;
+            }
+        } else if constexpr (N == 1) {
+            v[0] = from_f32<T>(f[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __float_as_uint(f[i]);
+        }
+    }
+};
 
 struct RowParams {
     const void *x, *y;                               // [tokens, hidden] (x, or dout) and [pairs, hidden]
@@ -207,42 +246,53 @@ template <typename T, int N> __device__ __forceinline__ void store_vec(void* p, 
 template <typename T, int N> __device__ __forceinline__ void zero_behind(const RowParams& p) {
     const int threads = blockDim.x * blockDim.y, last = *p.last;
     const int64_t pairs = (int64_t)p.tokens * p.k, n = (pairs - last) * p.vecs;
+    const float none[N] = {};
     Vec<T, N> zero;
-#pragma unroll
-    for (int i = 0; i < N; ++i) zero.v[i] = from_f32<T>(0.f);
+    zero.from(none);
     for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * threads + threadIdx.y * blockDim.x + threadIdx.x;
          i < n; i += (int64_t)gridDim.x * gridDim.y * threads)
         store_vec<T, N>(p.out, (last + i / p.vecs) * p.ldo + i % p.vecs * N, zero);
 }
 
 constexpr int kBatch = 4;                            // slots whose rows a thread holds at a time: eight cost half the blocks
-                                                     // an SM (8192 x 8 rows of 4 KB: gradient 128 us to 98)
+                                                     // an SM (8192 x 8 rows of 4 KB: gradient 128 us, four 98)
 constexpr int kRowThreads = 256;
 
-// The places (-1: nowhere) and weights of slots j0.. of token t, which every lane of its warp gets: one load a warp.
+// A token's places (-1: nowhere) and weights, a slot a lane: one load a warp for 32 slots, dealt out by shuffles. (A load a
+// batch puts more trips to memory in a row. With it and the pairs of Vec, 8192 x 8 rows of 4 KB: weighted sum 68 us to
+// 55, gradient 98 to 94.)
 template <int N> struct Slots { int at[N]; float w[N]; };
-template <int N> __device__ __forceinline__ Slots<N> load_slots(const RowParams& p, int64_t t, int j0, bool live) {
-    const int lane = threadIdx.x & 31;
-    const bool in = live && lane < N && j0 + lane < p.k;
-    const int64_t i = t * p.k + j0 + lane;
-    const int at = in ? __ldcg(p.where + i) : -1;
-    const float w = in && p.w ? load_weight(p.w, p.w_dtype, i) : 1.f;
-    Slots<N> s;
-#pragma unroll
-    for (int b = 0; b < N; ++b) {
-        s.at[b] = __shfl_sync(0xffffffffu, at, b);
-        s.w[b] = __shfl_sync(0xffffffffu, w, b);
+struct LaneSlots {
+    int at;
+    float w;
+    // of slots j0 / 32 * 32.. of token t, when j0 is the first of 32
+    __device__ __forceinline__ void load(const RowParams& p, int64_t t, int j0, bool live) {
+        if (j0 % 32) return;
+        const int j = j0 + (threadIdx.x & 31);
+        const bool in = live && j < p.k;
+        const int64_t i = t * p.k + j;
+        at = in ? __ldcg(p.where + i) : -1;
+        w = in && p.w ? load_weight(p.w, p.w_dtype, i) : 1.f;
     }
-    return s;
-}
+    template <int N> __device__ __forceinline__ Slots<N> batch(int j0) const {
+        Slots<N> s;
+#pragma unroll
+        for (int b = 0; b < N; ++b) {
+            s.at[b] = __shfl_sync(0xffffffffu, at, (j0 + b) & 31);
+            s.w[b] = __shfl_sync(0xffffffffu, w, (j0 + b) & 31);
+        }
+        return s;
+    }
+};
 
 template <typename T, int N> __global__ void __launch_bounds__(kRowThreads) spread_kernel(const RowParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    for (int j0 = 0; j0 < p.k; j0 += kBatch) {
-        const Slots<kBatch> s = load_slots<kBatch>(p, t, j0, t < p.tokens);
-        if (t >= p.tokens) break;
+    LaneSlots mine;
+    for (int j0 = 0; j0 < p.k && t < p.tokens; j0 += kBatch) {       // a warp's rows are one token's
+        mine.load(p, t, j0, true);
+        const Slots<kBatch> s = mine.batch<kBatch>(j0);
         for (int v = blockIdx.y * blockDim.x + threadIdx.x; v < p.vecs; v += gridDim.y * blockDim.x) {
             const Vec<T, N> val = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
 #pragma unroll
@@ -260,7 +310,8 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) s
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (t >= p.tokens) return;
     const int lane = threadIdx.x & 31;
-    Slots<kBatch> s = load_slots<kBatch>(p, t, 0, true);
+    LaneSlots mine;
+    mine.load(p, t, 0, true);
     // whole warps go round, so that all lanes of one are there when it loads its slots
     for (int v0 = blockIdx.y * blockDim.x + threadIdx.x - lane; v0 < p.vecs; v0 += gridDim.y * blockDim.x) {
         const bool on = v0 + lane < p.vecs;
@@ -269,7 +320,8 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) s
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.f;
         for (int j0 = 0; j0 < p.k; j0 += kBatch) {
-            if (p.k > kBatch) s = load_slots<kBatch>(p, t, j0, true);
+            if (p.k > 32) mine.load(p, t, j0, true);
+            const Slots<kBatch> s = mine.batch<kBatch>(j0);
             Vec<T, N> rows[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b)
@@ -277,14 +329,15 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) s
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 if (s.at[b] < 0) continue;
+                float row[N];
+                rows[b].to(row);
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] = fmaf(s.w[b], to_f32(rows[b].v[i]), acc[i]);
+                for (int i = 0; i < N; ++i) acc[i] = fmaf(s.w[b], row[i], acc[i]);
             }
         }
         if (!on) continue;
         Vec<T, N> o;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o.v[i] = from_f32<T>(acc[i]);
+        o.from(acc);
         store_vec<T, N>(p.out, t * p.ldo + col, o);
     }
 }
@@ -297,13 +350,16 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) s
     const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int lane = threadIdx.x & 31, row_warps = blockDim.x >> 5, row_warp = threadIdx.x >> 5;
     const bool live = t < p.tokens;
+    LaneSlots mine;
     for (int j0 = 0; j0 < p.k; j0 += kBatch) {
-        const Slots<kBatch> s = load_slots<kBatch>(p, t, j0, live);
+        mine.load(p, t, j0, live);
+        const Slots<kBatch> s = mine.batch<kBatch>(j0);
         float dot[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) dot[b] = 0.f;
         for (int v = threadIdx.x; live && v < p.vecs; v += blockDim.x) {
-            const Vec<T, N> g = load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N);
+            float grad[N];
+            load_vec<T, N>(p.x, t * p.ldx + (int64_t)v * N).to(grad);
             Vec<T, N> rows[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b)
@@ -311,13 +367,15 @@ template <typename T, int N> __global__ void __launch_bounds__(kRowThreads, 4) s
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 if (s.at[b] < 0) continue;
-                Vec<T, N> o;
+                float row[N], scaled[N];
+                rows[b].to(row);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float gi = to_f32(g.v[i]);
-                    dot[b] = fmaf(gi, to_f32(rows[b].v[i]), dot[b]);
-                    o.v[i] = from_f32<T>(s.w[b] * gi);
+                    dot[b] = fmaf(grad[i], row[i], dot[b]);
+                    scaled[i] = s.w[b] * grad[i];
                 }
+                Vec<T, N> o;
+                o.from(scaled);
                 store_vec<T, N>(p.out, s.at[b] * p.ldo + (int64_t)v * N, o);
             }
         }

@@ -79,7 +79,7 @@ def test_order_of_lopsided_and_foreign_ids():
 
 
 CASES = [(1, 1, 1, 1), (1, 8, 128, 2048), (3, 2, 4, 7), (17, 8, 16, 64), (40, 3, 5, 129), (33, 9, 20, 96),
-         (5, 20, 8, 1000), (272, 8, 128, 512), (1300, 8, 64, 136), (2, 2, 3, 9000), (0, 2, 3, 16)]
+         (5, 20, 8, 1000), (6, 40, 64, 300), (9, 75, 16, 16), (272, 8, 128, 512), (1300, 8, 64, 136), (2, 2, 3, 9000), (0, 2, 3, 16)]
 
 
 def _half(want, dtype):
