@@ -6,19 +6,29 @@
 // scaled weight rounded to bf16 would double the squared error of the result). A CTA, one an SM, takes a contiguous run
 // of units (128 rows x 128 columns), row tile after row tile:
 //
-//   warp 16 (weights)   streams the run's records, 8.4 KB a unit and one linear range of the layout a row tile, into
+//   warps 0-3, 4-7      read the even and the odd pieces' accumulators out, group after group, acc += scale * sum (packed
+//                       fp32 pairs), while other pieces multiply, and write the finished row tile: y itself,
+//                       silu(gate) * up of it, or, where the tile is shared with the neighbouring run, an fp32 partial
+//                       that int4_join_kernel adds in run order
+//   from warp 8 (build) a warp turns the codes of one 16-row block (of two above 160 tokens) into bf16 / f16 integers and
+//                       stores them into the unit's A tile in tensor memory (two tcgen05.st.16x256b.x4 a block: the
+//                       layout is that store's order): 16 warps, two groups on alternate units, up to 64 tokens, where
+//                       the codes' turn binds; 8 up to 160; 4 above, where the accumulators take the registers
+//   weights             streams the run's records, 8.4 KB a unit and one linear range of the layout a row tile, into
 //                       rings in shared memory by bulk copies (codes and zero points in one, scales, which are used
 //                       later, in another), ahead of the previous kernel's end and up to 12 units ahead of their use
-//   warp 17 (x)         TMA of each unit's x tile [tokens x 128] (two 64-column boxes, 128-byte swizzle)
-//   warps 8-15 (build)  warp w turns the codes of one 16-row block into bf16 / f16 integers and stores them into the
-//                       unit's A tile in tensor memory (two tcgen05.st.16x256b.x4: the layout is that store's order)
+//   x                   TMA of each unit's x tile [tokens x 128] (two 64-column boxes, 128-byte swizzle)
 //   two warps (MMA)     one thread each issues tcgen05.mma kind::f16, A from TMEM, M = 128: a group's columns times a
 //                       piece of the tokens (quarters, halves, or all of few) into a zeroed accumulator, then a commit.
 //                       The warps take the even and the odd pieces, or of a single piece alternate units: a look at a
 //                       barrier costs an issuing thread 130 cycles even when it has nothing to wait for
-//   warps 0-3, 4-7      read the even and the odd pieces' accumulators out, group after group, acc += scale * sum
-//                       (packed fp32 pairs), while other pieces multiply, and write the finished row tile: y itself, silu(gate) * up of it, or, where the tile
-//                       is shared with the neighbouring run, an fp32 partial that int4_join_kernel adds in run order
+//
+// Measured (bf16, groups of 128): 28672 x 4096 at 272 tokens 80 us replayed from a graph (798 TFLOP/s; the product alone
+// would take 39 us at the measured rate); 128 experts of 1536 x 2048 on 2048 x 8 tokens 238 us (433 TFLOP/s; items are
+// padded to 160 places). What binds is the way of a unit from hand to hand: its accumulator goes from products to commit,
+// read-out and release, with 130 to 220 cycles for each look at a barrier, and a row tile's way out in between. A unit takes
+// some 3,100 and 2,500 cycles where its products are 1,088 and 640: the tensor pipe is busy 37 % and 21 % of the time. It is
+// not x (half of its traffic, 6 TB/s from L2, gone: the same time) nor the builders (twice as many: the same).
 //
 // Every wait is bounded (2 s): a launch that gives up records where, issues nothing more, drains what it issued and
 // exits (p2p_int4_status reads the site).

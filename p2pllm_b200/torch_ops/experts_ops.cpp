@@ -15,7 +15,8 @@ using torch::autograd::variable_list;
 constexpr int64_t kSmallTokens = 8;                   // items of up to here pick x's rows by the order
 
 // Places of one item, what one pass over an expert's weights takes: somewhat more than experts have on average, so that
-// few take two passes and no tile is mostly empty; at most what leaves the accumulators room.
+// few take two passes and no tile is mostly empty; at most what leaves the accumulators room. (128 experts of 1536 x 2048
+// with 128 pairs each on average: 255 us in items of 160 places, x's rows picked once a tile; 303 us of 256 before.)
 int64_t item_tokens(int64_t pairs, int64_t experts) {
     const double mean = (double)pairs / experts;
     if (pairs <= kSmallTokens || mean <= 4) return kSmallTokens;

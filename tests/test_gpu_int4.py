@@ -213,6 +213,40 @@ def test_modules_in_a_chain_read_what_the_one_before_wrote(tokens, sizes):
     kernels.int4_status()
 
 
+def test_calls_from_several_threads_at_once():
+    """Threads on streams of their own, modules of both kernels and routed experts among them."""
+    import threading
+    g = _gen(77)
+    tiles = [compact.Tiles([_block((), r, c, 64, True, torch.bfloat16, g)]) for r, c in ((640, 2048), (4096, 1024))]
+    experts = moe.Int4Experts([_block((16,), 128, 512, 32, False, torch.bfloat16, g)], gated=True)
+    xs = [torch.randn(t, q.cols, generator=g, device="cuda").bfloat16() for q in tiles for t in (1, 17, 150)]
+    xe, ids = torch.randn(70, 512, generator=g, device="cuda").bfloat16(), torch.randint(-1, 16, (70, 3), generator=g, device="cuda")
+
+    def run():
+        ys = [q(x) for q, part in zip(tiles, (xs[:3], xs[3:])) for x in part]
+        order = moe.sort_tokens(ids, 16)
+        y = experts(xe, order, gather=True)
+        return ys + [y, moe.from_experts(y, order)]
+    want = run()
+    torch.cuda.synchronize()
+    got, failed = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = [run() for _ in range(10)]
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert all(torch.equal(a, b) for rounds in got.values() for ys in rounds for a, b in zip(ys, want))
+
+
 def test_two_captured_graphs_replay_side_by_side():
     g = _gen(4)
     tiles = compact.Tiles([_block((), 4096, 4096, 128, False, torch.bfloat16, g)])
