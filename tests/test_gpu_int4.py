@@ -521,3 +521,64 @@ def test_expert_calls_that_do_not_fit_are_refused():
         moe.GroupedMoE(None, {"w13_weight": [block], "w2_weight": [("dense", torch.zeros(4, 64, 16, dtype=torch.bfloat16, device="cuda"))]})
     with pytest.raises(P2PError, match="do not match"):
         moe.GroupedMoE(None, {"w13_weight": [block], "w2_weight": [block]})
+
+
+# --- nothing to do, and a lot -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [0, 1, 5, 60, 700])
+def test_no_pair_has_an_expert(tokens):
+    """Rows behind the last pair, which are all of them: zero, or in a given output as they were."""
+    g = _gen(21)
+    up = moe.Int4Experts([_block((4,), 64, 96, 32, True, torch.bfloat16, g)], gated=True)
+    x = torch.randn(tokens, 96, generator=g, device="cuda").bfloat16()
+    order = moe.sort_tokens(torch.full((tokens, 2), 4, device="cuda"), 4)
+    assert int(order.n_items) == 0 and bool((order.where == -1).all()) and bool((order.order == -1).all())
+    y = up(x, order, gather=True)
+    assert y.shape == (tokens * 2, 32) and bool((y == 0).all())
+    out = torch.full((tokens * 2, 32), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert bool((up(x, order, gather=True, out=out) == 7).all())
+    back = moe.from_experts(y, order, torch.ones(tokens, 2, device="cuda"))
+    assert back.shape == (tokens, 32) and bool((back == 0).all())
+    assert compact.Tiles([_block((), 10, 96, 32, True, torch.bfloat16, g)])(x[:0]).shape == (0, 10)
+
+
+def test_some_rows_of_a_given_output_stay():
+    g = _gen(22)
+    for tokens in (6, 400):
+        experts = moe.Int4Experts([_block((8,), 48, 128, 64, False, torch.float16, g)])
+        ids = _ids(tokens, 3, 8, g, nowhere=0.5)
+        order = moe.sort_tokens(ids, 8)
+        routed = int(order.offsets[-1])
+        x = torch.randn(tokens, 128, generator=g, device="cuda").half()
+        out = torch.full((tokens * 3, 48), 7.0, dtype=torch.float16, device="cuda")
+        y = experts(x, order, gather=True)
+        experts(x, order, gather=True, out=out)
+        assert torch.equal(out[:routed], y[:routed]) and bool((out[routed:] == 7).all()) and bool((y[routed:] == 0).all())
+
+
+def test_outputs_past_32_bits():
+    """y of 2.3e9 elements: its last rows are those of a call of their own."""
+    g = _gen(23)
+    block = _block((), 28672, 128, 128, False, torch.bfloat16, g)
+    x = torch.randn(80000, 128, generator=g, device="cuda").bfloat16()
+    tiles = compact.Tiles([block])
+    y = tiles(x)
+    _check_product(y[-40:], x[-40:], _dense64(block), torch.bfloat16)
+    _check_product(y[74880:74910], x[74880:74910], _dense64(block), torch.bfloat16)      # around element 2^31
+
+
+@pytest.mark.parametrize("tokens", [1, 300])
+def test_experts_past_32_bits_of_weights(tokens):
+    """4.4 GB of layout: the last expert and the first one."""
+    g = _gen(24)
+    E, R, C = 520, 4096, 4096
+    block = _block((E,), R, C, 128, False, torch.bfloat16, g)
+    experts = moe.Int4Experts([block])
+    assert experts.nbytes() > 2 ** 32
+    ids = torch.tensor([[E - 1, 0]], device="cuda").expand(tokens, 2)
+    x = torch.randn(tokens, C, generator=g, device="cuda").bfloat16()
+    order = moe.sort_tokens(ids, E)
+    y = moe.from_experts(experts(x, order, gather=True), order, torch.tensor([[1.0, 0.0]], device="cuda").expand(tokens, 2))
+    for e, got in ((E - 1, y), (0, experts(x, order, gather=True)[:tokens])):
+        one = tuple(t[e] if torch.is_tensor(t) else t for t in block)
+        _check_product(got, x, _dense64(one), torch.bfloat16)

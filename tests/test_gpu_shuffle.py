@@ -307,3 +307,31 @@ def test_calls_that_do_not_fit_are_refused():
         moe.from_experts(torch.zeros(6, 8, device="cuda"), order, torch.zeros(3, 2, device="cuda").int())
     with pytest.raises(P2PError, match="CUDA"):
         moe.to_experts(x.cpu(), order)
+
+
+def test_rows_past_32_bits():
+    """2.6e9 elements of rows: the last places, and the sums and gradients of the last tokens."""
+    T, K, H, E = 40000, 8, 8192, 16
+    g = _gen(30)
+    ids = _ids(T, K, E, g)
+    order = moe.sort_tokens(ids, E)
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    rows = moe.to_experts(x, order)
+    last = int(order.offsets[-1])
+    at = torch.arange(last - 50, last, device="cuda")
+    assert torch.equal(rows[at], x[order.order[at].long() // K])
+    w = torch.rand(T, K, generator=g, device="cuda").requires_grad_(True)
+    out = moe.from_experts(rows, order, w)
+    cot = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    (dw,) = torch.autograd.grad(out, w, cot)
+    t = slice(T - 20, T)
+    there = (order.where.view(T, K)[t] >= 0).double()
+    dot = (x[t].double() * cot[t].double()).sum(1, keepdim=True)
+    # sums of 8192 fp32 terms, each addition off by half a unit, by lanes and warps in a tree: below 64 roundings of the
+    # absolute sum
+    slack = 64 * 2.0 ** -24 * (x[t].double() * cot[t].double()).abs().sum(1, keepdim=True)
+    assert bool(((dw[t].double() - dot * there).abs() <= slack).all())
+    want = x[t].double() * (w[t].detach().double() * there).sum(1, keepdim=True)
+    # a product and an addition a slot, each half a unit of the absolute sum; then half a step of bf16
+    bound = 2 * K * 2.0 ** -24 * want.abs()
+    assert bool(((out[t].detach().double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all())
