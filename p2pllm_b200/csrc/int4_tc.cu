@@ -25,10 +25,10 @@
 //
 // Measured (bf16, groups of 128): 28672 x 4096 at 272 tokens 80 us replayed from a graph (798 TFLOP/s; the product alone
 // would take 39 us at the measured rate); 128 experts of 1536 x 2048 on 2048 x 8 tokens 238 us (433 TFLOP/s; items are
-// padded to 160 places). What binds is the way of a unit from hand to hand: its accumulator goes from products to commit,
-// read-out and release, with 130 to 220 cycles for each look at a barrier, and a row tile's way out in between. A unit takes
-// some 3,100 and 2,500 cycles where its products are 1,088 and 640: the tensor pipe is busy 37 % and 21 % of the time. It is
-// not x (half of its traffic, 6 TB/s from L2, gone: the same time) nor the builders (twice as many: the same).
+// padded to 160 places). What binds is the way of a unit from hand to hand, with 130 to 220 cycles for each look at a
+// barrier, and the partials and their join: with products, read-out and building all left out 272 tokens still take 60 us of
+// 85. A unit takes some 3,100 and 2,500 cycles where its products are 1,088 and 640: the tensor pipe is busy 37 % and 21 %
+// of the time. Half of x's traffic (6 TB/s from L2) or twice the builders change nothing.
 //
 // Every wait is bounded (2 s): a launch that gives up records where, issues nothing more, drains what it issued and
 // exits (p2p_int4_status reads the site).
