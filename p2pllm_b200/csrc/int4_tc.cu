@@ -46,7 +46,7 @@ using namespace sm100;
 
 constexpr int kPromoteWarps = 8;
 constexpr int kBuildWarp = kPromoteWarps;               // 8..
-// Warps that build one unit, and groups of them taking alternate units: up to 64 tokens the codes' turn binds; above 128
+// Warps that build one unit, and groups of them taking alternate units: up to 64 tokens the codes' turn binds; above 160
 // the promoting warps' accumulators leave registers for four builders only.
 constexpr int group_warps(int acc) { return acc >= 96 ? 4 : 8; }
 constexpr int build_groups(int acc) { return acc <= 32 ? 2 : 1; }

@@ -124,6 +124,13 @@ class Layout:
                  int(gated), ptr(self.data), stream_of(codes))
             torch.cuda.current_stream(self.device).synchronize()   # the products read weights ahead of their stream
 
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k != "_op"}          # an operator cannot be pickled
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._op = _lib.ops().int4_mm
+
     def check_x(self, x: torch.Tensor) -> None:
         require_cuda(x)
         if x.dtype != self.dtype:

@@ -200,6 +200,13 @@ class Int4Experts:
         self.rows, self.cols, self.dtype, self.device = (self.int4.rows, self.int4.cols, self.int4.dtype,
                                                          self.int4.device)
 
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k != "_op"}          # an operator cannot be pickled
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._op = _lib.ops().int4_grouped
+
     def __call__(self, x: torch.Tensor, order: TokenOrder, gather: bool = False,
                  out: torch.Tensor | None = None) -> torch.Tensor:
         q = self.int4

@@ -213,6 +213,19 @@ def test_modules_in_a_chain_read_what_the_one_before_wrote(tokens, sizes):
     kernels.int4_status()
 
 
+def test_modules_can_be_copied_and_pickled():
+    import copy
+    import pickle
+    g = _gen(78)
+    tiles = compact.Tiles([_block((), 40, 128, 64, True, torch.bfloat16, g)])
+    experts = moe.Int4Experts([_block((3,), 40, 128, 64, True, torch.bfloat16, g)])
+    x = torch.randn(9, 128, generator=g, device="cuda").bfloat16()
+    order = moe.sort_tokens(torch.randint(0, 3, (9, 1), generator=g, device="cuda"), 3)
+    for again in (copy.deepcopy, lambda t: pickle.loads(pickle.dumps(t))):
+        assert torch.equal(again(tiles)(x), tiles(x))
+        assert torch.equal(again(experts)(x, order), experts(x, order))
+
+
 def test_calls_from_several_threads_at_once():
     """Threads on streams of their own, modules of both kernels and routed experts among them."""
     import threading
