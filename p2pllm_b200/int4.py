@@ -122,7 +122,7 @@ class Layout:
         with torch.cuda.device(self.device):
             call("p2p_int4_layout", ptr(codes), ptr(scales), ptr(zeros), self.experts, self.rows, cols, group,
                  int(gated), ptr(self.data), stream_of(codes))
-            torch.cuda.current_stream(self.device).synchronize()   # the products read weights ahead of their stream
+        kernels.settle(self.data)
 
     def __getstate__(self) -> dict:
         return {k: v for k, v in self.__dict__.items() if k != "_op"}          # an operator cannot be pickled
@@ -130,6 +130,7 @@ class Layout:
     def __setstate__(self, state: dict) -> None:
         self.__dict__.update(state)
         self._op = _lib.ops().int4_mm
+        kernels.settle(self.data)                              # copied or loaded a moment ago
 
     def check_x(self, x: torch.Tensor) -> None:
         require_cuda(x)

@@ -41,6 +41,13 @@ def _rezero_workspaces(dev: torch.device, purpose: str) -> int:
     return n
 
 
+def settle(*weights: torch.Tensor) -> None:
+    """Waits until the current streams have written these weights. The products read theirs before the stream's previous
+    kernel has ended, so a layout is used only after the kernel or copy that filled it is known to be over."""
+    for device in {w.device for w in weights if w.is_cuda}:
+        torch.cuda.current_stream(device).synchronize()
+
+
 def _rows2d(x: torch.Tensor) -> torch.Tensor:
     x = x.reshape(-1, x.shape[-1])
     if x.stride(-1) != 1:
