@@ -86,7 +86,7 @@ def _nbytes(blocks) -> int:
     return sum(t.numel() * t.element_size() for b in blocks for t in b[1:] if torch.is_tensor(t))
 
 
-class Tiles:
+class Tiles(kernels.Settled):
     """A module's row blocks on the GPU, as the compact GEMM reads them; calling it multiplies tokens by them.
     The B200 counterpart of p2p/compact.py:113-202 (Tiles). bf16 / f16 modules whose columns are a multiple of 8 are
     re-laid once into (128-row x 64-column) segments of packed (value, row, column) words and multiplied on tcgen05
@@ -199,7 +199,7 @@ def gate_up_rows(blocks: list) -> tuple:
     return interleave_gate_up(values).contiguous(), None if idx is None else interleave_gate_up(idx).contiguous()
 
 
-class GatedTiles:
+class GatedTiles(kernels.Settled):
     """A gated MLP's gate and up projections as one tensor-core module whose GEMM also applies the gate: calling it on
     x [T, cols] returns dtype(silu(g) * u) [T, R], g and u being the projections' outputs rounded to the model dtype
     -- what SGLang's SiluAndMul makes of the gate_up projection's output, without writing it (p2p/compact.py:205-224

@@ -84,7 +84,7 @@ def expand(block: tuple, experts=None) -> torch.Tensor:
     return dense
 
 
-class Layout:
+class Layout(kernels.Settled):
     """Row blocks of one module (or, with a leading expert dimension, of one routed-expert tensor) in the layout of
     csrc/int4.cuh, built once at load. gated: the first half of the rows is the gate, the second half the up
     projection, and the products return silu(gate) * up.
@@ -128,9 +128,8 @@ class Layout:
         return {k: v for k, v in self.__dict__.items() if k != "_op"}          # an operator cannot be pickled
 
     def __setstate__(self, state: dict) -> None:
-        self.__dict__.update(state)
+        super().__setstate__(state)
         self._op = _lib.ops().int4_mm
-        kernels.settle(self.data)                              # copied or loaded a moment ago
 
     def check_x(self, x: torch.Tensor) -> None:
         require_cuda(x)

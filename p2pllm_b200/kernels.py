@@ -48,6 +48,15 @@ def settle(*weights: torch.Tensor) -> None:
         torch.cuda.current_stream(device).synchronize()
 
 
+class Settled:
+    """A module's weights in a layout that the products read ahead of their stream: a copy, or what pickle.loads made, waits
+    for them as building them does."""
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        settle(*(t for t in state.values() if torch.is_tensor(t)))
+
+
 def _rows2d(x: torch.Tensor) -> torch.Tensor:
     x = x.reshape(-1, x.shape[-1])
     if x.stride(-1) != 1:

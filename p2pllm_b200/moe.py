@@ -34,7 +34,7 @@ from .compact import _cols, gate_up_rows, to_compact
 ITEM_TOKENS = 256                       # tokens one grouped CTA takes (an accumulator of at most 256 columns)
 
 
-class ExpertTiles:
+class ExpertTiles(kernels.Settled):
     """A routed-expert tensor [E, rows, cols] from its row blocks (each ("dense", W [E, r, C]) or ("sparse" |
     "compact", values [E, r, k], words | idx [E, r, ...], C), in row order), laid out for the grouped GEMM: expert
     e's rows start at row tile e * item_row_tiles. Built once at load (one layout build an expert)."""

@@ -26,3 +26,18 @@ def test_modules_copied_behind_a_busy_stream():
             a @ a
         assert torch.equal(again(tiles)(x), want[0])
         assert torch.equal(again(experts)(x[:, :2048], order), want[1])
+
+
+@pytest.mark.parametrize("layout", ["tc", "mask"])
+def test_pruned_modules_copied_behind_a_busy_stream(layout):
+    g = _gen(2)
+    w = torch.randn(4096, 4096, generator=g, device="cuda").bfloat16()
+    from p2pllm_b200 import kernels
+    kept = kernels.wanda_select(w, torch.ones(4096, device="cuda"), 1024)
+    tiles = compact.Tiles([("compact", kept["values"], kept["idx"], 4096)], layout=layout)
+    x = torch.randn(17, 4096, generator=g, device="cuda").bfloat16()
+    want = tiles(x)
+    for again in (copy.deepcopy, lambda t: pickle.loads(pickle.dumps(t))):
+        for _ in range(50):
+            w @ w
+        assert torch.equal(again(tiles)(x), want)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from p2pllm_b200 import _lib, int4
+from p2pllm_b200 import _lib, compact, int4, moe
 
 
 @pytest.fixture(scope="module")
@@ -47,3 +47,11 @@ def test_a_layout_that_comes_back_waits_for_its_weights(lib, waits):
     again = int4.Layout.__new__(int4.Layout)
     again.__setstate__(_layout().__getstate__())
     assert waits == [torch.device("cuda", 0)]
+
+
+@pytest.mark.parametrize("kind", [compact.Tiles, compact.GatedTiles, moe.ExpertTiles])
+def test_pruned_layouts_that_come_back_wait_for_their_weights(waits, kind):
+    state = {"layout": "tc", "words": torch.zeros(8, dtype=torch.int32).as_subclass(OnGpu), "blocks": None}
+    again = kind.__new__(kind)
+    again.__setstate__(dict(state))
+    assert waits == [torch.device("cuda", 0)] and again.words is state["words"]
