@@ -93,6 +93,8 @@ class Tiles(kernels.Settled):
     tensor cores; fp32 modules (and others) keep rows of values + column indices for the CUDA-core kernel. A module
     whose blocks are all 4-bit ones takes the layout "int4"."""
 
+    int4 = None                     # also of modules pickled before there were 4-bit blocks
+
     @staticmethod
     def usable(blocks: list) -> bool:
         """CUDA tensors of bf16, f16 or f32, 2-D blocks (p2p/compact.py:117-122 asks for the same, less fp32, plus
@@ -105,7 +107,6 @@ class Tiles(kernels.Settled):
     def __init__(self, blocks: list, layout: str | None = None):
         if not blocks:
             raise P2PError("a module needs at least one row block")
-        self.int4 = None
         if any(b[0] == "int4" for b in blocks):
             self._init_int4(blocks, layout)
             return
@@ -206,8 +207,9 @@ class GatedTiles(kernels.Settled):
     multiplies the two projections; the activation is the model's own). Blocks: the gate rows, then the up rows. Of
     4-bit blocks, which take any number of rows and columns, g and u are the unrounded fp32 sums."""
 
+    int4 = None                     # also of modules pickled before there were 4-bit blocks
+
     def __init__(self, blocks: list):
-        self.int4 = None
         if any(b[0] == "int4" for b in blocks):
             if any(b[0] != "int4" or b[1].dim() != 2 for b in blocks):
                 raise P2PError("4-bit blocks make up a whole module, in the layout \"int4\", of 2-D blocks")

@@ -242,6 +242,8 @@ class GroupedMoE(torch.nn.Module):
     (gate rows, then up rows), "w2_weight": blocks of [E, H, R]}, all of them 4-bit blocks or none. apply(layer, dispatch_output) returns the layer's
     output [T, H] in x's dtype. Other attributes are the layer's own method's."""
 
+    is_int4 = False                 # also of layers pickled before there were 4-bit blocks
+
     def __init__(self, method, weights: dict):
         super().__init__()
         self.method = method

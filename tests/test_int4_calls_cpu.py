@@ -1,4 +1,6 @@
 """How 4-bit modules and the token shuffle take calls that their main tests leave out, without a GPU."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -55,3 +57,28 @@ def test_pruned_layouts_that_come_back_wait_for_their_weights(waits, kind):
     again = kind.__new__(kind)
     again.__setstate__(dict(state))
     assert waits == [torch.device("cuda", 0)] and again.words is state["words"]
+
+
+def test_modules_pickled_before_4_bit_blocks_still_run(monkeypatch):
+    """Their state has no word of 4 bits."""
+    ran = []
+    for name in ("spmm_tc", "spmm_tc_gated"):
+        monkeypatch.setattr(compact.kernels, name, lambda *a, name=name, **k: ran.append(name))
+    monkeypatch.setattr(moe, "route", lambda *a: ran.append("route") or (_ for _ in ()).throw(StopIteration))
+    state = {"layout": "tc", "words": torch.zeros(8, dtype=torch.int32), "seg": torch.zeros(2, dtype=torch.int64), "rows": 4,
+             "layout_rows": 8, "cols": 8, "seg_cap": 1, "blocks": None, "dtype": torch.bfloat16}
+    for kind in (compact.Tiles, compact.GatedTiles):
+        module = kind.__new__(kind)
+        module.__setstate__(dict(state))
+        module(torch.zeros(1, 8, dtype=torch.bfloat16))
+        assert module.nbytes() == 48
+    layer = moe.GroupedMoE.__new__(moe.GroupedMoE)
+    torch.nn.Module.__init__(layer)
+    experts = compact.Tiles.__new__(compact.Tiles)
+    experts.__setstate__(state | {"experts": 2})
+    layer.method, layer.w13 = None, experts
+    x, ids = torch.zeros(1, 8, dtype=torch.bfloat16), torch.zeros(1, 2, dtype=torch.int64)
+    topk = SimpleNamespace(topk_ids=ids, topk_weights=torch.zeros(1, 2))
+    with pytest.raises(StopIteration):
+        layer.apply(None, SimpleNamespace(hidden_states=x, topk_output=topk))
+    assert ran == ["spmm_tc", "spmm_tc_gated", "route"]
