@@ -24,10 +24,35 @@ int launch_status(const char* what) {
     return P2P_OK;
 }
 
+// The limit belongs to the kernel and the device, not to the call, so it only ever rises: a smaller request of another
+// thread must not take it away between a call's own request and its launch. What was asked so far is kept in a table of
+// open addresses (no allocation that could throw across the C ABI); with the table full a request sets the limit itself.
+namespace {
+struct SmemLimit {
+    const void* kernel;
+    int device, bytes;
+};
+constexpr int kSmemLimits = 4096;
+SmemLimit g_smem_limits[kSmemLimits];
+std::mutex g_smem_mu;
+}  // namespace
+
 int allow_smem(const void* kernel, int bytes, const char* what) {
     if (bytes <= 48 * 1024) return P2P_OK;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return fail(P2P_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+    const std::lock_guard<std::mutex> lock(g_smem_mu);
+    SmemLimit* at = nullptr;
+    const uintptr_t start = (reinterpret_cast<uintptr_t>(kernel) >> 4) * 31 + (uintptr_t)dev;
+    for (int i = 0; i < kSmemLimits && !at; ++i) {
+        SmemLimit* slot = &g_smem_limits[(start + i) % kSmemLimits];
+        if (!slot->kernel || (slot->kernel == kernel && slot->device == dev)) at = slot;
+    }
+    if (at && at->kernel && at->bytes >= bytes) return P2P_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return fail(P2P_ECUDA, "%s: %d bytes of shared memory: %s", what, bytes, cudaGetErrorString(e));
+    if (at) *at = {kernel, dev, bytes};
     return P2P_OK;
 }
 

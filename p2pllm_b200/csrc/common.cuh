@@ -14,7 +14,8 @@ namespace p2p {
 int fail(int code, const char* fmt, ...);
 // P2P_OK if the last launch succeeded, else P2P_ECUDA with the CUDA error named after `what`.
 int launch_status(const char* what);
-// Opts a kernel into `bytes` of dynamic shared memory (once per kernel and size class); P2P_ECUDA on failure.
+// Opts a kernel into at least `bytes` of dynamic shared memory on the current device; P2P_ECUDA on failure. The limit never
+// falls again, so threads may ask for different sizes of one kernel.
 int allow_smem(const void* kernel, int bytes, const char* what);
 // The number of SMs of the current device (cached per device).
 int sm_count();

@@ -653,8 +653,7 @@ SmallPlan plan_small(const Int4Call& c) {
 template <typename T, int NT, bool G32>
 int launch_small(const CUtensorMap& map, const SmallParams& p, const SmallPlan& pl, cudaStream_t st, const char* what) {
     auto kernel = int4_small_kernel<T, NT, G32>;
-    static SmemAllowed allowed;
-    if (int e = allowed((const void*)kernel, pl.smem, what)) return e;
+    if (int e = allow_smem((const void*)kernel, pl.smem, what)) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -16,8 +16,6 @@
 // a tcgen05.st.16x256b.x4 of 16 rows by 64 columns into tensor memory.
 // Of a gated module the even row blocks are gate rows, the odd ones the same units' up rows.
 #pragma once
-#include <atomic>
-
 #include "sm100.cuh"
 
 namespace p2p {
@@ -150,21 +148,5 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 }  // namespace sm100
-
-// allow_smem once a kernel and device: asked on every call it costs the host more than half a microsecond.
-struct SmemAllowed {
-    static constexpr int kMost = 226 * 1024;
-    std::atomic<int> bytes[64] = {};
-    int operator()(const void* kernel, int need, const char* what) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || need > kMost) return allow_smem(kernel, need, what);
-        if (bytes[dev].load(std::memory_order_relaxed) >= need) return P2P_OK;
-        // all that these kernels ask for (their static part fits the rest), so that calls of another size on another
-        // thread cannot lower it again
-        if (int e = allow_smem(kernel, kMost, what)) return e;
-        bytes[dev].store(kMost, std::memory_order_relaxed);
-        return P2P_OK;
-    }
-};
 
 }  // namespace p2p

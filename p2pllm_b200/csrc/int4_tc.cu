@@ -694,8 +694,7 @@ TcPlan plan_tc(int most, bool routed) {
 template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
     auto kernel = int4_tc_kernel<T, PIECES, W0, W1>;
     constexpr int kThreads = threads_of(W0 + W1);
-    static SmemAllowed allowed;
-    if (int e = allowed((const void*)kernel, smem, what)) return e;
+    if (int e = allow_smem((const void*)kernel, smem, what)) return e;
     if (promote_regs(W0 + W1) > 0) {                     // the register split needs what it was written for
         static std::atomic<int> regs{0};
         if (regs == 0) {

@@ -41,3 +41,30 @@ def test_pruned_modules_copied_behind_a_busy_stream(layout):
         for _ in range(50):
             w @ w
         assert torch.equal(again(tiles)(x), want)
+
+
+def test_sorts_of_different_sizes_from_several_threads():
+    """1024 experts take 139 KB of shared memory, 512 with many pairs 70 KB: requests of one thread must not take room
+    from another's."""
+    import threading
+    g = _gen(3)
+    cases = [(torch.randint(0, e, (t, 8), generator=g, device="cuda"), e) for t, e in ((2048, 1024), (2048, 512), (16, 600))]
+    want = [moe.sort_tokens(ids, e) for ids, e in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    got = moe.sort_tokens(*cases[i % 3])
+                torch.cuda.current_stream().synchronize()
+                assert torch.equal(got.where, want[i % 3].where) and torch.equal(got.offsets, want[i % 3].offsets)
+        except BaseException as e:
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
