@@ -259,6 +259,11 @@ std::tuple<at::Tensor, at::Tensor> call_sum_back(const at::Tensor& dout, const a
 }
 
 bool needs_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Whether t carries a tangent, which a call below autograd would lose without a word.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+void check_tangents(bool any) {
+    TORCH_CHECK(!any, "p2p_b200: forward-mode derivatives of the token shuffle are not offered");
+}
 
 struct Spread : torch::autograd::Function<Spread> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& where,
@@ -299,12 +304,14 @@ struct Sum : torch::autograd::Function<Sum> {
 };
 
 at::Tensor moe_spread_grad(const at::Tensor& x, const at::Tensor& where, const at::Tensor& offsets, int64_t topk) {
+    check_tangents(has_tangent(x));
     if (needs_grad(x)) return Spread::apply(x, where, offsets, topk);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_spread(x, where, offsets, topk);
 }
 at::Tensor moe_sum_grad(const at::Tensor& y, const at::Tensor& where, const at::Tensor& offsets,
                         const std::optional<at::Tensor>& weights, int64_t topk) {
+    check_tangents(has_tangent(y) || (weights && has_tangent(*weights)));
     if (needs_grad(y) || (weights && needs_grad(*weights))) return Sum::apply(y, where, offsets, weights, topk);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_sum(y, where, offsets, weights, topk);
@@ -312,6 +319,7 @@ at::Tensor moe_sum_grad(const at::Tensor& y, const at::Tensor& where, const at::
 std::tuple<at::Tensor, at::Tensor> moe_sum_back_grad(const at::Tensor& dout, const at::Tensor& y,
                                                      const at::Tensor& where, const at::Tensor& offsets,
                                                      const at::Tensor& weights, int64_t topk) {
+    check_tangents(has_tangent(dout) || has_tangent(y) || has_tangent(weights));
     TORCH_CHECK(!(needs_grad(dout) || needs_grad(y) || needs_grad(weights)),
                 "p2p_b200: second derivatives of the weighted sum are not offered");
     at::AutoDispatchBelowADInplaceOrView below;

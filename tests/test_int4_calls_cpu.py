@@ -3,6 +3,7 @@ from types import SimpleNamespace
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from p2pllm_b200 import _lib, compact, int4, moe
 
@@ -82,3 +83,29 @@ def test_modules_pickled_before_4_bit_blocks_still_run(monkeypatch):
     with pytest.raises(StopIteration):
         layer.apply(None, SimpleNamespace(hidden_states=x, topk_output=topk))
     assert ran == ["spmm_tc", "spmm_tc_gated", "route"]
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, device="meta", dtype=dtype)
+
+
+@pytest.fixture
+def order(lib):
+    return moe.TokenOrder(*_lib.ops().moe_sort(_meta(17, 8, dtype=torch.int64), 128), 17, 8)
+
+
+@pytest.mark.parametrize("which", ["rows there", "sums back", "weighted sums back", "weights", "gradient"])
+def test_tangents_are_not_lost_on_the_way_to_the_experts_and_back(lib, order, which):
+    """Forward-mode derivatives are refused, as they are where an input needs a gradient, and not returned as none."""
+    ops, x, y, w = _lib.ops(), _meta(17, 96), _meta(136, 96), _meta(17, 8)
+    call, t = {"rows there": (lambda t: ops.moe_spread(t, order.where, order.offsets, 8), x),
+               "sums back": (lambda t: ops.moe_sum(t, order.where, order.offsets, None, 8), y),
+               "weighted sums back": (lambda t: ops.moe_sum(t, order.where, order.offsets, w, 8), y),
+               "weights": (lambda t: ops.moe_sum(y, order.where, order.offsets, t, 8), w),
+               "gradient": (lambda t: ops.moe_sum_back(t, y, order.where, order.offsets, w, 8)[0], x)}[which]
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        call(fwAD.make_dual(t, torch.empty_like(t)))
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(call, (t,), (torch.empty_like(t),))
+    with fwAD.dual_level():                          # no tangent: the call goes through
+        assert call(t).device.type == "meta"
