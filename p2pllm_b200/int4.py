@@ -14,6 +14,7 @@ and a scale for every `group` columns of a row, against 0.85 bytes for keep 36 w
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _lib, kernels
 from ._lib import P2PError, call, dtype_code, ptr, require_cuda, stream_of
@@ -139,7 +140,7 @@ class Layout(kernels.Settled):
             raise P2PError(f"x lies on {x.device}, the weights on {self.device}")
         if x.dim() != 2 or x.shape[1] != self.cols:
             raise P2PError(f"x of {tuple(x.shape)} does not have {self.cols} columns")
-        if x.requires_grad and torch.is_grad_enabled():
+        if (x.requires_grad and torch.is_grad_enabled()) or fwAD.unpack_dual(x).tangent is not None:
             raise P2PError("4-bit weights are for inference: x must not need a gradient")
 
     def mm(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

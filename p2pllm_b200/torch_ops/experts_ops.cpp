@@ -59,8 +59,6 @@ void check_int4(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64
                 bool gated) {
     check_matrix(x, "x");
     TORCH_CHECK(x.size(1) == cols, "p2p_b200: x of ", x.sizes(), " does not have ", cols, " columns");
-    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()),
-                "p2p_b200: 4-bit weights are for inference: x must not need a gradient");
     TORCH_CHECK(group == 32 || group == 64 || group == 128, "p2p_b200: groups of ", group, " columns, not 32, 64 or 128");
     const int64_t need = p2p_int4_layout_bytes(experts, rows, cols, (int)group, zeros, gated);
     TORCH_CHECK(need > 0 && layout.device() == x.device() && layout.scalar_type() == at::kByte && layout.is_contiguous() &&
@@ -326,6 +324,48 @@ std::tuple<at::Tensor, at::Tensor> moe_sum_back_grad(const at::Tensor& dout, con
     return call_sum_back(dout, y, where, offsets, weights, topk);
 }
 
+// The products as autograd sees them: an input that is differentiated in either mode, under torch.func too, is refused.
+
+void check_inference(const at::Tensor& x) {
+    TORCH_CHECK(!needs_grad(x) && !has_tangent(x), "p2p_b200: 4-bit weights are for inference: x must not need a gradient");
+}
+void check_inference(const at::Tensor& x, const at::Tensor& out) {
+    check_inference(x);
+    TORCH_CHECK(!needs_grad(out) && !has_tangent(out), "p2p_b200: 4-bit weights are for inference: out must not need a gradient");
+}
+
+at::Tensor int4_mm_grad(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t rows, int64_t cols, int64_t group, bool gated) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::int4_mm", "").typed<decltype(int4_mm)>();
+    check_inference(x);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, layout, zeros, rows, cols, group, gated);
+}
+void int4_mm_into_grad(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t rows, int64_t cols, int64_t group,
+                       bool gated, const at::Tensor& out) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::int4_mm_into", "").typed<decltype(int4_mm_into)>();
+    check_inference(x, out);
+    at::AutoDispatchBelowADInplaceOrView below;
+    op.call(x, layout, zeros, rows, cols, group, gated, out);
+}
+at::Tensor int4_grouped_grad(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols,
+                             int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
+                             const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::int4_grouped", "").typed<decltype(int4_grouped)>();
+    check_inference(x);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, layout, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk, gather);
+}
+void int4_grouped_into_grad(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols,
+                            int64_t group, bool gated, const at::Tensor& order, const at::Tensor& where, const at::Tensor& offsets,
+                            const at::Tensor& items, const at::Tensor& n_items, int64_t topk, bool gather,
+                            const at::Tensor& out) {
+    static const auto op =
+        c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::int4_grouped_into", "").typed<decltype(int4_grouped_into)>();
+    check_inference(x, out);
+    at::AutoDispatchBelowADInplaceOrView below;
+    op.call(x, layout, zeros, experts, rows, cols, group, gated, order, where, offsets, items, n_items, topk, gather, out);
+}
+
 // ---- shapes ----------------------------------------------------------------------------------------------------------
 
 at::Tensor int4_mm_meta(const at::Tensor& x, const at::Tensor&, bool, int64_t rows, int64_t, int64_t, bool gated) {
@@ -385,6 +425,10 @@ TORCH_LIBRARY_IMPL(p2p_b200, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(p2p_b200, Autograd, m) {
+    m.impl("int4_mm", &int4_mm_grad);
+    m.impl("int4_mm_into", &int4_mm_into_grad);
+    m.impl("int4_grouped", &int4_grouped_grad);
+    m.impl("int4_grouped_into", &int4_grouped_into_grad);
     m.impl("moe_spread", &moe_spread_grad);
     m.impl("moe_sum", &moe_sum_grad);
     m.impl("moe_sum_back", &moe_sum_back_grad);

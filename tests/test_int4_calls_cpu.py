@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from p2pllm_b200 import _lib, compact, int4, moe
+from p2pllm_b200 import P2PError, _lib, compact, int4, moe
 
 
 @pytest.fixture(scope="module")
@@ -109,3 +109,43 @@ def test_tangents_are_not_lost_on_the_way_to_the_experts_and_back(lib, order, wh
         torch.func.jvp(call, (t,), (torch.empty_like(t),))
     with fwAD.dual_level():                          # no tangent: the call goes through
         assert call(t).device.type == "meta"
+
+
+@pytest.mark.parametrize("which", ["mm", "mm_into", "grouped", "grouped_into"])
+def test_products_refuse_to_be_differentiated_in_any_mode(lib, order, which):
+    """4-bit products are for inference: forward mode and torch.func's transforms are refused as requires_grad is, and so
+    is an output that takes part in a graph."""
+    ops, w = _lib.ops(), _meta(100, dtype=torch.uint8)
+    sizes = (False, 40, 64, 64, False)
+    sorted_ = (order.order, order.where, order.offsets, order.items, order.n_items, 8, True)
+    x, out = _meta(17, 64), _meta(17 if "mm" in which else 136, 40)
+    run = {"mm": lambda t: ops.int4_mm(t, w, *sizes), "mm_into": lambda t, y=out: ops.int4_mm_into(t, w, *sizes, y),
+           "grouped": lambda t: ops.int4_grouped(t, w, False, 128, *sizes[1:], *sorted_),
+           "grouped_into": lambda t, y=out: ops.int4_grouped_into(t, w, False, 128, *sizes[1:], *sorted_, y)}[which]
+    total = lambda t: (run(t) if "into" not in which else run(t) or t).float().sum()
+    run(x)
+    with torch.no_grad():
+        run(x.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="inference"):
+        run(x.clone().requires_grad_(True))
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="inference"):
+        run(fwAD.make_dual(x, torch.empty_like(x)))
+    for transform in (lambda: torch.func.grad(total)(x), lambda: torch.func.vjp(total, x),
+                      lambda: torch.func.jvp(total, (x,), (torch.empty_like(x),))):
+        with pytest.raises(RuntimeError, match="inference"):
+            transform()
+    if "into" in which:
+        with pytest.raises(RuntimeError, match="out must not"):
+            run(x, out.clone().requires_grad_(True))
+        with torch.no_grad():
+            run(x, out.clone().requires_grad_(True))
+
+
+def test_a_dual_x_is_refused_with_the_packages_own_error(lib, monkeypatch):
+    monkeypatch.setattr(int4, "require_cuda", lambda *ts: None)
+    layout = _layout()
+    layout.device, layout.cols = torch.device("cpu"), 4
+    x = torch.zeros(2, 4, dtype=torch.bfloat16)
+    layout.check_x(x)
+    with fwAD.dual_level(), pytest.raises(P2PError, match="gradient"):
+        layout.check_x(fwAD.make_dual(x, torch.ones_like(x)))
