@@ -118,7 +118,8 @@ class Layout(kernels.Settled):
         if nbytes < 0:
             raise P2PError(f"a gated module has as many gate rows as up rows, not {self.rows} in all")
         self._op = _lib.ops().int4_mm
-        self.data = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        # bytes in a tensor of the weights' dtype (a whole number of them), by which the operators know what they multiply
+        self.data = torch.empty(nbytes // 2, dtype=self.dtype, device=self.device)
         codes, scales, zeros = codes.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
         with torch.cuda.device(self.device):
             call("p2p_int4_layout", ptr(codes), ptr(scales), ptr(zeros), self.experts, self.rows, cols, group,
@@ -130,6 +131,8 @@ class Layout(kernels.Settled):
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
+        if self.data.dtype == torch.uint8:                     # pickled when data was plain bytes
+            self.data = self.data.view(self.dtype)
         self._op = _lib.ops().int4_mm
 
     def check_x(self, x: torch.Tensor) -> None:
@@ -160,4 +163,4 @@ class Layout(kernels.Settled):
         return out
 
     def nbytes(self) -> int:
-        return self.data.numel()
+        return self.data.nbytes

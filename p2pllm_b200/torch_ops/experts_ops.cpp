@@ -61,8 +61,11 @@ void check_int4(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64
     TORCH_CHECK(x.size(1) == cols, "p2p_b200: x of ", x.sizes(), " does not have ", cols, " columns");
     TORCH_CHECK(group == 32 || group == 64 || group == 128, "p2p_b200: groups of ", group, " columns, not 32, 64 or 128");
     const int64_t need = p2p_int4_layout_bytes(experts, rows, cols, (int)group, zeros, gated);
-    TORCH_CHECK(need > 0 && layout.device() == x.device() && layout.scalar_type() == at::kByte && layout.is_contiguous() &&
-                    layout.numel() >= need, "p2p_b200: the 4-bit layout does not hold ", rows, " x ", cols, " weights");
+    // the layout's bytes do not say what their scales are, its tensor's dtype does
+    TORCH_CHECK(layout.scalar_type() == x.scalar_type(), "p2p_b200: x is ", x.scalar_type(), ", the 4-bit layout's weights ",
+                layout.scalar_type());
+    TORCH_CHECK(need > 0 && layout.device() == x.device() && layout.is_contiguous() && (int64_t)layout.nbytes() >= need,
+                "p2p_b200: the 4-bit layout does not hold ", rows, " x ", cols, " weights");
 }
 
 void check_rows_out(const at::Tensor& out, const at::Tensor& x, int64_t rows, int64_t cols) {

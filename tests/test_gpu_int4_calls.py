@@ -6,7 +6,7 @@ import pickle
 import pytest
 import torch
 
-from p2pllm_b200 import compact, moe
+from p2pllm_b200 import _lib, compact, moe
 from test_gpu_int4 import _block, _gen
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,25 @@ def test_sorts_of_different_sizes_from_several_threads():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_the_operators_know_the_weights_dtype(tokens):
+    """A layout's bytes read with the wrong 16-bit type would be other scales: f16 tokens on bf16 weights are refused,
+    and so is a layout whose tensor does not say what it holds."""
+    g = _gen(4)
+    q = compact.Tiles([_block((), 40, 64, 64, True, torch.bfloat16, g)]).int4
+    e = moe.Int4Experts([_block((4,), 40, 64, 64, True, torch.bfloat16, g)])
+    order = moe.sort_tokens(torch.zeros(tokens, 1, dtype=torch.int32, device="cuda"), 4)
+    x = torch.randn(tokens, 64, generator=g, device="cuda").bfloat16()
+    ops = _lib.ops()
+    mm = lambda x, data: ops.int4_mm(x, data, True, 40, 64, 64, False)
+    grouped = lambda x, data: ops.int4_grouped(x, data, True, 4, 40, 64, 64, False, order.order, order.where, order.offsets,
+                                               order.items, order.n_items, 1, True)
+    assert torch.equal(mm(x, q.data), q.mm(x)) and torch.equal(grouped(x, e.int4.data), e(x, order, gather=True))
+    for call, data in ((mm, q.data), (grouped, e.int4.data)):
+        for bad_x, bad in ((x.half(), data), (x.float(), data), (x, data.view(torch.uint8)), (x, data.view(torch.float16))):
+            with pytest.raises(RuntimeError, match="4-bit layout's weights"):
+                call(bad_x, bad)
+    with pytest.raises(RuntimeError, match="does not hold"):
+        mm(x, q.data[:-1])

@@ -149,3 +149,9 @@ def test_a_dual_x_is_refused_with_the_packages_own_error(lib, monkeypatch):
     layout.check_x(x)
     with fwAD.dual_level(), pytest.raises(P2PError, match="gradient"):
         layout.check_x(fwAD.make_dual(x, torch.ones_like(x)))
+
+
+def test_layouts_pickled_as_plain_bytes_come_back_with_their_dtype(lib, waits):
+    again = int4.Layout.__new__(int4.Layout)
+    again.__setstate__(_layout().__getstate__())
+    assert again.data.dtype == torch.bfloat16 and again.data.numel() == 32 and again.nbytes() == 64
