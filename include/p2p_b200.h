@@ -326,8 +326,9 @@ int p2p_peer_status(int reset, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------
  * (2d) 4-bit weights with group scales: W[r, c] = (code[r, c] - zero[r, g]) * scale[r, g], g = c / group, the groups
- * 32, 64 or 128 columns, code in 0..15, scales in the weights' dtype (bf16 or f16), zero 8 where no zero points are
- * given. No counterpart in the reference, which keeps 16 bits a kept weight.
+ * 32, 64 or 128 columns, code and zero in 0..15 (the low four bits of a zero point's byte are read), scales in the
+ * weights' dtype (bf16 or f16), zero 8 where no zero points are given. No counterpart in the reference, which keeps 16
+ * bits a kept weight.
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* Codes [rows, ceil(cols / 2)] (the even column in the low half of a byte), scales [rows, ceil(cols / group)] and, if

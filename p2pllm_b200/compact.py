@@ -268,6 +268,10 @@ class CompactMoE(torch.nn.Module):
     def __init__(self, method, weights: dict):
         super().__init__()
         self.method, self.weights = method, weights
+        for blocks in weights.values():
+            for block in blocks:
+                if block[0] == "int4":                         # here once, not in every pass
+                    int4.check_zeros(int4.check_block(block)[2])
 
     def __getattr__(self, name):
         try:

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* __restrict__
     const int64_t stride = (int64_t)gridDim.x * blockDim.x;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * n_bytes; i += stride) {
         const int64_t row = i / n_bytes, c = i % n_bytes * 2, at = row * groups + c / group;
-        const float s = to_f32(scales[at]), z = zeros ? (float)zeros[at] : 8.f;
+        const float s = to_f32(scales[at]), z = zeros ? (float)(zeros[at] & 15) : 8.f;
         dense[row * cols + c] = from_f32<T>(((float)(codes[i] & 15) - z) * s);
         if (c + 1 < cols) dense[row * cols + c + 1] = from_f32<T>(((float)(codes[i] >> 4) - z) * s);
     }

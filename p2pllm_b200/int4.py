@@ -71,10 +71,20 @@ def check_block(block: tuple) -> tuple:
     return codes, scales, zeros, cols, group
 
 
+def check_zeros(zeros: torch.Tensor | None) -> None:
+    """Zero points are codes, 0..15: a larger one is refused. Reads one number back: for load time."""
+    if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+        raise P2PError(f"4-bit zero points are 0 to 15, not {int(zeros.max())}")
+
+
 def expand(block: tuple, experts=None) -> torch.Tensor:
-    """The dense rows [.., rows, cols] that a block stands for, in its scales' dtype; of routed experts only `experts`."""
+    """The dense rows [.., rows, cols] that a block stands for, in its scales' dtype; of routed experts only `experts`,
+    which is done in every pass and leaves the check of the zero points to who keeps the block."""
     codes, scales, zeros, cols, group = check_block(block)
-    if experts is not None:
+    if experts is None:
+        if zeros is not None and not torch.cuda.is_current_stream_capturing():
+            check_zeros(zeros)
+    else:
         codes, scales, zeros = codes[experts], scales[experts], None if zeros is None else zeros[experts]
     codes, scales, zeros = codes.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
     dense = torch.empty(*codes.shape[:-1], cols, dtype=scales.dtype, device=scales.device)
@@ -98,6 +108,8 @@ class Layout(kernels.Settled):
         if not blocks:
             raise P2PError("a module needs at least one row block")
         parts = [check_block(b) for b in blocks]
+        for p in parts:
+            check_zeros(p[2])
         codes, scales, zeros, cols, group = parts[0]
         for c, s, _, n, g in parts[1:]:
             if (n, g, s.dtype, c.dim(), c.device) != (cols, group, scales.dtype, codes.dim(), codes.device) or \

@@ -6,7 +6,7 @@ import pickle
 import pytest
 import torch
 
-from p2pllm_b200 import _lib, compact, moe
+from p2pllm_b200 import P2PError, _lib, compact, int4, moe
 from test_gpu_int4 import _block, _gen
 
 pytestmark = pytest.mark.gpu
@@ -90,3 +90,31 @@ def test_the_operators_know_the_weights_dtype(tokens):
                 call(bad_x, bad)
     with pytest.raises(RuntimeError, match="does not hold"):
         mm(x, q.data[:-1])
+
+
+@pytest.mark.parametrize("zero", [16, 255])
+def test_zero_points_that_are_no_codes_are_refused(zero):
+    """16 would multiply as 0 and expand as 16."""
+    g = _gen(5)
+    lead = ((), (3,))
+    for make, dims in ((lambda b: compact.Tiles([b]), lead[0]), (lambda b: compact.GatedTiles([b]), lead[0]),
+                       (lambda b: int4.expand(b), lead[0]), (lambda b: moe.Int4Experts([b]), lead[1]),
+                       (lambda b: compact.CompactMoE(None, {"w2_weight": [b]}), lead[1])):
+        block = _block(dims, 32, 130, 32, True, torch.bfloat16, g)
+        make(block)
+        block[3][..., -1, -1] = zero
+        with pytest.raises(P2PError, match=f"0 to 15, not {zero}"):
+            make(block)
+
+
+def test_whole_blocks_can_be_expanded_while_a_graph_is_captured():
+    g = _gen(6)
+    block = _block((), 32, 128, 32, True, torch.bfloat16, g)
+    want = int4.expand(block)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dense = int4.expand(block)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dense, want)

@@ -155,3 +155,10 @@ def test_layouts_pickled_as_plain_bytes_come_back_with_their_dtype(lib, waits):
     again = int4.Layout.__new__(int4.Layout)
     again.__setstate__(_layout().__getstate__())
     assert again.data.dtype == torch.bfloat16 and again.data.numel() == 32 and again.nbytes() == 64
+
+
+def test_zero_points_are_codes():
+    for good in (None, torch.zeros(0, dtype=torch.uint8), torch.full((3,), 15, dtype=torch.uint8)):
+        int4.check_zeros(good)
+    with pytest.raises(P2PError, match="0 to 15, not 16"):
+        int4.check_zeros(torch.tensor([[3, 16], [0, 1]], dtype=torch.uint8))
