@@ -49,13 +49,12 @@ def _rows(block: tuple) -> int:
     return block[1].shape[-2]
 
 
-def _cols(block: tuple) -> int:
-    return block[3] if block[0] in ("sparse", "compact") else block[1].shape[-1]
-
-
 def _take(block: tuple, a: int, b: int) -> tuple:
     if block[0] == "dense":
         return ("dense", block[1][..., a:b, :])
+    if block[0] == "int4":
+        _, codes, scales, zeros, cols, group = block
+        return ("int4", codes[..., a:b, :], scales[..., a:b, :], None if zeros is None else zeros[..., a:b, :], cols, group)
     kind, values, meta, cols = block
     return (kind, values[..., a:b, :], meta[..., a:b, :], cols)
 
@@ -121,7 +120,7 @@ class ShardedCompact:
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
         self.rank = dist.get_rank(group) if dist.is_initialized() else 0
         self.rows = sum(_rows(b) for b in blocks)
-        self.cols = _cols(blocks[0])
+        self.cols = compact._cols(blocks[0])
         self.ranges = row_ranges(self.rows, self.world)
         start, stop = self.ranges[self.rank]
         self.fused = (self.world > 1) if fused is None else fused
@@ -172,7 +171,7 @@ class ShardedCompact:
                 kernels.spmm_mask_peers(x2, t.data, t.seg, self.mine, self.cols, ptrs, self.world,
                                         self.ranges[self.rank][0], self.rows)
             else:
-                raise P2PError("the fused all-gather needs a tensor-core layout (tc or mask)")
+                raise P2PError("without a push the fused all-gather needs the layout tc or mask")
         if sync:
             self.peers.barrier()
         return buf[:T]

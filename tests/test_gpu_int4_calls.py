@@ -6,8 +6,8 @@ import pickle
 import pytest
 import torch
 
-from p2pllm_b200 import P2PError, _lib, compact, int4, moe
-from test_gpu_int4 import _block, _gen
+from p2pllm_b200 import P2PError, _lib, compact, int4, moe, shard
+from test_gpu_int4 import _block, _check_product, _dense64, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,18 @@ def test_whole_blocks_can_be_expanded_while_a_graph_is_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(dense, want)
+
+
+@pytest.mark.parametrize("tokens", [1, 17, 40])
+def test_a_sharded_4_bit_module(tokens):
+    """One rank's module, and two ranks' rows by hand, each rank writing its columns of y."""
+    g = _gen(7)
+    blocks = [_block((), r, 130, 32, z, torch.bfloat16, g) for r, z in ((200, True), (57, False))]
+    x = torch.randn(tokens, 130, generator=g, device="cuda").bfloat16()
+    want = compact.Tiles(blocks)(x)
+    assert torch.equal(shard.ShardedCompact(blocks).apply(None, x), want)
+    y = torch.zeros(tokens, 257, dtype=torch.bfloat16, device="cuda")
+    for start, stop in shard.row_ranges(257, 2):
+        mine = shard.shard_blocks(blocks, start, stop)
+        compact.Tiles(mine)(x, out=y[:, start:stop])
+        _check_product(y[:, start:stop], x, torch.cat([_dense64(b) for b in mine]), torch.bfloat16)

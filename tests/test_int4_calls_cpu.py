@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from p2pllm_b200 import P2PError, _lib, compact, int4, moe
+from p2pllm_b200 import P2PError, _lib, compact, int4, moe, shard
 
 
 @pytest.fixture(scope="module")
@@ -162,3 +162,28 @@ def test_zero_points_are_codes():
         int4.check_zeros(good)
     with pytest.raises(P2PError, match="0 to 15, not 16"):
         int4.check_zeros(torch.tensor([[3, 16], [0, 1]], dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("world", [1, 2, 3, 8])
+def test_4_bit_blocks_are_cut_by_rows(world):
+    """Every rank's blocks, put together again, are the module's."""
+    g = torch.Generator().manual_seed(world)
+    rand = lambda *s: torch.randint(0, 256, s, generator=g, dtype=torch.uint8)
+    blocks = [("int4", rand(r, 65), rand(r, 5).bfloat16(), rand(r, 5) % 16 if z else None, 130, 32)
+              for r, z in ((200, True), (57, False), (143, True))]
+    whole = [[], [], []]
+    for start, stop in shard.row_ranges(400, world):
+        mine = shard.shard_blocks(blocks, start, stop)
+        assert sum(b[1].shape[0] for b in mine) == stop - start and all(b[0] == "int4" and b[4:] == (130, 32) for b in mine)
+        for k, into in enumerate(whole, 1):
+            into += [torch.full_like(b[1][:, :5], 8) if b[k] is None else b[k] for b in mine]
+    for k, parts in enumerate(whole, 1):
+        want = [torch.full_like(b[1][:, :5], 8) if b[k] is None else b[k] for b in blocks]
+        assert torch.equal(torch.cat(parts), torch.cat(want))
+
+
+def test_a_sharded_4_bit_module_knows_its_columns(monkeypatch):
+    monkeypatch.setattr(compact, "Tiles", lambda blocks, layout=None: SimpleNamespace(blocks=blocks))
+    block = ("int4", torch.zeros(200, 65, dtype=torch.uint8), torch.ones(200, 5, dtype=torch.bfloat16), None, 130, 32)
+    module = shard.ShardedCompact([block])
+    assert (module.rows, module.cols, module.mine) == (200, 130, 200) and module.local.tiles.blocks[0][1].shape == (200, 65)
