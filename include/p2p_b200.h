@@ -381,6 +381,13 @@ size_t p2p_int4_grouped_workspace(int64_t max_items, int64_t item_tokens, int64_
  * launch's y is undefined); reset != 0 clears it. Syncs the stream. */
 int p2p_int4_status(int reset, void* stream);
 
+/* Test of that give-up path: p2p_int4_mm in which every CTA withholds its x load number `hold` (0..4095; of one or two
+ * 128-column steps each), so that the waits for it run out after wait_us (1000..2000000). The launch drains what it issued
+ * and ends; y is undefined. */
+int p2p_int4_withhold(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout, int has_zeros,
+                      int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                      int64_t hold, int64_t wait_us, void* stream);
+
 /* ------------------------------------------------------------------------------------------------------------------
  * (2e) Tokens sorted by expert and back, all on the device (p2p_moe_route's counts go to the host)
  * ------------------------------------------------------------------------------------------------------------------ */

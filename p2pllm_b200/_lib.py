@@ -85,6 +85,8 @@ SIGNATURES = {
     "p2p_int4_workspace": ([_i64, _i64, _i64, _int], _sz),
     "p2p_int4_mm": ([_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _i64, _vp, _sz, _vp], _int),
     "p2p_int4_status": ([_int, _vp], _int),
+    "p2p_int4_withhold": ([_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _i64, _vp, _sz, _i64, _i64, _vp],
+                          _int),
     "p2p_int4_grouped": ([_vp, _int, _i64, _i64, _vp, _int, _i64, _int, _int, _vp, _vp, _i64, _i64, _vp, _int, _vp, _i64,
                           _vp, _i64, _vp, _sz, _vp], _int),
     "p2p_int4_grouped_workspace": ([_i64, _i64, _i64, _i64, _int], _sz),

@@ -150,7 +150,6 @@ constexpr int kComputeWarps = 8;                       // one a row block of the
 constexpr int kSmallThreads = (kComputeWarps + 1) * 32;
 constexpr int kMaxSlots = 8;
 constexpr int kRowPad = 132;                           // floats a token of the partial tile: 128 rows, padded
-constexpr uint64_t kSmallWaitNs = 2000000000ull;
 
 __device__ int g_small_error;            // site of the first wait that gave up since the last reset (0: none)
 __device__ unsigned g_small_failed_seq;  // sequence number of the last launch in which a wait gave up
@@ -172,6 +171,7 @@ struct SmallParams {
     int topk;
     const int32_t* routed;              // not null: output rows from *routed to pairs become zero
     int64_t pairs;
+    int hold;                           // a test's withheld slot: neither its weights nor its x are loaded; -1: none
     uint64_t wait_ns;
     unsigned seq;
 };
@@ -330,12 +330,13 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
             int u = u0;
             if (!p.items) {
                 // the ring's first fill: weights, then, once the previous kernel has ended, x
+                const int fill = p.hold >= 0 ? min(p.hold, n_slots) : n_slots;
                 for (int pass = 0; pass < 2; ++pass) {
                     int i = 0;
-                    for (u = u0; u < u1 && i < n_slots;) {
+                    for (u = u0; u < u1 && i < fill;) {
                         const SmallTile t = small_tile(p, u / p.units);
                         const int kz = min(p.units, u % p.units + (u1 - u));
-                        for (int k = u % p.units; k < kz && i < n_slots; ++i) {
+                        for (int k = u % p.units; k < kz && i < fill; ++i) {
                             const int n = min(2, kz - k);
                             if (pass == 0) load_w(i, t, k, n); else load_x(i, t, k, n);
                             k += n;
@@ -353,6 +354,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
                 const int kz = min(p.units, u % p.units + (u1 - u));
                 pick(t);
                 for (int k = u % p.units; k < kz;) {
+                    if (!(ok = used != p.hold)) break;               // a test withholds this load
                     if (used >= n_slots && !(ok = wait_one(empty(slot), ph ^ 1u, 1, wc))) break;
                     const int n = min(2, kz - k);
                     load_w(slot, t, k, n);
@@ -712,7 +714,8 @@ int run_small(const Int4Call& c, const int32_t* order, int topk, void* workspace
     p.topk = topk;
     p.routed = c.routed;
     p.pairs = c.pairs;
-    p.wait_ns = kSmallWaitNs;
+    p.hold = c.hold;
+    p.wait_ns = c.wait_ns;
     p.seq = next_seq();
     const int64_t x_rows = order ? c.pairs / topk : c.items ? c.pairs : c.tokens;
     CUtensorMap map;
@@ -825,12 +828,13 @@ extern "C" size_t p2p_int4_grouped_workspace(int64_t max_items, int64_t item_tok
     return plan_small(c).workspace;
 }
 
-extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout,
-                           int has_zeros, int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace,
-                           size_t workspace_bytes, void* stream) {
+namespace {
+// p2p_int4_mm on a call that brings a test's withheld load and wait limit, or their defaults.
+int int4_mm(Int4Call c, const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout,
+            int has_zeros, int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace,
+            size_t workspace_bytes, void* stream) {
     P2P_REQUIRE(tokens >= 0 && rows >= 0 && tokens <= 0x7fffffff, "p2p_int4_mm: bad shape");
     if (tokens == 0 || rows == 0) return P2P_OK;
-    Int4Call c = {};
     c.x = x; c.dtype = dtype; c.tokens = tokens; c.cols = cols; c.ldx = ldx;
     c.layout = layout; c.has_zeros = has_zeros != 0;
     c.rows = rows; c.group = group; c.gated = gated != 0; c.y = y; c.ldy = ldy;
@@ -843,6 +847,27 @@ extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t col
         return dtype == P2P_BF16 ? run_small<__nv_bfloat16>(c, nullptr, 1, workspace, st, "p2p_int4_mm")
                                  : run_small<__half>(c, nullptr, 1, workspace, st, "p2p_int4_mm");
     return int4_tc_run(c, workspace, st, "p2p_int4_mm");
+}
+}  // namespace
+
+extern "C" int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout,
+                           int has_zeros, int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+    return int4_mm({}, x, dtype, tokens, cols, ldx, layout, has_zeros, rows, group, gated, y, ldy, workspace,
+                   workspace_bytes, stream);
+}
+
+extern "C" int p2p_int4_withhold(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout,
+                                 int has_zeros, int64_t rows, int group, int gated, void* y, int64_t ldy,
+                                 void* workspace, size_t workspace_bytes, int64_t hold, int64_t wait_us, void* stream) {
+    P2P_REQUIRE(hold >= 0 && hold < 4096, "p2p_int4_withhold: load %lld", (long long)hold);
+    P2P_REQUIRE(wait_us >= 1000 && wait_us <= 2000000, "p2p_int4_withhold: a limit of 1 ms to 2 s (%lld us)",
+                (long long)wait_us);
+    Int4Call c = {};
+    c.hold = (int)hold;
+    c.wait_ns = (uint64_t)wait_us * 1000ull;
+    return int4_mm(c, x, dtype, tokens, cols, ldx, layout, has_zeros, rows, group, gated, y, ldy, workspace,
+                   workspace_bytes, stream);
 }
 
 extern "C" int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout,

@@ -129,12 +129,13 @@ struct Runs {
 }  // namespace q4
 namespace sm100 {
 
-// mbar_wait, with many tests of the phase between two looks at the clock and the failure flag: each look takes about a
-// microsecond, which a hand-over between two roles cannot wait for.
+// mbar_wait, with many tests of the phase before it looks at the clock and the failure flag: each such look takes about a
+// microsecond, which a hand-over between two roles cannot wait for. A test sleeps for at most two microseconds, so all of
+// them last a millisecond: the limit starts, and another wait's failure is seen, that much later at most.
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int site, const WaitCtl& wc) {
 #pragma unroll 1
-    for (int i = 0; i < 4096; ++i)
-        if (mbar_try(bar, parity)) return true;
+    for (int i = 0; i < 512; ++i)
+        if (mbar_try<2000u>(bar, parity)) return true;
     return mbar_wait(bar, parity, site, wc);
 }
 

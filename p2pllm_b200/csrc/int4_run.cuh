@@ -19,6 +19,8 @@ struct Int4Call {
     const int32_t *items, *n_items;     // routed: x's rows are the places
     int64_t max_items, item_tokens, pairs;
     const int32_t* routed;              // not null: y's rows from *routed to pairs become zero
+    int hold = -1;                      // a test's withheld x load (each CTA's load of that number is never issued), or -1
+    uint64_t wait_ns = 2000000000ull;   // how long a pipeline wait may take before the launch gives up
 };
 
 // Bytes of workspace int4_tc_run needs for a dense call.

@@ -66,7 +66,6 @@ constexpr int kTmemCols = 512;
 constexpr int kMaxW = 12, kMaxX = 8, kMaxA = 6, kMaxBuf = 4, kMaxPieces = 4;
 constexpr int kSSlots = 16;                             // scales wait for the rings before them: more than W + A slots hold
 constexpr int kSmemLimit = 227 * 1024 - 1024;
-constexpr uint64_t kWaitNs = 2000000000ull;
 
 __device__ int g_int4_error;            // site of the first wait that gave up since the last reset (0: none)
 __device__ unsigned g_int4_failed_seq;  // sequence number of the last launch in which a wait gave up
@@ -85,6 +84,7 @@ struct TcParams {
     float* partial;                     // [ctas][2][n_max][128]; null: every CTA takes whole row tiles
     int n_max, ctas;
     int x_rows, box_rows, w_slots, x_slots, a_slots, bufs, a_col0;
+    int hold;                           // a test's withheld x tile; -1: none
     uint64_t wait_ns;
     unsigned seq;
 };
@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                     const Tile t = tile_at(p, u, u1);
                     const int boxes = (n_total(t.n) + p.box_rows - 1) / p.box_rows;
                     for (int k = t.k0; k < t.k1; ++k) {
+                        if (!(ok = used != p.hold)) break;           // a test withholds this load
                         if (used >= SX && !(ok = wait_one(xempty(slot), ph ^ 1u, 3, wc))) break;
                         mbar_expect_tx(xfull(slot), (uint32_t)(2 * boxes * p.box_rows) * 128u);
                         for (int b = 0; b < boxes; ++b)
@@ -801,7 +802,8 @@ int int4_tc_run(const Int4Call& c, void* workspace, cudaStream_t st, const char*
     p.a_slots = pl.a_slots;
     p.bufs = pl.bufs;
     p.a_col0 = pl.a_col0;
-    p.wait_ns = kWaitNs;
+    p.hold = c.hold;
+    p.wait_ns = c.wait_ns;
     p.seq = next_seq();
     CUtensorMap map;
     if (int e = encode_x_map(&map, c.x, c.dtype, routed ? c.pairs : c.tokens, c.cols, c.ldx, pl.box_rows)) return e;

@@ -47,14 +47,14 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 
 // One test of the phase; a thread whose phase is not complete sleeps in hardware (up to the suspend-time hint, in ns)
 // until it completes, instead of spinning on the issue slots its warp scheduler shares with working warps.
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+template <uint32_t HINT_NS = 1000000u> __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(1000000u)
+        : "r"(bar), "r"(parity), "r"(HINT_NS)
         : "memory");
     return ok != 0;
 }

@@ -428,6 +428,22 @@ def int4_status(device=None, reset: bool = True) -> None:
         call("p2p_int4_status", int(reset), torch.cuda.current_stream(dev).cuda_stream)
 
 
+def int4_withhold(layout, x: torch.Tensor, hold: int, wait_us: int) -> torch.Tensor:
+    """A dense 4-bit product (layout: int4.Layout) in which every CTA withholds its x load number `hold`, so the pipeline's
+    bounded waits run out after wait_us: the give-up path under test. y is undefined; int4_status reports it."""
+    layout.check_x(x)
+    x = x.contiguous()
+    rows = layout.rows // 2 if layout.gated else layout.rows
+    out = torch.zeros(x.shape[0], rows, dtype=x.dtype, device=x.device)
+    need = _lib.load().p2p_int4_workspace(x.shape[0], layout.rows, layout.cols, layout.gated)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        call("p2p_int4_withhold", ptr(x), dtype_code(x), x.shape[0], layout.cols, x.stride(0), ptr(layout.data),
+             layout.has_zeros, layout.rows, layout.group, layout.gated, ptr(out), out.stride(0), ptr(ws), need, hold,
+             wait_us, stream_of(x))
+    return out
+
+
 def _ptr_array(ts) -> ctypes.Array:
     arr = (ctypes.c_void_p * len(ts))()
     for i, t in enumerate(ts):

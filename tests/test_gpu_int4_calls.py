@@ -6,7 +6,7 @@ import pickle
 import pytest
 import torch
 
-from p2pllm_b200 import P2PError, _lib, compact, int4, moe, shard
+from p2pllm_b200 import P2PError, _lib, compact, int4, kernels, moe, shard
 from test_gpu_int4 import _block, _check_product, _dense64, _gen
 
 pytestmark = pytest.mark.gpu
@@ -133,3 +133,31 @@ def test_a_sharded_4_bit_module(tokens):
         mine = shard.shard_blocks(blocks, start, stop)
         compact.Tiles(mine)(x, out=y[:, start:stop])
         _check_product(y[:, start:stop], x, torch.cat([_dense64(b) for b in mine]), torch.bfloat16)
+
+
+@pytest.mark.parametrize("tokens,rows,cols,hold", [
+    (1, 256, 4096, 0), (17, 256, 4096, 1), (17, 20000, 1024, 0), (32, 40000, 1024, 3), (40, 300, 4096, 0), (64, 20000, 2048, 3),
+    (100, 20000, 2048, 0), (150, 20000, 1024, 5), (190, 20000, 1024, 0), (190, 20000, 1024, 4), (272, 20000, 1024, 0),
+    (272, 20000, 1024, 6), (600, 300, 1024, 0)])
+def test_a_withheld_load_ends_the_launch_with_an_error_status(tokens, rows, cols, hold):
+    """Failure detection without a fault: every CTA withholds one load of x, so the waits for it run out after 20 ms. The
+    launch must end by itself and soon (a wait that does not see another's failure, or starts its limit late, takes
+    seconds), the status must name the wait that gave up, and the next launch is an ordinary one."""
+    import time
+    g = _gen(8)
+    block = _block((), rows, cols, 64, True, torch.bfloat16, g)
+    tiles = compact.Tiles([block])
+    x = torch.randn(tokens, cols, generator=g, device="cuda").bfloat16()
+    want = tiles(x)
+    kernels.int4_status()
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    kernels.int4_withhold(tiles.int4, x, hold=hold, wait_us=20000)
+    torch.cuda.synchronize()
+    elapsed = time.perf_counter() - t0
+    assert elapsed < 1.0, elapsed
+    with pytest.raises(P2PError, match="timed out"):
+        kernels.int4_status(reset=True)
+    kernels.int4_status()                                           # reset: clean again
+    assert torch.equal(tiles(x), want)
+    kernels.int4_status()

@@ -187,3 +187,10 @@ def test_a_sharded_4_bit_module_knows_its_columns(monkeypatch):
     block = ("int4", torch.zeros(200, 65, dtype=torch.uint8), torch.ones(200, 5, dtype=torch.bfloat16), None, 130, 32)
     module = shard.ShardedCompact([block])
     assert (module.rows, module.cols, module.mine) == (200, 130, 200) and module.local.tiles.blocks[0][1].shape == (200, 65)
+
+
+def test_withhold_test_entry_checks_its_limits(lib):
+    fake = 65536
+    for hold, limit, needle in ((0, 10, b"1 ms to 2 s"), (0, 3000000, b"1 ms to 2 s"), (-1, 5000, b"load"), (4096, 5000, b"load")):
+        assert lib.p2p_int4_withhold(fake, 0, 4, 64, 64, fake, 0, 16, 64, 0, fake, 16, None, 0, hold, limit, None) == -1
+        assert needle in lib.p2p_last_error()
