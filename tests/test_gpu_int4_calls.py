@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from p2pllm_b200 import P2PError, _lib, compact, int4, kernels, moe, shard
-from test_gpu_int4 import _block, _check_product, _dense64, _gen
+from test_gpu_int4 import DT, _block, _check_gated, _check_product, _dense64, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +161,59 @@ def test_a_withheld_load_ends_the_launch_with_an_error_status(tokens, rows, cols
     kernels.int4_status()                                           # reset: clean again
     assert torch.equal(tiles(x), want)
     kernels.int4_status()
+
+
+# Every width of the tensor-core product: its accumulators' spacing is the tokens of a tile in steps of 16.
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens,rows,cols", [
+    (34, 260, 640), (49, 4098, 321), (113, 300, 640), (129, 260, 1030), (145, 20000, 257), (160, 300, 640), (161, 300, 640),
+    (177, 260, 1030), (192, 20000, 257), (193, 300, 640), (225, 260, 321), (257, 300, 640), (340, 300, 640), (384, 20000, 257),
+    (385, 260, 640), (545, 300, 321)])
+def test_products_of_every_width(tokens, rows, cols, gated, group, zeros, dtype):
+    g = _gen(tokens * 1009 + rows)
+    block = _block((), rows, cols, group, zeros, DT[dtype], g)
+    if gated:
+        x = (torch.randn(tokens, cols, generator=g, device="cuda") / cols ** 0.5).to(DT[dtype])
+        _check_gated(compact.GatedTiles([block])(x), x, _dense64(block), DT[dtype])
+    else:
+        x = torch.randn(tokens, cols, generator=g, device="cuda").to(DT[dtype])
+        _check_product(compact.Tiles([block])(x), x, _dense64(block), DT[dtype])
+
+
+def _skewed(tokens, topk, experts, g, power):
+    """Ids of which the low ones come up often and the high ones hardly ever, a tenth of the pairs nowhere."""
+    ids = (torch.rand(tokens, topk, generator=g, device="cuda") ** power * experts).long().clamp(max=experts - 1)
+    return torch.where(torch.rand(tokens, topk, generator=g, device="cuda") < 0.1, -1, ids)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("tokens,topk,experts,rows,cols,group,zeros,power", [
+    (40, 1, 8, 66, 130, 32, True, 3),                                # items of 16 places, some experts with one pair or none
+    (300, 2, 40, 66, 130, 64, False, 3),                             # 32
+    (280, 4, 32, 130, 257, 32, True, 6),                             # 64, one expert with most of the pairs
+    (250, 8, 25, 66, 320, 128, True, 4),                             # 128
+    (260, 3, 7, 130, 257, 32, True, 1), (440, 4, 16, 300, 640, 128, False, 5),          # 160
+    (500, 3, 8, 130, 257, 32, True, 1), (700, 4, 12, 300, 640, 64, True, 6), (1100, 1, 4, 66, 96, 128, False, 2),   # 256
+    (600, 2, 3, 260, 1030, 32, False, 1)])
+def test_experts_items_of_every_size(tokens, topk, experts, rows, cols, group, zeros, power, gather, gated, dtype):
+    g = _gen(tokens + rows)
+    block = _block((experts,), rows, cols, group, zeros, DT[dtype], g)
+    order = moe.sort_tokens(_skewed(tokens, topk, experts, g, power), experts)
+    x = torch.randn(tokens if gather else tokens * topk, cols, generator=g, device="cuda")
+    x = (x / cols ** 0.5 if gated else x).to(DT[dtype])
+    tiles = moe.Int4Experts([block], gated=gated)
+    y = tiles(x, order, gather=gather)
+    w, offsets = _dense64(block), order.offsets.tolist()
+    xs = x[(order.order.clamp(min=0) // topk).long()] if gather else x
+    for e in range(experts):
+        a, b = offsets[e], offsets[e + 1]
+        if a < b:
+            (_check_gated if gated else _check_product)(y[a:b], xs[a:b], w[e], DT[dtype])
+    assert bool((y[offsets[-1]:] == 0).all())
+    out = torch.full_like(y, 5.0)
+    tiles(x, order, gather=gather, out=out)
+    assert torch.equal(out[:offsets[-1]], y[:offsets[-1]]) and bool((out[offsets[-1]:] == 5.0).all())
