@@ -167,19 +167,17 @@ def from_experts(y: torch.Tensor, order: TokenOrder, weights: torch.Tensor | Non
     """[T, H]: per token the sum over its slots, in slot order and fp32, of weights[t, j] times the slot's row of
     y [T K, H] (no weights: 1); slots routed nowhere add nothing. Gradients for y (zero behind the last pair) and for
     weights [T, K] (bfloat16, float16 or float32)."""
-    if weights is None or weights.dim() == 2:
-        try:                                        # the operator makes the same checks, at less cost
-            return _lib.ops().moe_sum(y, order.where, order.offsets, weights, order.topk)
-        except RuntimeError:
-            pass
-    _check_rows(y, order, order.tokens * order.topk)
-    if weights is not None:
-        require_cuda(weights)
-        if tuple(weights.shape) != (order.tokens, order.topk) or weights.device != order.device:
-            raise P2PError(f"weights of {tuple(weights.shape)} on {weights.device}, wanted "
-                           f"{(order.tokens, order.topk)} on {order.device}")
-        dtype_code(weights)
-    return _lib.ops().moe_sum(y, order.where, order.offsets, weights, order.topk)
+    try:                                            # the operator makes the same checks, at less cost
+        return _lib.ops().moe_sum(y, order.where, order.offsets, weights, order.topk)
+    except RuntimeError:
+        _check_rows(y, order, order.tokens * order.topk)
+        if weights is not None:
+            require_cuda(weights)
+            if tuple(weights.shape) != (order.tokens, order.topk) or weights.device != order.device:
+                raise P2PError(f"weights of {tuple(weights.shape)} on {weights.device}, wanted "
+                               f"{(order.tokens, order.topk)} on {order.device}") from None
+            dtype_code(weights)
+        raise
 
 
 class Int4Experts:

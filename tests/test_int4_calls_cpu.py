@@ -194,3 +194,26 @@ def test_withhold_test_entry_checks_its_limits(lib):
     for hold, limit, needle in ((0, 10, b"1 ms to 2 s"), (0, 3000000, b"1 ms to 2 s"), (-1, 5000, b"load"), (4096, 5000, b"load")):
         assert lib.p2p_int4_withhold(fake, 0, 4, 64, 64, fake, 0, 16, 64, 0, fake, 16, None, 0, hold, limit, None) == -1
         assert needle in lib.p2p_last_error()
+
+
+@pytest.mark.parametrize("call", ["to_experts", "from_experts", "mm"])
+def test_a_call_that_fails_is_not_made_again(monkeypatch, call):
+    """Out of memory, say: raised once and as it is."""
+    tried = []
+
+    def fail(*a):
+        tried.append(1)
+        raise torch.OutOfMemoryError("no room")
+    monkeypatch.setattr(_lib, "ops", lambda: SimpleNamespace(moe_spread=fail, moe_sum=fail))
+    for module in (moe, int4):
+        monkeypatch.setattr(module, "require_cuda", lambda *ts: None)
+    where = torch.zeros(6, dtype=torch.int32)
+    order = moe.TokenOrder(where, where, torch.zeros(5, dtype=torch.int32), where, where, 3, 2)
+    layout = _layout()
+    layout.device, layout.cols, layout._op = torch.device("cpu"), 4, fail
+    run = {"to_experts": lambda: moe.to_experts(torch.zeros(3, 8), order),
+           "from_experts": lambda: moe.from_experts(torch.zeros(6, 8), order, torch.zeros(3, 2)),
+           "mm": lambda: layout.mm(torch.zeros(3, 4, dtype=torch.bfloat16))}[call]
+    with pytest.raises(torch.OutOfMemoryError, match="no room"):
+        run()
+    assert len(tried) == 1
