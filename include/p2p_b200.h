@@ -395,14 +395,14 @@ int p2p_int4_withhold(const void* x, int dtype, int64_t tokens, int64_t cols, in
 /* ids [n_pairs] (32- or 64-bit: ids_bytes) of (token, slot) pairs; an id outside 0..experts - 1 is routed nowhere.
  * order [n_pairs]: the routed pairs sorted by expert, those of one expert in their own order, then -1; where
  * [n_pairs]: each pair's place in it, or -1; offsets [experts + 1]: each expert's first place, the last one the number
- * of routed pairs; items [max_items, 4]: {expert, first place, places, 0}, runs of at most item_tokens places of one
- * expert, and n_items [1] their number. max_items >= min(n_pairs, ceil(n_pairs / item_tokens) + experts); at most 1024
+ * of routed pairs; items [max_items, 4]: {expert, first place, places, 0}, runs of at most item_tokens (1..65536) places
+ * of one expert, and n_items [1] their number. max_items >= min(n_pairs, ceil(n_pairs / item_tokens) + experts); at most 1024
  * experts. One launch, deterministic. */
 int p2p_moe_sort(const void* ids, int ids_bytes, int64_t n_pairs, int experts, int32_t* order, int32_t* where,
                  int32_t* offsets, int32_t* items, int64_t max_items, int item_tokens, int32_t* n_items, void* stream);
 
 /* out [tokens * k, hidden]: row where[t * k + j] = x[t] for every routed pair; rows from *routed (offsets[experts]) on
- * are zero. dtype bf16, f16 or f32. */
+ * are zero. dtype bf16, f16 or f32; here and below at most 2^30 columns. */
 int p2p_moe_spread(const void* x, int dtype, int64_t tokens, int k, int64_t hidden, int64_t ldx, const int32_t* where,
                    const int32_t* routed, void* out, int64_t ldo, void* stream);
 

@@ -440,7 +440,8 @@ int run_rows(RowOp op, RowParams& p, int dtype, int64_t hidden, cudaStream_t st,
 
 int check_rows(const char* what, int dtype, int64_t tokens, int k, int64_t hidden) {
     if (!dtype_ok(dtype)) return fail(P2P_EUNSUPPORTED, "%s: bf16, f16 or f32", what);
-    P2P_REQUIRE(tokens >= 0 && k >= 1 && hidden >= 1 && hidden <= 0x7fffffff && tokens <= 0x7fffffff / k,
+    // 2^30 columns: a column's number plus one step of the whole grid stays below 2^31
+    P2P_REQUIRE(tokens >= 0 && k >= 1 && hidden >= 1 && hidden <= 0x40000000 && tokens <= 0x7fffffff / k,
                 "%s: bad shape (%lld tokens, %d slots, %lld columns)", what, (long long)tokens, k, (long long)hidden);
     return P2P_OK;
 }
@@ -453,7 +454,7 @@ using namespace p2p;
 extern "C" int p2p_moe_sort(const void* ids, int ids_bytes, int64_t n_pairs, int experts, int32_t* order,
                             int32_t* where, int32_t* offsets, int32_t* items, int64_t max_items, int item_tokens,
                             int32_t* n_items, void* stream) {
-    P2P_REQUIRE(n_pairs >= 0 && n_pairs <= 0x7fffffff - 65536 && experts >= 1 && item_tokens >= 1,
+    P2P_REQUIRE(n_pairs >= 0 && n_pairs <= 0x7fffffff - 65536 && experts >= 1 && item_tokens >= 1 && item_tokens <= 65536,
                 "p2p_moe_sort: %lld pairs, %d experts, items of %d", (long long)n_pairs, experts, item_tokens);
     if (experts > kSortExperts)
         return fail(P2P_EUNSUPPORTED, "p2p_moe_sort: %d experts, at most %d", experts, kSortExperts);

@@ -217,3 +217,14 @@ def test_a_call_that_fails_is_not_made_again(monkeypatch, call):
     with pytest.raises(torch.OutOfMemoryError, match="no room"):
         run()
     assert len(tried) == 1
+
+
+@pytest.mark.parametrize("call", [
+    lambda l, f: l.p2p_moe_spread(f, 0, 1, 1, 2 ** 30 + 1, 2 ** 30 + 1, f, f, f, 2 ** 30 + 1, None),
+    lambda l, f: l.p2p_moe_sum(f, 0, 1, 1, 2 ** 31 - 1, 2 ** 31 - 1, f, None, 2, f, 2 ** 31 - 1, None),
+    lambda l, f: l.p2p_moe_sum_back(f, f, 0, 1, 1, 2 ** 31 - 1, 2 ** 31, 2 ** 31, f, f, f, 2, f, 2 ** 31, f, None),
+    lambda l, f: l.p2p_moe_sort(f, 4, 64, 8, f, f, f, f, 64, 2 ** 31 - 1, f, None)])
+def test_sizes_whose_counters_would_pass_32_bits_are_refused(lib, call):
+    """A column's number steps by the grid, an item's pairs are rounded up: both in 32 bits."""
+    assert call(lib, 65536) == -1
+    assert b"columns" in lib.p2p_last_error() or b"items of" in lib.p2p_last_error()
