@@ -157,7 +157,7 @@ __device__ unsigned g_small_failed_seq;  // sequence number of the last launch i
 struct SmallParams {
     const uint8_t* layout;
     int record, zeros, scales_at;       // bytes of a unit's record; whether it holds zero points; where its scales start
-    int units, row_tiles, col_tiles, group_shift, gated;
+    int units, row_tiles, group_shift, gated;
     int tokens, n_max, out_rows;        // n_max: tokens of a tile, at most
     int splits;                         // > 0: CTAs of a cluster, each with its share of one row tile; 0: runs
     float* partial;                     // runs: [ctas][2][n_max][128], the row tiles a run shares with its neighbours
@@ -209,22 +209,22 @@ struct SmallTile {
 };
 __device__ __forceinline__ SmallTile small_tile(const SmallParams& p, int id) {
     SmallTile t;
-    const int col = id / p.row_tiles;                    // an item, or a tile of the tokens
-    t.rt = id - col * p.row_tiles;
+    const int item = id / p.row_tiles;                   // 0 of a dense call
+    t.rt = id - item * p.row_tiles;
     int64_t expert = 0;
     if (p.items) {
-        const int4 it = __ldcg(reinterpret_cast<const int4*>(p.items) + col);
+        const int4 it = __ldcg(reinterpret_cast<const int4*>(p.items) + item);
         expert = it.x;
         t.first = it.y;
         t.n = min(it.z, p.n_max);
     } else {
-        t.first = col * p.n_max;
-        t.n = min(p.n_max, p.tokens - t.first);
+        t.first = 0;
+        t.n = p.tokens;
     }
     t.records = p.layout + (expert * p.row_tiles + t.rt) * p.units * p.record;
     return t;
 }
-__device__ __forceinline__ int small_tiles(const SmallParams& p) { return (p.items ? *p.n_items : p.col_tiles) * p.row_tiles; }
+__device__ __forceinline__ int small_tiles(const SmallParams& p) { return (p.items ? *p.n_items : 1) * p.row_tiles; }
 // Runs of a launch: no more than it has units (routed launches learn that here), so that none is empty.
 __device__ __forceinline__ uint32_t small_runs(uint32_t units_all, uint32_t ctas) { return max(1u, min(ctas, units_all)); }
 
@@ -618,17 +618,16 @@ unsigned next_seq() {
 // 24; 128 experts on 17 tokens 78 to 100 us).
 struct SmallPlan {
     int nt, splits, ctas, slots, half_bytes, x_at, x_sub, smem;
-    int64_t col_tiles, tiles;
+    int64_t tiles;
     size_t workspace;
 };
 
 SmallPlan plan_small(const Int4Call& c) {
     SmallPlan pl = {};
     const bool routed = c.items != nullptr;
-    const int64_t most = routed ? c.item_tokens : c.tokens < 32 ? c.tokens : 32;
+    const int64_t most = routed ? c.item_tokens : c.tokens;
     pl.nt = (int)q4::div_up(most, 8);
-    pl.col_tiles = routed ? c.max_items : q4::div_up(c.tokens, pl.nt * 8);
-    pl.tiles = q4::row_tiles(c.rows, c.gated) * pl.col_tiles;
+    pl.tiles = q4::row_tiles(c.rows, c.gated) * (routed ? c.max_items : 1);
     const int64_t units = q4::div_up(c.cols, q4::kUnitCols), per_sm = 2, resident = per_sm * sm_count();
     if (pl.tiles * 2 <= resident) {
         // a power of two: clusters of three leave SMs empty
@@ -694,7 +693,6 @@ int run_small(const Int4Call& c, const int32_t* order, int topk, void* workspace
     p.scales_at = q4::kCodeBytes + q4::unit_zero_bytes(c.group, c.has_zeros);
     p.units = (int)q4::div_up(c.cols, q4::kUnitCols);
     p.row_tiles = (int)q4::row_tiles(c.rows, c.gated);
-    p.col_tiles = (int)pl.col_tiles;
     p.group_shift = c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
     p.gated = c.gated;
     p.tokens = (int)c.tokens;

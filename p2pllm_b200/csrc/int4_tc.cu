@@ -19,9 +19,9 @@
 //                       later, in another), ahead of the previous kernel's end and up to 12 units ahead of their use
 //   x                   TMA of each unit's x tile [tokens x 128] (two 64-column boxes, 128-byte swizzle)
 //   two warps (MMA)     one thread each issues tcgen05.mma kind::f16, A from TMEM, M = 128: a group's columns times a
-//                       piece of the tokens (quarters, halves, or all of few) into a zeroed accumulator, then a commit.
-//                       The warps take the even and the odd pieces, or of a single piece alternate units: a look at a
-//                       barrier costs an issuing thread 130 cycles even when it has nothing to wait for
+//                       piece of the tokens (quarters or halves) into a zeroed accumulator, then a commit. The warps take
+//                       the even and the odd pieces: a look at a barrier costs an issuing thread 130 cycles even when it
+//                       has nothing to wait for
 //
 // Measured (bf16, groups of 128): 28672 x 4096 at 272 tokens 80 us replayed from a graph (798 TFLOP/s; the product alone
 // would take 39 us at the measured rate); 128 experts of 1536 x 2048 on 2048 x 8 tokens 238 us (433 TFLOP/s; items are
@@ -54,10 +54,10 @@ constexpr int threads_of(int acc) { return (kPromoteWarps + build_groups(acc) * 
 // Registers a thread of promoting, building and other warps: what the launch gives (a whole register file over the
 // threads, in eights), dealt anew. 0: as launched.
 constexpr int promote_regs(int acc) { return acc >= 96 ? 200 : acc >= 64 ? 136 : 0; }
-constexpr int build_regs(int acc) { return acc >= 96 ? 64 : 64; }
+constexpr int kBuildRegs = 64;
 constexpr int other_regs(int acc) { return acc >= 96 ? 40 : 48; }
 constexpr int dealt_regs(int acc) {
-    return kPromoteWarps * 32 * promote_regs(acc) + build_groups(acc) * group_warps(acc) * 32 * build_regs(acc) + 128 * other_regs(acc);
+    return kPromoteWarps * 32 * promote_regs(acc) + build_groups(acc) * group_warps(acc) * 32 * kBuildRegs + 128 * other_regs(acc);
 }
 constexpr int kWSlotBytes = q4::kCodeBytes + 512;       // codes and up to four groups' zero points
 constexpr int kSSlotBytes = 1024;                       // up to four groups' scales
@@ -172,10 +172,9 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int u, int u1) {
     }
     return t;
 }
-// Pieces of the tokens, each a multiple of 16: all of them up to 32, halves up to 160, quarters above. (An accumulator
-// that is read out cannot take products: with four pieces three multiply meanwhile.)
+// Pieces of the tokens, each a multiple of 16: halves up to 160 tokens, quarters above. (An accumulator that is read out
+// cannot take products: with four pieces three multiply meanwhile.)
 __host__ __device__ constexpr int n_total(int n) { return (n + 15) & ~15; }
-__host__ __device__ constexpr int pieces_of(int n_max) { return n_max <= 32 ? 1 : n_max <= 160 ? 2 : 4; }
 template <int PIECES> __device__ __forceinline__ int piece_size(int n, int i) { return (n_total(n) / 16 - i + PIECES - 1) / PIECES * 16; }
 template <int PIECES> __device__ __forceinline__ int piece_begin(int n, int i) {
     int at = 0;
@@ -190,6 +189,7 @@ template <typename T, int PIECES, int W0, int W1>
 __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                               const __grid_constant__ TcParams p) {
     // The promoting warps need an accumulator of up to 144 registers and take what the others give back.
+    static_assert(PIECES == 2 || (PIECES == 4 && W1 > 0), "one or two pieces for each half of the promoting warps");
     constexpr int kAcc = W0 + W1, kGroups = build_groups(kAcc), kGroupWarps = group_warps(kAcc);
     constexpr bool kSplitRegs = promote_regs(kAcc) > 0;
     constexpr bool kStaged = kAcc > 32;                  // sums leave through tensor memory
@@ -220,11 +220,11 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < SW; ++s) { mbar_init(wfull(s), 1); mbar_init(wempty(s), kGroupWarps); }
-        for (int s = 0; s < SX; ++s) { mbar_init(xfull(s), 1); mbar_init(xempty(s), PIECES == 1 ? 1 : 2); }
-        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kGroupWarps); mbar_init(aempty(s), PIECES == 1 ? 1 : 2); }
+        for (int s = 0; s < SX; ++s) { mbar_init(xfull(s), 1); mbar_init(xempty(s), 2); }
+        for (int s = 0; s < SA; ++s) { mbar_init(afull(s), kGroupWarps); mbar_init(aempty(s), 2); }
         for (int b = 0; b < NB; ++b)
             for (int i = 0; i < kMaxPieces; ++i) { mbar_init(dfull(i, b), 1); mbar_init(dempty(i, b), 4); }
-        for (int s = 0; s < kSSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), PIECES == 1 ? 4 : kPromoteWarps); }
+        for (int s = 0; s < kSSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), kPromoteWarps); }
         mbar_init(done, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -308,26 +308,23 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
         } else {
             const int h = warp - kMmaWarp;
             if (elect_one()) {
-                // a single piece's units alternate between the two warps, which then skip every other slot and buffer
-                constexpr int kStride = PIECES == 1 ? 2 : 1;
                 int sa = 0, sx = 0, sb = 0, jobs = 0;
                 uint32_t pha = 0, phx = 0, phb = 0;
                 bool ok = true;
                 const uint64_t x_desc = sw128_desc(x_ring);
-                const uint32_t d0 = tmem + d_col(PIECES == 1 ? 0 : h, 0), d1 = tmem + d_col(h + 2, 0);
+                const uint32_t d0 = tmem + d_col(h, 0), d1 = tmem + d_col(h + 2, 0);
                 // one unit: SUBS groups of 8 / SUBS products of K = 16 for each of this warp's pieces
                 auto unit = [&](auto subs_, uint32_t id0, uint32_t id1, uint32_t row0, uint32_t row1) {
                     constexpr int SUBS = decltype(subs_)::value, STEPS = 8 / SUBS;
                     const uint32_t a = tmem + (uint32_t)(p.a_col0 + sa * kACols);
                     const uint64_t b0 = x_desc + (uint64_t)((uint32_t)(sx * x_bytes) >> 4);
                     const uint64_t b1 = b0 + (uint64_t)(sub_bytes >> 4);
-                    const int first = PIECES == 1 ? 0 : h;
 #pragma unroll
                     for (int s = 0; s < SUBS; ++s) {
                         if (s == 0) {
-                            if (!(ok = wait_three(afull(sa), pha, xfull(sx), phx, dempty(first, sb), phb ^ 1u, jobs >= NB, 5, wc))) return;
+                            if (!(ok = wait_three(afull(sa), pha, xfull(sx), phx, dempty(h, sb), phb ^ 1u, jobs >= NB, 5, wc))) return;
                         } else {
-                            if (jobs >= NB && !(ok = wait_one(dempty(first, sb), phb ^ 1u, 7, wc))) return;
+                            if (jobs >= NB && !(ok = wait_one(dempty(h, sb), phb ^ 1u, 7, wc))) return;
                         }
                         tc_fence_after();
                         auto piece = [&](uint32_t d, uint32_t row, uint32_t id) {
@@ -339,7 +336,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                             }
                         };
                         piece(d0 + sb * p.n_max, row0, id0);
-                        umma_commit(dfull(first, sb));
+                        umma_commit(dfull(h, sb));
                         if constexpr (PIECES == 4) {
                             if (jobs >= NB && !(ok = wait_one(dempty(h + 2, sb), phb ^ 1u, 7, wc))) return;
                             tc_fence_after();
@@ -350,22 +347,13 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                         advance(sb, phb, 1, NB);
                     }
                 };
-                auto skip = [&] {                        // the other warp's unit
-                    advance(sa, pha, 1, SA);
-                    advance(sx, phx, 1, SX);
-                    for (int s = 0; s < subs; ++s) advance(sb, phb, 1, NB);
-                    jobs += subs;
-                };
-                if (PIECES == 1 && h) skip();
                 for (int u = u0; u < u1 && ok;) {
                     const Tile t = tile_at(p, u, u1);
-                    const int n0 = piece_size<PIECES>(t.n, PIECES == 1 ? 0 : h), n1 = PIECES == 4 ? piece_size<PIECES>(t.n, h + 2) : 0;
+                    const int n0 = piece_size<PIECES>(t.n, h), n1 = PIECES == 4 ? piece_size<PIECES>(t.n, h + 2) : 0;
                     const uint32_t id0 = n0 > 0 ? idesc_f16<T>(n0) : 0u, id1 = n1 > 0 ? idesc_f16<T>(n1) : 0u;
-                    const uint32_t row0 = (uint32_t)(piece_begin<PIECES>(t.n, PIECES == 1 ? 0 : h) * 128) >> 4;
+                    const uint32_t row0 = (uint32_t)(piece_begin<PIECES>(t.n, h) * 128) >> 4;
                     const uint32_t row1 = (uint32_t)(piece_begin<PIECES>(t.n, h + 2) * 128) >> 4;
-                    int k = t.k0;
-                    if (PIECES == 1) k += (int)((u - u0 + h) & 1);
-                    for (; k < t.k1; k += kStride) {
+                    for (int k = t.k0; k < t.k1; ++k) {
                         if (subs == 1) unit(std::integral_constant<int, 1>(), id0, id1, row0, row1);
                         else if (subs == 2) unit(std::integral_constant<int, 2>(), id0, id1, row0, row1);
                         else unit(std::integral_constant<int, 4>(), id0, id1, row0, row1);
@@ -374,7 +362,6 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                         umma_commit(xempty(sx));
                         advance(sa, pha, 1, SA);
                         advance(sx, phx, 1, SX);
-                        if (PIECES == 1) skip();
                     }
                     u += t.k1 - t.k0;
                 }
@@ -384,7 +371,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
             __syncwarp();
         }
     } else if (warp >= kBuildWarp) {
-        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(build_regs(kAcc)));
+        if (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBuildRegs));
         const int group = (warp - kBuildWarp) / kGroupWarps, w = (warp - kBuildWarp) % kGroupWarps;
         constexpr int kBlocks = 8 / kGroupWarps;                                // row blocks a warp builds
         const int blk0 = 2 * (w & 3) + (kBlocks == 1 ? w >> 2 : 0);             // lanes 32 (w % 4).. are this warp's
@@ -443,7 +430,7 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
         int sb = 0, ss = 0;
         uint32_t phb = 0, phs = 0;
         bool ok = true;
-        for (int u = u0; u < u1 && ok && h < PIECES;) {
+        for (int u = u0; u < u1 && ok;) {
             const Tile t = tile_at(p, u, u1);
             const int size[2] = {piece_size<PIECES>(t.n, h), W1 ? piece_size<PIECES>(t.n, h + 2) : 0};
             uint64_t acc[(W0 + W1) / 2];
@@ -728,7 +715,6 @@ template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMa
 }
 
 template <typename T> int launch_width(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
-    if (p.n_max <= 32) return launch_tc<T, 1, 32, 0>(map, p, smem, st, what);
     if (p.n_max <= 64) return launch_tc<T, 2, 32, 0>(map, p, smem, st, what);
     if (p.n_max <= 128) return launch_tc<T, 2, 64, 0>(map, p, smem, st, what);
     if (p.n_max <= 160) return launch_tc<T, 2, 80, 0>(map, p, smem, st, what);
