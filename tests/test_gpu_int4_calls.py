@@ -6,8 +6,8 @@ import pickle
 import pytest
 import torch
 
-from p2pllm_b200 import P2PError, _lib, compact, int4, kernels, moe, shard
-from test_gpu_int4 import DT, _block, _check_gated, _check_product, _dense64, _gen
+from p2pllm_b200 import P2PError, _lib, compact, int4, kernels, moe, prepare, shard
+from test_gpu_int4 import DT, Dispatch, TopK, _block, _check_gated, _check_product, _dense64, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,89 @@ def test_experts_items_of_every_size(tokens, topk, experts, rows, cols, group, z
     out = torch.full_like(y, 5.0)
     tiles(x, order, gather=gather, out=out)
     assert torch.equal(out[:offsets[-1]], y[:offsets[-1]]) and bool((out[offsets[-1]:] == 5.0).all())
+
+
+class _Experts(torch.nn.Module):
+    def __init__(self, E, R, H, g):
+        super().__init__()
+        rand = lambda *s: torch.nn.Parameter((torch.randn(*s, generator=g, device="cuda") * 0.1).bfloat16(), False)
+        self.w13_weight, self.w2_weight = rand(E, 2 * R, H), rand(E, H, R)
+
+
+def _expert_model(E, R, H, seed):
+    """One layer of routed experts beside two plain projections, of a seed."""
+    g, nn = _gen(seed), torch.nn
+    layer = nn.Module()
+    layer.mlp = nn.Module()
+    layer.mlp.experts = _Experts(E, R, H, g)
+    for name, shape in (("gate_proj", (R, H)), ("down_proj", (H, R))):
+        linear = nn.Module()
+        linear.weight = nn.Parameter(torch.randn(shape, generator=g, device="cuda").bfloat16(), False)
+        setattr(layer.mlp, name, linear)
+    model = nn.Module()
+    model.layers = nn.ModuleList([layer])
+    return model
+
+
+class _DenseMethod:
+    """A layer's own method on whatever expert weights it is given, in 32 bits."""
+
+    def apply(self, layer, d):
+        t, out = d.topk_output, 0
+        for j in range(t.topk_ids.shape[1]):
+            gate, up = torch.einsum("trh,th->tr", layer.w13_weight[t.topk_ids[:, j]].float(), d.hidden_states.float()).chunk(2, -1)
+            h = torch.nn.functional.silu(gate) * up
+            out = out + t.topk_weights[:, j:j + 1] * torch.einsum("thr,tr->th", layer.w2_weight[t.topk_ids[:, j]].float(), h)
+        return out
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_4_bit_files_of_routed_experts_install_in_every_form(tmp_path, zero_points):
+    """Dense rows written back, experts expanded in every pass, and experts multiplied in 4 bits. Bounds: the two weights
+    that are expanded are the same; the product in 4 bits rounds h, the experts' rows and the sums to bf16, at most half
+    a step each of its norm, and its weights not at all, where expanded ones are rounded once each: below 5 half steps."""
+    E, R, H, T, K = 6, 40, 64, 33, 2
+    g = _gen(9)
+    paths = prepare.write_int4(_expert_model(E, R, H, 5).layers, [0], str(tmp_path), group=32, zero_points=zero_points)
+    models = {}
+    for form in ("dense", "compact", "grouped"):
+        models[form] = _expert_model(E, R, H, 5)
+        models[form].layers[0].mlp.experts.quant_method = _DenseMethod()
+        prepare.install_replica(models[form], paths[0], form=form)
+    original = _expert_model(E, R, H, 5).layers[0].mlp.experts
+    dense = models["dense"].layers[0].mlp.experts
+    for name in ("w13_weight", "w2_weight"):
+        w = getattr(original, name)
+        halves = w.chunk(2, dim=1) if name == "w13_weight" else (w,)
+        want = torch.cat([int4.expand(int4.quantize(h, 32, zero_points)) for h in halves], dim=1)
+        assert torch.equal(getattr(dense, name), want)
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    ids = torch.randint(0, E - 1, (T, K), generator=g, device="cuda")               # one expert that no token reaches
+    weights = torch.rand(T, K, generator=g, device="cuda")
+    d = Dispatch(x, TopK(weights / weights.sum(-1, keepdim=True), ids))
+    want = _DenseMethod().apply(dense, d)
+    layers = {f: m.layers[0].mlp.experts for f, m in models.items()}
+    assert isinstance(layers["compact"].quant_method, compact.CompactMoE) and isinstance(layers["grouped"].quant_method, moe.GroupedMoE)
+    assert layers["grouped"].quant_method.is_int4 and layers["grouped"].w13_weight.numel() == 0
+    assert torch.equal(layers["compact"].quant_method.apply(layers["compact"], d), want)
+    got = layers["grouped"].quant_method.apply(layers["grouped"], d)
+    assert float((got.float() - want).norm() / want.norm()) <= 5 * torch.finfo(torch.bfloat16).eps / 2
+
+
+def test_calls_under_inference_mode():
+    g = _gen(10)
+    tiles = compact.Tiles([_block((), 40, 128, 64, True, torch.bfloat16, g)])
+    experts = moe.Int4Experts([_block((4,), 128, 128, 64, True, torch.bfloat16, g)])
+    x = torch.randn(9, 128, generator=g, device="cuda").bfloat16()
+    ids, w = torch.randint(0, 4, (9, 2), generator=g, device="cuda"), torch.rand(9, 2, generator=g, device="cuda")
+
+    def run(x):
+        order = moe.sort_tokens(ids, 4)
+        out = torch.empty(9, 40, dtype=x.dtype, device="cuda")
+        return (tiles(x), tiles(x, out=out), experts(x, order, gather=True), moe.to_experts(x, order),
+                moe.from_experts(experts(x, order, gather=True), order, w))
+    want = run(x)
+    with torch.inference_mode():
+        for t in (x, x.clone(), x.requires_grad_(False)):
+            got = run(t)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(a.is_inference() for a in got)
