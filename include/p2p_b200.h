@@ -358,8 +358,9 @@ size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols, int gated)
 
 /* y [tokens, rows] = x [tokens, cols] W^T of a module in the layout; gated: y [tokens, rows / 2] =
  * dtype(silu(gate) * up), from the fp32 sums. Each group's sum of exact code differences is multiplied by its scale in
- * fp32; no weight is rounded. Any tokens, rows and cols; x's rows start on 16-byte boundaries (ldx a multiple of 8). As the other GEMMs, a programmatic dependent of the stream's previous kernel that reads its weights
- * before that kernel completes. */
+ * fp32; no weight is rounded. Any tokens, rows and cols; x's rows start on 16-byte boundaries (ldx a multiple of 8). As
+ * the other GEMMs, a programmatic dependent of the stream's previous kernel that reads its weights before that kernel
+ * completes. */
 int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t ldx, const void* layout, int has_zeros,
                 int64_t rows, int group, int gated, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
                 void* stream);
@@ -369,10 +370,10 @@ int p2p_int4_mm(const void* x, int dtype, int64_t tokens, int64_t cols, int64_t 
  * place p is p itself, or with items of at most 8 places, where order is not null, order[p] / topk (x then has pairs / topk
  * rows). routed: null, or the number of routed pairs on the device: rows from there to
  * `pairs` become zero (null: they stay as they were). */
-int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout, int has_zeros, int64_t rows, int group, int gated, const int32_t* items,
-                     const int32_t* n_items, int64_t max_items, int64_t item_tokens, const int32_t* order, int topk,
-                     const int32_t* routed, int64_t pairs, void* y, int64_t ldy, void* workspace,
-                     size_t workspace_bytes, void* stream);
+int p2p_int4_grouped(const void* x, int dtype, int64_t cols, int64_t ldx, const void* layout, int has_zeros, int64_t rows,
+                     int group, int gated, const int32_t* items, const int32_t* n_items, int64_t max_items,
+                     int64_t item_tokens, const int32_t* order, int topk, const int32_t* routed, int64_t pairs, void* y,
+                     int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace p2p_int4_grouped needs, as p2p_int4_workspace. */
 size_t p2p_int4_grouped_workspace(int64_t max_items, int64_t item_tokens, int64_t rows, int64_t cols, int gated);
@@ -396,8 +397,8 @@ int p2p_int4_withhold(const void* x, int dtype, int64_t tokens, int64_t cols, in
  * order [n_pairs]: the routed pairs sorted by expert, those of one expert in their own order, then -1; where
  * [n_pairs]: each pair's place in it, or -1; offsets [experts + 1]: each expert's first place, the last one the number
  * of routed pairs; items [max_items, 4]: {expert, first place, places, 0}, runs of at most item_tokens (1..65536) places
- * of one expert, and n_items [1] their number. max_items >= min(n_pairs, ceil(n_pairs / item_tokens) + experts); at most 1024
- * experts. One launch, deterministic. */
+ * of one expert, and n_items [1] their number. max_items >= min(n_pairs, ceil(n_pairs / item_tokens) + experts); at most
+ * 1024 experts. One launch, deterministic. */
 int p2p_moe_sort(const void* ids, int ids_bytes, int64_t n_pairs, int experts, int32_t* order, int32_t* where,
                  int32_t* offsets, int32_t* items, int64_t max_items, int item_tokens, int32_t* n_items, void* stream);
 

@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
                 const uint32_t x_rows = p.order ? (uint32_t)t.n : (uint32_t)(NT * 8);
                 mbar_expect_tx(full(slot), n * (w_bytes + 2u * 128u * x_rows));
                 for (int i = 0; i < n; ++i)
-                    bulk_load(base + (2 * slot + i) * p.half_bytes, t.records + (int64_t)(k + i) * p.record, w_bytes, full(slot));
+                    bulk_load(base + (2 * slot + i) * p.half_bytes, t.records + (int64_t)(k + i) * p.record, w_bytes,
+                              full(slot));
             };
             int rows[8];                                             // x's rows of a tile that picks them, at most 8
             auto pick = [&](const SmallTile& t) {
@@ -491,7 +492,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                float* at = red + (c * 8 + token_of(2 * j + (i & 1))) * kRowPad + (blk + b) * 16 + n + 8 * (i >> 1);
+                                float* at = red + (c * 8 + token_of(2 * j + (i & 1))) * kRowPad + (blk + b) * 16 + n +
+                                            8 * (i >> 1);
                                 *at = h ? acc[b][c][i] : acc[b][c][i] + *at;
                             }
                 }
@@ -559,7 +561,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2) int4_small_kernel(const __gr
 
 // Row tiles that several runs share: their fp32 partials added in run order. A block takes a row tile, a warp a token at
 // a time, a thread four rows.
-template <typename T> __global__ void __launch_bounds__(256) int4_small_join_kernel(const __grid_constant__ SmallParams p, int ctas) {
+template <typename T>
+__global__ void __launch_bounds__(256) int4_small_join_kernel(const __grid_constant__ SmallParams p, int ctas) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // Every block waits, those without work too: this kernel's end stands for the end of the one before.
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -794,8 +797,14 @@ extern "C" int p2p_int4_layout(const uint8_t* codes, const void* scales, const u
 
 namespace {
 // Calls of up to this many tokens take the kernel above, which multiplies on the warps' own tensor path, so that nothing
-// changes hands; above, that path's rate binds. 28672 x 4096 (bf16, groups of 128): 33.8 us at 32 tokens here, 33.5 us at 33
-// on tcgen05, which takes the same at any smaller count.
+// changes hands; above, that path's rate binds. Both sides, us at 32 tokens here and at 33 on tcgen05, which takes the same
+// up to 48 (bf16; groups of 128, 64 and 32):
+//   28672 x 4096     34.4, 34.6    34.3, 48.2    38.3, 75.5
+//    6912 x 5120     18.2, 18.4    18.2, 22.2    19.4, 30.0    (zero points)
+//    4096 x 14336    20.7, 24.8    20.9, 31.5    23.2, 45.0
+//    1024 x 4096      8.4, 25.4     8.6, 22.4     8.4, 24.9
+// The switch is where the two meet for large modules with groups of 128. Below it tcgen05 never wins; above it, small
+// modules and finer groups would take two tiles of tokens here in less, which the kernel above does not cut.
 constexpr int64_t kSmallTokens = 32;
 
 int check_int4(const Int4Call& c, const char* what) {
@@ -820,7 +829,8 @@ extern "C" size_t p2p_int4_workspace(int64_t tokens, int64_t rows, int64_t cols,
 }
 
 extern "C" size_t p2p_int4_grouped_workspace(int64_t max_items, int64_t item_tokens, int64_t rows, int64_t cols, int gated) {
-    if (max_items <= 0 || item_tokens <= 0 || item_tokens > kSmallTokens || rows <= 0 || cols <= 0 || (gated && rows % 2)) return 0;
+    if (max_items <= 0 || item_tokens <= 0 || item_tokens > kSmallTokens || rows <= 0 || cols <= 0 || (gated && rows % 2))
+        return 0;
     Int4Call c = {};
     static const int32_t some = 0;
     c.items = &some; c.max_items = max_items; c.item_tokens = item_tokens;

@@ -1,5 +1,5 @@
-// (2d) The 4-bit product on tcgen05 tensor cores: y[t, r] = sum_c (code[r, c] - zero[r, g]) scale[r, g] x[t, c] for
-// every token count at which the streams below stay busy (int4.cu keeps the small calls), dense or for routed experts.
+// (2d) The 4-bit product on tcgen05 tensor cores: y[t, r] = sum_c (code[r, c] - zero[r, g]) scale[r, g] x[t, c] for more
+// than 32 tokens, or items of more than 32 places (int4.cu keeps the others and says why), dense or for routed experts.
 //
 // Scales stay out of the tensor cores: a group's sum of exact small integers times x goes to TMEM in fp32, and the
 // warps that read it out multiply it by the group's scale on the way into fp32 registers, so no weight is rounded (one
@@ -23,15 +23,17 @@
 //                       the even and the odd pieces: a look at a barrier costs an issuing thread 130 cycles even when it
 //                       has nothing to wait for
 //
-// Measured (bf16, groups of 128): 28672 x 4096 at 272 tokens 80 us replayed from a graph (798 TFLOP/s; the product alone
-// would take 39 us at the measured rate); 128 experts of 1536 x 2048 on 2048 x 8 tokens 238 us (433 TFLOP/s; items are
-// padded to 160 places). What binds is the way of a unit from hand to hand, with 130 to 220 cycles for each look at a
-// barrier, and the partials and their join: with products, read-out and building all left out 272 tokens still take 60 us of
-// 85. A unit takes some 3,100 and 2,500 cycles where its products are 1,088 and 640: the tensor pipe is busy 37 % and 21 %
-// of the time. Half of x's traffic (6 TB/s from L2) or twice the builders change nothing.
+// Measured (bf16, groups of 128): 28672 x 4096 at 272 tokens 88 us a call and 80 us replayed from a graph (724 and 794
+// TFLOP/s; the product alone would take 39 us at the measured rate); 128 experts of 1536 x 2048 on 2048 x 8 tokens 240 us
+// (429 TFLOP/s; items of up to 160 places, whose products are of their own places in steps of 16, their accumulators 160
+// columns apart). Groups of 32 take longer, a hand-over a group: 6913 x 5119 at 33 tokens 37 us, 4096 x 14336 at 40, 160 and
+// 272 tokens 45, 74 and 108. What binds is the way of a unit from hand to hand, with 130 to 220 cycles for each look at a
+// barrier, and the partials and their join: with products, read-out and building all left out of a copy, 272 tokens took 60
+// us of 85. A unit takes some 3,100 and 2,500 cycles where its products are 1,088 and 640: the tensor pipe is busy 37 % and
+// 21 % of the time. Half of x's traffic (6 TB/s from L2) or twice the builders change nothing.
 //
-// Every wait is bounded (2 s): a launch that gives up records where, issues nothing more, drains what it issued and
-// exits (p2p_int4_status reads the site).
+// Every wait is bounded (2 s, and a millisecond of tests before the clock is looked at): a launch that gives up records
+// where, issues nothing more, drains what it issued and exits (p2p_int4_status reads the site, p2p_int4_withhold tests it).
 #include <atomic>
 
 #include "int4.cuh"
@@ -57,7 +59,8 @@ constexpr int promote_regs(int acc) { return acc >= 96 ? 200 : acc >= 64 ? 136 :
 constexpr int kBuildRegs = 64;
 constexpr int other_regs(int acc) { return acc >= 96 ? 40 : 48; }
 constexpr int dealt_regs(int acc) {
-    return kPromoteWarps * 32 * promote_regs(acc) + build_groups(acc) * group_warps(acc) * 32 * kBuildRegs + 128 * other_regs(acc);
+    return kPromoteWarps * 32 * promote_regs(acc) + build_groups(acc) * group_warps(acc) * 32 * kBuildRegs +
+           128 * other_regs(acc);
 }
 constexpr int kWSlotBytes = q4::kCodeBytes + 512;       // codes and up to four groups' zero points
 constexpr int kSSlotBytes = 1024;                       // up to four groups' scales
@@ -175,7 +178,9 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int u, int u1) {
 // Pieces of the tokens, each a multiple of 16: halves up to 160 tokens, quarters above. (An accumulator that is read out
 // cannot take products: with four pieces three multiply meanwhile.)
 __host__ __device__ constexpr int n_total(int n) { return (n + 15) & ~15; }
-template <int PIECES> __device__ __forceinline__ int piece_size(int n, int i) { return (n_total(n) / 16 - i + PIECES - 1) / PIECES * 16; }
+template <int PIECES> __device__ __forceinline__ int piece_size(int n, int i) {
+    return (n_total(n) / 16 - i + PIECES - 1) / PIECES * 16;
+}
 template <int PIECES> __device__ __forceinline__ int piece_begin(int n, int i) {
     int at = 0;
 #pragma unroll
@@ -322,7 +327,8 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
 #pragma unroll
                     for (int s = 0; s < SUBS; ++s) {
                         if (s == 0) {
-                            if (!(ok = wait_three(afull(sa), pha, xfull(sx), phx, dempty(h, sb), phb ^ 1u, jobs >= NB, 5, wc))) return;
+                            if (!(ok = wait_three(afull(sa), pha, xfull(sx), phx, dempty(h, sb), phb ^ 1u, jobs >= NB, 5, wc)))
+                                return;
                         } else {
                             if (jobs >= NB && !(ok = wait_one(dempty(h, sb), phb ^ 1u, 7, wc))) return;
                         }
@@ -407,7 +413,8 @@ __global__ void __launch_bounds__(threads_of(W0 + W1), 1) int4_tc_kernel(const _
                         codes.expand(words[k], a);
                         r[4 * k] = a[0]; r[4 * k + 1] = a[2]; r[4 * k + 2] = a[1]; r[4 * k + 3] = a[3];
                     }
-                    tmem_st_16x256b_x4(tmem + ((uint32_t)(16 * blk) << 16) + (uint32_t)(p.a_col0 + sa * kACols + half * 32), r);
+                    const uint32_t col = (uint32_t)(p.a_col0 + sa * kACols + half * 32);
+                    tmem_st_16x256b_x4(tmem + ((uint32_t)(16 * blk) << 16) + col, r);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(wempty(sw));
@@ -669,7 +676,8 @@ TcPlan plan_tc(int most, bool routed) {
     pl.a_slots = (kTmemCols - pl.a_col0) / kACols;
     if (pl.a_slots > kMaxA) pl.a_slots = kMaxA;
     const int x_bytes = 2 * pl.x_rows * 128;
-    const int fixed = 1024 + kSSlots * kSSlotBytes + 8 * (2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * kMaxBuf * kMaxPieces + 2 * kSSlots + 1);
+    const int barriers = 2 * kMaxW + 2 * kMaxX + 2 * kMaxA + 2 * kMaxBuf * kMaxPieces + 2 * kSSlots + 1;
+    const int fixed = 1024 + kSSlots * kSSlotBytes + 8 * barriers;
     // eight units of weights in flight at least, then x, then as much again as is left for weights
     pl.x_slots = (kSmemLimit - fixed - 8 * kWSlotBytes) / x_bytes;
     if (pl.x_slots > kMaxX) pl.x_slots = kMaxX;
@@ -679,7 +687,8 @@ TcPlan plan_tc(int most, bool routed) {
     return pl;
 }
 
-template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
+template <typename T, int PIECES, int W0, int W1>
+int launch_tc(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
     auto kernel = int4_tc_kernel<T, PIECES, W0, W1>;
     constexpr int kThreads = threads_of(W0 + W1);
     if (int e = allow_smem((const void*)kernel, smem, what)) return e;
@@ -692,7 +701,8 @@ template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMa
             regs = a.numRegs;
         }
         if (regs * kThreads < dealt_regs(W0 + W1))
-            return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread for %d in all", what, regs.load(), dealt_regs(W0 + W1));
+            return fail(P2P_EUNSUPPORTED, "%s: built with %d registers a thread for %d in all", what, regs.load(),
+                        dealt_regs(W0 + W1));
     }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -714,7 +724,8 @@ template <typename T, int PIECES, int W0, int W1> int launch_tc(const CUtensorMa
     return launch_status(what);
 }
 
-template <typename T> int launch_width(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
+template <typename T>
+int launch_width(const CUtensorMap& map, const TcParams& p, int smem, cudaStream_t st, const char* what) {
     if (p.n_max <= 64) return launch_tc<T, 2, 32, 0>(map, p, smem, st, what);
     if (p.n_max <= 128) return launch_tc<T, 2, 64, 0>(map, p, smem, st, what);
     if (p.n_max <= 160) return launch_tc<T, 2, 80, 0>(map, p, smem, st, what);

@@ -121,7 +121,7 @@ class TokenOrder:
     order: torch.Tensor           # int32 [T K]: the pair token * K + slot at each place, -1 behind the last
     where: torch.Tensor           # int32 [T K]: each pair's place, -1 if it is routed nowhere
     offsets: torch.Tensor         # int32 [experts + 1]: each expert's first place, then the number of routed pairs
-    items: torch.Tensor           # int32 [.., 4]: {expert, first place, places, 0}, runs of one expert's places
+    items: torch.Tensor           # int32 [4 n]: n of {expert, first place, places, 0}, runs of one expert's places
     n_items: torch.Tensor         # int32 [1]
     tokens: int
     topk: int
@@ -237,8 +237,8 @@ class Int4Experts:
 
 class GroupedMoE(torch.nn.Module):
     """A FusedMoE's quant_method for compact routed experts, gated SiLU: weights {"w13_weight": blocks of [E, 2R, H]
-    (gate rows, then up rows), "w2_weight": blocks of [E, H, R]}, all of them 4-bit blocks or none. apply(layer, dispatch_output) returns the layer's
-    output [T, H] in x's dtype. Other attributes are the layer's own method's."""
+    (gate rows, then up rows), "w2_weight": blocks of [E, H, R]}, all of them 4-bit blocks or none. apply(layer,
+    dispatch_output) returns the layer's output [T, H] in x's dtype. Other attributes are the layer's own method's."""
 
     is_int4 = False                 # also of layers pickled before there were 4-bit blocks
 
@@ -281,7 +281,7 @@ class GroupedMoE(torch.nn.Module):
         x2 = x.reshape(-1, x.shape[-1])
         if x2.dtype != self.w13.dtype:
             raise P2PError(f"x is {x2.dtype}, the experts {self.w13.dtype}")
-        if self.is_int4:                            # four launches, no read back: the pass can be captured
+        if self.is_int4:                            # four to seven launches, no read back: the pass can be captured
             order = sort_tokens(ids if ids.dtype in (torch.int32, torch.int64) else ids.long(), self.w13.experts)
             down = self.w2(self.w13(x2, order, gather=True), order)
             return from_experts(down, order, weights).reshape(*x.shape[:-1], self.w2.rows)

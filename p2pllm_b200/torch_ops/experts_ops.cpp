@@ -1,6 +1,7 @@
 // The 4-bit products and the token shuffle around routed experts as torch custom operators (namespace p2p_b200). The
-// products are for inference: an x that needs a gradient is refused. The shuffle's two directions are differentiable;
-// their gradients are the library's own kernels, one level deep (second derivatives of the weighted sum are refused).
+// products are for inference: an x that is differentiated, in either mode, is refused. The shuffle's two directions are
+// differentiable in reverse mode; their gradients are the library's own kernels, one level deep (second derivatives of the
+// weighted sum are refused, and inputs with a forward-mode tangent).
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <algorithm>
@@ -12,14 +13,24 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr int64_t kSmallTokens = 8;                   // items of up to here pick x's rows by the order
+constexpr int64_t kPickTokens = 8;                    // items of up to here pick x's rows by the order
 
 // Places of one item, what one pass over an expert's weights takes: somewhat more than experts have on average, so that
-// few take two passes and no tile is mostly empty; at most what leaves the accumulators room. (128 experts of 1536 x 2048
-// with 128 pairs each on average: 255 us in items of 160 places, x's rows picked once a tile; 303 us of 256 before.)
+// few take two passes and no tile is mostly empty; at most what leaves the accumulators room. Both sides of every step, us
+// of the product alone at a mean number of pairs (128 experts, ids evenly drawn; 1536 x 2048 gated, bf16, groups of 128 |
+// 2048 x 768, f16, groups of 32, zero points):
+//   mean   4: items of   8:  56 |  40, of  16:  58 |  44      mean   5: of   8:  60 |  45, of  16:  62 |  48
+//   mean  10: items of  16:  67 |  51, of  32:  81 |  61      mean  12: of  16:  70 |  54, of  32:  85 |  63
+//   mean  24: items of  32: 113 |  80, of  64: 124 | 139      mean  26: of  32: 116 |  81, of  64: 123 | 138
+//   mean  48: items of  64: 130 | 142, of 128: 158 | 180      mean  52: of  64: 141 | 153, of 128: 176 | 198
+//   mean 100: items of 128: 201 | 226, of 160: 203 | 228      mean 118: of 128: 238 | 273, of 160: 225 | 254
+//   mean 130: items of 160: 227 | 255, of 256: 262 | 326      mean 134: of 160: 226 | 256, of 256: 261 | 327
+//                                                             mean 200: of 160: 384 | 454, of 256: 311 | 387
+// The smaller size holds on a little past most steps (to a mean of 5, 12, 26, 52, 104 and between 134 and 160); with skewed
+// ids some experts are past theirs, and the steps are early for them.
 int64_t item_tokens(int64_t pairs, int64_t experts) {
     const double mean = (double)pairs / experts;
-    if (pairs <= kSmallTokens || mean <= 4) return kSmallTokens;
+    if (pairs <= kPickTokens || mean <= 4) return kPickTokens;
     return mean <= 10 ? 16 : mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 100 ? 128 : mean <= 130 ? 160 : 256;
 }
 
@@ -55,8 +66,8 @@ at::Tensor moe_spread(const at::Tensor& x_in, const at::Tensor& where, const at:
 
 // ---- 4-bit products --------------------------------------------------------------------------------------------------
 
-void check_int4(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols, int64_t group,
-                bool gated) {
+void check_int4(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t experts, int64_t rows, int64_t cols,
+                int64_t group, bool gated) {
     check_matrix(x, "x");
     TORCH_CHECK(x.size(1) == cols, "p2p_b200: x of ", x.sizes(), " does not have ", cols, " columns");
     TORCH_CHECK(group == 32 || group == 64 || group == 128, "p2p_b200: groups of ", group, " columns, not 32, 64 or 128");
@@ -114,12 +125,12 @@ void int4_grouped_run(const at::Tensor& x_in, const at::Tensor& layout, bool zer
     if (pairs == 0) return;
     const int64_t most = item_tokens(pairs, experts);
     // few pairs: the product picks x's rows itself
-    const bool pick = gather && most <= kSmallTokens;
+    const bool pick = gather && most <= kPickTokens;
     const at::Tensor x = aligned_rows(gather && !pick ? moe_spread(x_in, where, offsets, topk) : x_in);
     const size_t need = p2p_int4_grouped_workspace(items.numel() / 4, most, rows, cols, gated);
     const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte)) : at::Tensor();
-    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, aligned_stride(x), layout.data_ptr(), zeros, rows, (int)group, gated, ints(items, x, 0, "items"),
-                           ints(n_items, x, 1, "n_items"), items.numel() / 4, most,
+    check(p2p_int4_grouped(x.data_ptr(), dtype_code(x), cols, aligned_stride(x), layout.data_ptr(), zeros, rows, (int)group,
+                           gated, ints(items, x, 0, "items"), ints(n_items, x, 1, "n_items"), items.numel() / 4, most,
                            pick ? at_order : nullptr, (int)topk, zero_behind ? at_offsets + experts : nullptr, pairs,
                            out.data_ptr(), row_stride(out), need ? ws.data_ptr() : nullptr, need, stream_of(x)),
           "p2p_int4_grouped");
@@ -334,10 +345,12 @@ void check_inference(const at::Tensor& x) {
 }
 void check_inference(const at::Tensor& x, const at::Tensor& out) {
     check_inference(x);
-    TORCH_CHECK(!needs_grad(out) && !has_tangent(out), "p2p_b200: 4-bit weights are for inference: out must not need a gradient");
+    TORCH_CHECK(!needs_grad(out) && !has_tangent(out),
+                "p2p_b200: 4-bit weights are for inference: out must not need a gradient");
 }
 
-at::Tensor int4_mm_grad(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t rows, int64_t cols, int64_t group, bool gated) {
+at::Tensor int4_mm_grad(const at::Tensor& x, const at::Tensor& layout, bool zeros, int64_t rows, int64_t cols,
+                        int64_t group, bool gated) {
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("p2p_b200::int4_mm", "").typed<decltype(int4_mm)>();
     check_inference(x);
     at::AutoDispatchBelowADInplaceOrView below;
@@ -375,12 +388,14 @@ at::Tensor int4_mm_meta(const at::Tensor& x, const at::Tensor&, bool, int64_t ro
     return at::empty({x.size(0), gated ? rows / 2 : rows}, x.options());
 }
 void int4_mm_into_meta(const at::Tensor&, const at::Tensor&, bool, int64_t, int64_t, int64_t, bool, const at::Tensor&) {}
-at::Tensor int4_grouped_meta(const at::Tensor& x, const at::Tensor&, bool, int64_t, int64_t rows, int64_t, int64_t, bool gated, const at::Tensor& order,
-                             const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool) {
+at::Tensor int4_grouped_meta(const at::Tensor& x, const at::Tensor&, bool, int64_t, int64_t rows, int64_t, int64_t,
+                             bool gated, const at::Tensor& order, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, const at::Tensor&, int64_t, bool) {
     return at::empty({order.numel(), gated ? rows / 2 : rows}, x.options());
 }
-void int4_grouped_into_meta(const at::Tensor&, const at::Tensor&, bool, int64_t, int64_t, int64_t, int64_t, bool, const at::Tensor&, const at::Tensor&,
-                            const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool, const at::Tensor&) {}
+void int4_grouped_into_meta(const at::Tensor&, const at::Tensor&, bool, int64_t, int64_t, int64_t, int64_t, bool,
+                            const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const at::Tensor&, int64_t, bool, const at::Tensor&) {}
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort_meta(const at::Tensor& ids, int64_t experts) {
     const auto o = ids.options().dtype(at::kInt);
     const int64_t n = ids.numel();
